@@ -683,6 +683,95 @@ walsh_status walsh_linear_split_fwd(const void* x, int x_dtype, int64_t M, int K
 walsh_status walsh_rmsnorm(const void* x, int dtype, int64_t rows, int C, const float* w,
                            float eps, void* y, int y_dtype, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Serving: paged key/value cache and token sampling
+ * No counterparts in the reference, whose cache holds one sequence
+ * (src/model/chassis.py:262-330) and whose sampling is temperature and top-k
+ * (src/model/mhc.py:767-782).
+ * ------------------------------------------------------------------------- */
+
+/* One layer of a paged key/value cache.  Element (page, head, slot, d) of
+ * k_pages / v_pages is at page * page_stride + head * head_stride + slot *
+ * row_stride + d (strides in elements, the same for both; multiples of 16
+ * bytes; hd contiguous elements; hd in {16, 32, 64, 128}).  A dense cache
+ * [B, H, ctx, hd] is one of B pages of ctx slots.
+ * Key j of sequence b lies in slot j % page_size of page page_table[b][j /
+ * page_size].  Entries behind a sequence's last page, and of pages no key of
+ * which is seen, are not read.  kv_lens[b] counts the keys of sequence b, the
+ * newest included.
+ * window > 0: a token at position p sees the keys p - window + 1 .. p and the
+ * first `sinks` keys; window = 0: all keys up to p.
+ * err (may be null): receives WALSH_ERR_INDEX when a kernel meets a page id, a
+ * slot, a position, a length or an offset out of range; the access is skipped
+ * (keys of such a page count as not seen). */
+typedef struct {
+  void* k_pages;
+  void* v_pages;
+  int dtype;
+  int n_pages, kv_heads, page_size, head_dim;
+  int64_t page_stride, head_stride, row_stride;
+  const int32_t* page_table; /* [B, table_cols], rows table_stride apart */
+  int64_t table_stride;
+  int table_cols;
+  const int32_t* kv_lens; /* [B] */
+  int window, sinks;
+  float scale; /* of the scores; > 0 */
+  int32_t* err;
+} walsh_paged_kv;
+
+/* Appends ntok tokens: k, v [ntok, kv_heads, hd] (token and head strides
+ * *_ts, *_hs in elements) go to slots[i] = page * page_size + slot of the
+ * pages (a negative slot is not stored: padding), after an RMS norm of each
+ * head of k (k_norm [hd], null for none) and the rotation of its pairs (2i,
+ * 2i+1) by rope_cos / rope_sin [n_pos, hd/2] at positions[i] (positions null:
+ * no rotation; the pairing of src/model/chassis.py:339-345).  q [ntok,
+ * q_heads, hd] (null: none) is normed by q_norm and rotated the same way into
+ * q_out [ntok, q_heads, hd]; its rows at a position out of range become zero.
+ * Slots are distinct: of two tokens for one slot either may be stored.  slots
+ * and positions are int64 when idx64, else int32.  Uses the pages, n_pages,
+ * strides and err of kv; its table and lengths may be null. */
+walsh_status walsh_paged_append(const walsh_paged_kv* kv, const void* q, int64_t q_ts, int64_t q_hs, const void* k,
+                                int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts, int64_t v_hs, int64_t ntok,
+                                int q_heads, const void* slots, const void* positions, int idx64,
+                                const float* rope_cos, const float* rope_sin, int64_t n_pos, const float* q_norm,
+                                const float* k_norm, float eps, void* q_out, void* stream);
+
+/* Attention of each sequence's newest token (position kv_lens[b] - 1, already
+ * appended): q [B, q_heads, hd] with strides q_bs, q_hs -> o [B, q_heads, hd].
+ * q_heads is a multiple of kv_heads; head h reads key/value head h / (q_heads
+ * / kv_heads).  A sequence of length 0 gives zeros.  max_len: an upper bound
+ * of kv_lens the work is cut by (a longer sequence is still computed whole).
+ * scratch: walsh_paged_attn_scratch_bytes (-1 for rejected arguments) for the
+ * same description, used by this call alone; null when that is 0. */
+int64_t walsh_paged_attn_scratch_bytes(const walsh_paged_kv* kv, int B, int q_heads, int max_len);
+walsh_status walsh_paged_attn_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_bs, int64_t q_hs, int B,
+                                  int q_heads, int max_len, void* scratch, void* o, void* stream);
+
+/* Attention of several new tokens per sequence: rows q_offsets[b] ..
+ * q_offsets[b+1]-1 of q [q_rows, q_heads, hd] are the last tokens of sequence
+ * b, already appended; o [q_rows, q_heads, hd].  Rows outside every span are
+ * left as they are; a token that sees no key gives zeros.  max_q: an upper
+ * bound of the spans the grid is sized by (longer spans are still computed). */
+walsh_status walsh_paged_prefill_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts, int64_t q_hs,
+                                     int64_t q_rows, const int32_t* q_offsets, int B, int q_heads, int max_q, void* o,
+                                     void* stream);
+
+/* One token per row of logits [rows, vocab] (rows ld elements apart; vocab <=
+ * 2^18) from the uniform numbers u [rows] in [0, 1): weights exp(l / T); the
+ * top_k largest (<= 0: all; ties to the lower index); of those the smallest
+ * leading part whose mass reaches top_p of theirs (>= 1: all); of those the
+ * weights of at least min_p times the largest (<= 0: all).  The draw is the
+ * first token in index order whose running mass exceeds u times the mass of
+ * the kept tokens.  T = 0: the largest logit.  NaN logits count as -inf; with
+ * +inf logits only these have weight; a row without a finite or +inf logit
+ * gives -1.  Each parameter is one value for all rows, or per row where its
+ * *_rows pointer is given (a T that is not > 0 draws the largest logit).
+ * logp (may be null): log probability of the drawn token among the kept. */
+walsh_status walsh_sample_tokens(const void* logits, int dtype, int64_t ld, int64_t rows, int vocab, const float* u,
+                                 double temperature, int top_k, double top_p, double min_p,
+                                 const float* temperature_rows, const int32_t* top_k_rows, const float* top_p_rows,
+                                 const float* min_p_rows, int64_t* ids, float* logp, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -84,13 +84,22 @@ SIGNATURES = {
     "walsh_hadamard_linear_dense_weights": [P, P, P, c_int, c_int, P, P, P],
     "walsh_hadamard_linear_dense_fwd": [P, c_int, c_int64, c_int, P, P, P, P],
     "walsh_hlin_pk_error": [c_int],
+    "walsh_paged_append": [P, P, c_int64, c_int64, P, c_int64, c_int64, P, c_int64, c_int64, c_int64, c_int, P, P,
+                           c_int, P, P, c_int64, P, P, c_float, P, P],
+    "walsh_paged_attn_fwd": [P, P, c_int64, c_int64, c_int, c_int, c_int, P, P, P],
+    "walsh_paged_attn_scratch_bytes": [P, c_int, c_int, c_int],
+    "walsh_paged_prefill_fwd": [P, P, c_int64, c_int64, c_int64, P, c_int, c_int, c_int, P, P],
+    "walsh_sample_tokens": [P, c_int, c_int64, c_int64, c_int, P, ctypes.c_double, c_int, ctypes.c_double,
+                            ctypes.c_double, P, P, P, P, P, P, P],
 }
 _RESTYPE = {"walsh_status_str": ctypes.c_char_p, "walsh_ipc_handle_bytes": c_int, "walsh_chmod_mlp_tc_scratch_bytes": ctypes.c_int64,
-            "walsh_linear_split_tc_scratch_bytes": ctypes.c_int64}
+            "walsh_linear_split_tc_scratch_bytes": ctypes.c_int64,
+            "walsh_paged_attn_scratch_bytes": ctypes.c_int64}
 # kernels each entry point launches (for the launch accounting reported by bench.py)
 KERNELS_PER_CALL = {"walsh_ternary_quantize_pack": 2, "walsh_chmod_fwd_noalloc": 3, "walsh_octo_set_mainloop": 0, "walsh_octo_set_narrow": 0, "walsh_octo_set_tma_store": 0,
                     "walsh_chmod_mlp_tc": 3, "walsh_chmod_mlp_tc_scratch_bytes": 0,
                     "walsh_linear_split_tc_fwd": 2, "walsh_linear_split_tc_scratch_bytes": 0,
+                    "walsh_paged_attn_scratch_bytes": 0,
                     "walsh_tc05_error": 0, "walsh_attn_set_path": 0, "walsh_map_error": 0, "walsh_map_set_pipe": 0, "walsh_hlin_pk_error": 0, "walsh_chmod_chunk_rows": 0, "walsh_status_str": 0,
                     "walsh_abi_version": 0, "walsh_ipc_handle": 0, "walsh_ipc_open": 0, "walsh_ipc_close": 0,
                     "walsh_ipc_handle_bytes": 0}
@@ -111,6 +120,14 @@ ROUTE_TOPK, ROUTE_THRESHOLD = 0, 1
 class MoeRouting(ctypes.Structure):
     """walsh_moe_routing: the expert-selection rule (NULL = the reference's top-k)."""
     _fields_ = [("mode", c_int), ("min_experts", c_int), ("threshold", c_float)]
+
+
+class PagedKV(ctypes.Structure):
+    """walsh_paged_kv: one layer of a paged key/value cache."""
+    _fields_ = [("k_pages", P), ("v_pages", P), ("dtype", c_int), ("n_pages", c_int), ("kv_heads", c_int),
+                ("page_size", c_int), ("head_dim", c_int), ("page_stride", c_int64), ("head_stride", c_int64),
+                ("row_stride", c_int64), ("page_table", P), ("table_stride", c_int64), ("table_cols", c_int),
+                ("kv_lens", P), ("window", c_int), ("sinks", c_int), ("scale", c_float), ("err", P)]
 
 
 class WalshError(RuntimeError):

@@ -572,3 +572,237 @@ def rmsnorm(x, w, eps=1e-6, out_dtype=None):
     call("walsh_rmsnorm", ptr(x), dcode(x.dtype), x.numel() // C, C, ptr(w), float(eps), ptr(y), dcode(out_dtype),
          stream())
     return y
+
+
+# ---------------------------------------------------------------------------
+# serving: paged key/value cache and token sampling
+# ---------------------------------------------------------------------------
+
+def _call_on(t, name, *args):
+    """call(name, *args, stream) on t's device and its current stream."""
+    if t.device.index == torch._C._cuda_getDevice():
+        return call(name, *args, stream())
+    with torch.cuda.device(t.device):
+        return call(name, *args, stream())
+
+
+def _same_device(first, *tensors):
+    require_cuda(first, *tensors)
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+
+
+def _head_rows(x, heads, hd, dtype, what):
+    """x [N, heads, hd] and its token and head strides, copied when a row is
+    not contiguous or not on 16-byte boundaries."""
+    if x.dim() != 3 or x.shape[2] != hd or (heads is not None and x.shape[1] != heads):
+        raise ValueError(f"{what} has shape {tuple(x.shape)}; expected [N, {heads or 'heads'}, {hd}]")
+    if x.dtype != dtype:
+        raise ValueError(f"{what} is {x.dtype}; the pages are {dtype}")
+    vec = 16 // x.element_size()
+    n, h, _ = x.shape
+    st, sh, sd = x.stride()
+    if sd != 1 or (st % vec and n > 1) or (sh % vec and h > 1):
+        x = x.contiguous()
+        st, sh, sd = x.stride()
+    if x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+        st, sh, sd = x.stride()
+    return x, (st if n > 1 else 0), (sh if h > 1 else 0)
+
+
+def _index_vector(x, n, what, dtypes=(torch.int32,)):
+    if x.dtype not in dtypes or x.dim() != 1 or x.shape[0] != n:
+        raise ValueError(f"{what} must be {' or '.join(str(d)[6:] for d in dtypes)} [{n}], got {x.dtype} {tuple(x.shape)}")
+    return _c(x)
+
+
+def _out_rows(out, like, shape):
+    if out is None:
+        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if out.shape != shape or out.dtype != like.dtype or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {like.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
+    return out
+
+
+def _paged_kv(k_pages, v_pages, page_table=None, kv_lens=None, window=0, sinks=0, scale=None, err=None):
+    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+        raise ValueError(f"k_pages and v_pages must be alike [n_pages, kv_heads, page_size, hd], got "
+                         f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
+    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        raise ValueError("k_pages and v_pages must have the same strides and contiguous rows")
+    n, h, ps, hd = k_pages.shape
+    sp, sh, sr, _ = k_pages.stride()
+    kv = _lib.PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), dcode(k_pages.dtype), n, h, ps, hd,
+                      sp if n > 1 else 0, sh if h > 1 else 0, sr if ps > 1 else hd)
+    if err is not None:
+        if err.dtype != torch.int32 or err.numel() != 1:
+            raise ValueError("err must be one int32")
+        kv.err = err.data_ptr()
+    if page_table is not None:
+        if page_table.dtype != torch.int32 or page_table.dim() != 2 or (page_table.shape[1] > 1
+                                                                       and page_table.stride(1) != 1):
+            raise ValueError(f"page_table must be int32 [B, columns] with contiguous rows, got {page_table.dtype} "
+                             f"{tuple(page_table.shape)}")
+        if window < 0 or sinks < 0:
+            raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
+        kv.page_table = page_table.data_ptr()
+        kv.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else 0
+        kv.table_cols = page_table.shape[1]
+        kv.kv_lens = kv_lens.data_ptr()
+        kv.window, kv.sinks = int(window), int(sinks)
+        kv.scale = hd ** -0.5 if scale is None else float(scale)
+    return kv
+
+
+def paged_append(q, k, v, k_pages, v_pages, slots, positions=None, rope=None, q_norm=None, k_norm=None, eps=1e-6,
+                 q_out=None, err=None):
+    """Append tokens to a paged cache.  k, v [N, Hkv, hd] go to ``slots`` (int
+    [N], page * page_size + slot; negative: not stored) of k_pages, v_pages
+    [n_pages, Hkv, page_size, hd], k after an RMS norm over each head (k_norm
+    [hd] or None) and the rotation of its pairs (2i, 2i+1) at ``positions``
+    (int [N]; ``rope`` = (cos, sin) float32 [n_pos, hd/2]).  q [N, Hq, hd]
+    (or None) is normed by q_norm and rotated the same way; returns it as a
+    new [N, Hq, hd] (or None).  q, k, v may be strided views (of a fused
+    q|k|v, or head-major).  Slots must be distinct.  ``err`` (int32 [1])
+    becomes nonzero when a slot or position is out of range; such a token is
+    not stored and its q_out row is zero (for a position).  One launch."""
+    _same_device(k_pages, v_pages, q, k, v, slots, positions, q_norm, k_norm, q_out, err)
+    kv = _paged_kv(k_pages, v_pages, err=err)
+    hk, hd, dt = k_pages.shape[1], k_pages.shape[3], k_pages.dtype
+    k, k_ts, k_hs = _head_rows(k, hk, hd, dt, "k")
+    v, v_ts, v_hs = _head_rows(v, hk, hd, dt, "v")
+    n = k.shape[0]
+    hq = q_ts = q_hs = 0
+    if q is not None:
+        q, q_ts, q_hs = _head_rows(q, None, hd, dt, "q")
+        hq = q.shape[1]
+        q_out = _out_rows(q_out, q, (n, hq, hd))
+    elif q_out is not None or q_norm is not None:
+        raise ValueError("q_out and q_norm need q")
+    if v.shape[0] != n or (q is not None and q.shape[0] != n):
+        raise ValueError("q, k and v must have the same number of tokens")
+    slots = _index_vector(slots, n, "slots", (torch.int32, torch.int64))
+    cos = sin = None
+    if (positions is None) != (rope is None):
+        raise ValueError("positions and rope go together")
+    if positions is not None:
+        positions = _index_vector(positions, n, "positions", (torch.int32, torch.int64))
+        if positions.dtype != slots.dtype:
+            positions = positions.to(slots.dtype)
+        cos, sin = rope
+        _same_device(k_pages, cos, sin)
+        if (cos.dim() != 2 or cos.shape[1] != hd // 2 or cos.shape != sin.shape or cos.dtype != torch.float32
+                or sin.dtype != torch.float32):
+            raise ValueError(f"rope must be two float32 [n_pos, {hd // 2}] tables")
+        cos, sin = _c(cos), _c(sin)
+    for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (hd,) or not w.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous float32 [{hd}]")
+    if n == 0:
+        return q_out
+    _call_on(k_pages, "walsh_paged_append", ctypes.byref(kv), ptr(q), q_ts, q_hs, ptr(k), k_ts, k_hs, ptr(v), v_ts,
+             v_hs, n, hq, ptr(slots), ptr(positions), 1 if slots.dtype == torch.int64 else 0, ptr(cos), ptr(sin),
+             0 if cos is None else cos.shape[0], ptr(q_norm), ptr(k_norm), float(eps), ptr(q_out))
+    return q_out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, window=0, sinks=0, scale=None, out=None,
+                    err=None):
+    """Attention of each sequence's newest token over its pages: q [B, Hq, hd]
+    -> [B, Hq, hd].  ``page_table`` int32 [B, columns] lists each sequence's
+    pages in order, ``kv_lens`` int32 [B] its keys, the newest (already
+    appended) included; Hq is a multiple of the pages' heads.  ``window`` > 0
+    limits a token to the last ``window`` keys and the first ``sinks``; scores
+    are scaled by ``scale`` (default hd^-0.5).  ``max_len`` bounds kv_lens on
+    the host (default: what the table holds) and decides how the work is cut.
+    Sequences of length 0 give zeros.  ``err`` (int32 [1]) becomes nonzero
+    when a page id or length is out of range; keys of such a page are not
+    seen."""
+    _same_device(k_pages, v_pages, q, page_table, kv_lens, out, err)
+    kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
+    q, q_bs, q_hs = _head_rows(q, None, k_pages.shape[3], k_pages.dtype, "q")
+    B, hq, _ = q.shape
+    _index_vector(kv_lens, B, "kv_lens")
+    if page_table.shape[0] != B or not kv_lens.is_contiguous():
+        raise ValueError(f"{B} queries, a page table of {page_table.shape[0]} rows and kv_lens of stride "
+                         f"{kv_lens.stride(0)}")
+    out = _out_rows(out, q, q.shape)
+    if B == 0:
+        return out
+    if max_len is None:
+        max_len = page_table.shape[1] * k_pages.shape[2]
+    nbytes = call("walsh_paged_attn_scratch_bytes", ctypes.byref(kv), B, hq, int(max_len))
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
+    _call_on(q, "walsh_paged_attn_fwd", ctypes.byref(kv), ptr(q), q_bs, q_hs, B, hq, int(max_len), ptr(scratch),
+             ptr(out))
+    return out
+
+
+def paged_prefill_attention(q, q_offsets, k_pages, v_pages, page_table, kv_lens, max_q=None, window=0, sinks=0,
+                            scale=None, out=None, err=None):
+    """Causal attention of several new tokens per sequence over its pages: rows
+    q_offsets[b] .. q_offsets[b+1]-1 (int32 [B+1]) of q [N, Hq, hd] are the
+    last tokens of sequence b, already appended (query t of T at position
+    kv_len - T + t).  Pages, lengths, window, sinks, scale and err as in
+    paged_attention; ``max_q`` bounds the spans on the host (default N).  Rows
+    of ``out`` outside every span are left as they are."""
+    _same_device(k_pages, v_pages, q, q_offsets, page_table, kv_lens, out, err)
+    kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
+    q, q_ts, q_hs = _head_rows(q, None, k_pages.shape[3], k_pages.dtype, "q")
+    n, hq, _ = q.shape
+    B = page_table.shape[0]
+    _index_vector(kv_lens, B, "kv_lens")
+    q_offsets = _index_vector(q_offsets, B + 1, "q_offsets")
+    if not kv_lens.is_contiguous():
+        raise ValueError("kv_lens must be contiguous")
+    out = _out_rows(out, q, q.shape)
+    if n == 0 or B == 0:
+        return out
+    _call_on(q, "walsh_paged_prefill_fwd", ctypes.byref(kv), ptr(q), q_ts, q_hs, n, ptr(q_offsets), B, hq,
+             n if max_q is None else min(int(max_q), n), ptr(out))
+    return out
+
+
+def _row_param(x, rows, dtype, what):
+    """(scalar, tensor or None) of a sampling parameter given for all rows or per row."""
+    if not isinstance(x, torch.Tensor):
+        return x, None
+    if x.dtype != dtype or x.shape != (rows,):
+        raise ValueError(f"{what} must be a number or {str(dtype)[6:]} [{rows}], got {x.dtype} {tuple(x.shape)}")
+    return 0, _c(x)
+
+
+def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, want_logprob=False):
+    """One token per row of logits [B, V] (float32, bfloat16 or float16; V <=
+    2^18) from ``uniforms`` (float32 [B] in [0, 1)): softmax of logits /
+    temperature, restricted to the ``top_k`` largest (0: all; ties to the lower
+    index), then to the smallest leading part with mass >= ``top_p`` (>= 1:
+    all), then to weights of at least ``min_p`` times the largest, and drawn in
+    index order (the first token whose running mass exceeds u times the kept
+    mass).  temperature 0 takes the largest logit.  Each parameter is a number
+    or one value per row (float32; top_k int32).  Returns int64 [B] (-1 for a
+    row with no finite logit), with ``want_logprob`` also the float32 log
+    probability of the draw among the kept tokens."""
+    if logits.dim() != 2:
+        raise ValueError(f"logits must be [B, V], got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    tv, tr = _row_param(temperature, rows, torch.float32, "temperature")
+    kv, kr = _row_param(top_k, rows, torch.int32, "top_k")
+    pv, pr = _row_param(top_p, rows, torch.float32, "top_p")
+    mv, mr = _row_param(min_p, rows, torch.float32, "min_p")
+    _same_device(logits, uniforms, tr, kr, pr, mr)
+    if not tv >= 0 or pv != pv or mv != mv:
+        raise ValueError(f"temperature must be >= 0 and top_p, min_p numbers, got {tv}, {pv}, {mv}")
+    if uniforms.dtype != torch.float32 or uniforms.shape != (rows,):
+        raise ValueError(f"uniforms must be float32 [{rows}], got {uniforms.dtype} {tuple(uniforms.shape)}")
+    if vocab > 1 and logits.stride(1) != 1:
+        logits = logits.contiguous()
+    uniforms = _c(uniforms)
+    ids = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if want_logprob else None
+    _call_on(logits, "walsh_sample_tokens", ptr(logits), dcode(logits.dtype), logits.stride(0) if rows > 1 else 0,
+             rows, vocab, ptr(uniforms), float(tv), max(0, min(int(kv), vocab)), float(pv), float(mv), ptr(tr), ptr(kr),
+             ptr(pr), ptr(mr), ptr(ids), ptr(logp))
+    return (ids, logp) if want_logprob else ids
