@@ -331,6 +331,37 @@ def test_prefill_more_queries_than_keys_and_bad_offsets():
     close(out[2:5], want, bound)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hk,hd", LAYOUTS)
+def test_prefill_hidden_values_that_are_not_finite(dtype, hq, hk, hd):
+    """A key or value that is infinite or NaN reaches the tokens that see it and no others."""
+    g = gen(14)
+    n, window, sinks = 90, 20, 2
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [n], hk, 16, hd, dtype))
+    q = torch.randn(n, hq, hd, generator=g).to(dtype).to(DEV)
+    off = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    clean = ops.paged_prefill_attention(q, off, kp, vp, table, kl, window=window, sinks=sinks)
+
+    def at(j):
+        return int(table[0, j // 16]), j % 16
+
+    for j, value in ((40, float("nan")), (61, float("inf")), (77, float("-inf"))):
+        vp[at(j)[0], :, at(j)[1]] = value
+    kp[at(30)[0], :, at(30)[1]] = float("nan")
+    o = ops.paged_prefill_attention(q, off, kp, vp, table, kl, window=window, sinks=sinks)
+    t = torch.arange(n, device=DEV)
+    sees = lambda j: (t >= j) & (t < j + window)  # noqa: E731
+    touched = sees(40) | sees(61) | sees(77) | sees(30)
+    assert not torch.isfinite(o[touched].float()).any()
+    # rows computed once more add in another order: one rounding of the result and
+    # of the probabilities each way
+    d = (o[~touched].double() - clean[~touched].double()).abs()
+    k, v = R.gather_keys(kp, table[0], n), R.gather_keys(vp, table[0], n)
+    k, v = torch.where(torch.isfinite(k), k, 0), torch.where(torch.isfinite(v), v, 0)
+    _, bound = R.attend(q, k, v, 0, window, sinks)
+    assert (d <= 2 * bound[~touched]).all()
+
+
 # ---------------------------------------------------------------------------
 # use: streams, graphs, repeatability
 # ---------------------------------------------------------------------------

@@ -40,7 +40,53 @@ __device__ __forceinline__ int query_span(const PrefillArgs<T>& a, int b, int64_
   return (int)(q1 - q0);
 }
 
-// CUDA-core form: 64 rows x 32 keys a step, 256 threads; a half warp owns four
+// One row again by one warp, over the keys it sees and no others.  A tile
+// multiplies hidden keys by a probability of 0, which is no use when the value
+// is infinite or NaN (a later token's, say): rows that come out as NaN are
+// computed once more by this, so that only what a row sees reaches it.
+template <typename T, int HD>
+__device__ __noinline__ void prefill_row_again(const PrefillArgs<T>& a, int b, int hk, const T* qp, int pos, T* op) {
+  constexpr int DL = (HD + 31) / 32;  // channels per lane
+  const int lane = threadIdx.x & 31;
+  const int* trow = a.pg.table + (int64_t)b * a.pg.table_stride;
+  const T* kb = a.pg.k + (int64_t)hk * a.pg.head_stride;
+  const T* vb = a.pg.v + (int64_t)hk * a.pg.head_stride;
+  const Visible vis = visible_keys(pos, a.pg.window, a.pg.sinks);
+  float m = -CUDART_INF_F, l = 0.f, acc[DL];
+#pragma unroll
+  for (int i = 0; i < DL; ++i) acc[i] = 0.f;
+  for (int x0 = 0; x0 < vis.n; x0 += 32) {
+    int64_t off = -1;
+    float s = -CUDART_INF_F;
+    if (x0 + lane < vis.n) off = key_offset(a.pg, trow, vis.key(x0 + lane));
+    if (off >= 0) {
+      float dot = 0.f;
+      for (int d = 0; d < HD; ++d) dot = fmaf(to_f(qp[d]), to_f(kb[off + d]), dot);
+      s = dot * a.scale_log2;
+    }
+    const float mn = fmaxf(m, warp_max(s)), sub = mn == -CUDART_INF_F ? 0.f : mn;
+    const float corr = ex2_f32(m - sub), p = off >= 0 ? ex2_f32(s - sub) : 0.f;
+    m = mn;
+    l = l * corr + warp_sum(p);
+#pragma unroll
+    for (int i = 0; i < DL; ++i) acc[i] *= corr;
+    unsigned todo = __ballot_sync(0xffffffffu, off >= 0);
+    while (todo) {
+      const int j = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const float pj = __shfl_sync(0xffffffffu, p, j);
+      const int64_t oj = __shfl_sync(0xffffffffu, off, j);
+#pragma unroll
+      for (int i = 0; i < DL; ++i)
+        if (i * 32 + lane < HD) acc[i] = fmaf(pj, to_f(vb[oj + i * 32 + lane]), acc[i]);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < DL; ++i)
+    if (i * 32 + lane < HD) op[i * 32 + lane] = round_f<T>(l == 0.f ? 0.f : acc[i] / l);
+}
+
+// CUDA-core form for float32: 64 rows x 32 keys a step, 256 threads; a half warp owns four
 // rows (scores, softmax and accumulator), so only K and V tiles need barriers.
 template <typename T, int HD>
 __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArgs<T> a) {
@@ -175,18 +221,294 @@ __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArg
 #pragma unroll
     for (int o = 1; o < 16; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
     const int r = ty * 4 + i;
+    bool nan = false;
     if (r < nr) {
       const uint32_t t = fdiv((uint32_t)(r0 + r), a.group), g = (uint32_t)(r0 + r) - t * G;
       T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + g) * HD;
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) op[tx + 16 * d] = round_f<T>(L == 0.f ? 0.f : acc[i][d] / L);
+      for (int d = 0; d < HD / 16; ++d) {
+        const float x = L == 0.f ? 0.f : acc[i][d] / L;
+        nan |= x != x;
+        op[tx + 16 * d] = round_f<T>(x);
+      }
     }
+    const unsigned again = __ballot_sync(0xffffffffu, nan);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (again & (0xffffu << (16 * h))) {
+        const uint32_t x = (uint32_t)(r0 + (ty & ~1) * 4 + h * 4 + i), t = fdiv(x, a.group), g = x - t * G;
+        prefill_row_again<T, HD>(a, b, hk, a.q + (first + t) * a.q_ts + (int64_t)(hk * G + g) * a.q_hs, pos0 + (int)t,
+                                 a.o + ((first + t) * Hq + (int64_t)hk * G + g) * HD);
+      }
   }
   }
 }
 
+// Tensor-core form for 16-bit types (mma.sync m16n8k16, float32 accumulation):
+// W warps of 16 rows, K/V tiles of KT keys double-buffered in shared memory by
+// 16-byte asynchronous copies, one page lookup per key row and thread, made a
+// tile ahead.  Per tile and warp: S = Q K^T, the running maximum, P = 2^(c s -
+// c m) in float32, row sums of the float32 P, and O += P V with P rounded to
+// the type as the MMA operand: that rounding is relative to each probability
+// and independent between keys, so an output moves by about as much as its own
+// rounding does.  O and the row sums are only rescaled when a row's maximum has
+// grown by more than 8 powers of two since it was last moved (P <= 2^8).
+// With 16 channels the exponentials bound it (16 per clock and SM), with 32
+// they and the MMAs take the same time.
+template <int HD>
+__device__ __forceinline__ int row_swz(int r, int c) {  // 16-byte piece c of row r: its place in the row
+  if constexpr (HD == 16) return c ^ ((r >> 2) & 1);
+  else if constexpr (HD == 32) return c ^ ((r >> 1) & 3);
+  else return c ^ (r & 7);
+}
+
+template <typename T, int HD, int W, int KT>
+__global__ void __launch_bounds__(W * 32) paged_prefill_mma_kernel(const PrefillArgs<T> a) {
+  constexpr int QT = W * 16, NT = W * 32, CH = HD / 8, TILE = KT * HD;
+  extern __shared__ __align__(16) unsigned char smb[];
+  T* Ks = reinterpret_cast<T*>(smb);  // [2][KT][HD]
+  T* Vs = Ks + 2 * TILE;              // [2][KT][HD]
+  __shared__ uint8_t okr[2][KT];  // rows that hold a key (not past the end, not of a bad page)
+  const int b = blockIdx.z, hk = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t4 = lane & 3;
+  int64_t first;
+  const int T_ = query_span(a, b, &first);
+  const int G = (int)a.group.d;
+  const int64_t nrows = (int64_t)T_ * G, Hq = (int64_t)a.kv_heads * G;
+  const int len = seq_len(a.pg, b), pos0 = len - T_;
+  const int window = a.pg.window, sinks = a.pg.sinks;
+  const int* trow = a.pg.table + (int64_t)b * a.pg.table_stride;
+  const T* kb = a.pg.k + (int64_t)hk * a.pg.head_stride;
+  const T* vb = a.pg.v + (int64_t)hk * a.pg.head_stride;
+  const float c = a.scale_log2, thr = 8.f / c;
+  const int64_t tiles = (nrows + QT - 1) / QT;
+  // the grid covers max_q tokens, latest (longest) tiles first; tiles of a longer span follow in further turns
+  for (int64_t turn = blockIdx.x; turn < tiles; turn += gridDim.x) {
+    const int64_t r0 = (tiles - 1 - turn) * QT;
+    const int nr = (int)min64(QT, nrows - r0);
+    const int pos_first = pos0 + (int)fdiv((uint32_t)r0, a.group);
+    const int pos_last = pos0 + (int)fdiv((uint32_t)(r0 + nr - 1), a.group);
+    const int lo = window > 0 ? max(0, pos_first + 1 - window) : 0;
+    const int nsink = min(sinks, lo), n = nsink + max(0, pos_last + 1 - lo);
+    const int nt = (n + KT - 1) / KT;
+
+    // this thread's rows of a tile: page lookups for tile kt
+    constexpr int RPT = (KT * CH + NT - 1) / NT;  // 16-byte pieces per thread and matrix
+    int64_t off[RPT];
+    auto lookup = [&](int kt) {
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int x = kt * KT + (tid + i * NT) / CH;
+        off[i] = -1;
+        if ((tid + i * NT) < KT * CH && x < n) off[i] = key_offset(a.pg, trow, x < nsink ? x : lo + (x - nsink));
+      }
+    };
+    auto load = [&](int buf) {
+#pragma unroll
+      for (int i = 0; i < RPT; ++i) {
+        const int p = tid + i * NT, r = p / CH, ch = p - r * CH;
+        if (RPT * NT != KT * CH && p >= KT * CH) break;
+        const int64_t o = off[i] < 0 ? 0 : off[i];
+        const int at = buf * TILE + r * HD + row_swz<HD>(r, ch) * 8;
+        cp_async16(Ks + at, kb + o + ch * 8, off[i] < 0 ? 0 : 16);
+        cp_async16(Vs + at, vb + o + ch * 8, off[i] < 0 ? 0 : 16);
+        if (ch == 0) okr[buf][r] = off[i] >= 0;
+      }
+    };
+    __syncthreads();  // the buffers of the turn before are free
+    lookup(0);
+    load(0);
+    cp_async_commit();
+    if (nt > 1) lookup(1);
+
+    // Q fragments, this thread's two rows
+    const int rr = warp * 16 + g;
+    uint32_t qf[HD / 16][4];
+    int pos_lo, pos_hi;
+    {
+      const uint32_t* qp[2];
+      int ps[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = rr + 8 * h;
+        const uint32_t x = (uint32_t)(r0 + min(r, nr - 1)), t = fdiv(x, a.group), gi = x - t * G;
+        ps[h] = r < nr ? pos0 + (int)t : -1;
+        qp[h] = r < nr ? reinterpret_cast<const uint32_t*>(a.q + (first + t) * a.q_ts + (int64_t)(hk * G + gi) * a.q_hs)
+                       : nullptr;
+      }
+      pos_lo = ps[0];
+      pos_hi = ps[1];
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) qf[ks][j] = qp[j & 1] ? __ldg(qp[j & 1] + ks * 8 + t4 + (j >> 1) * 4) : 0u;
+    }
+    // positions of the warp's rows: which tiles it needs and which of them need masks
+    const int wr0 = warp * 16, wr1 = min(nr, wr0 + 16) - 1;
+    const int wpos_first = wr0 < nr ? pos0 + (int)fdiv((uint32_t)(r0 + wr0), a.group) : -1;
+    const int wpos_last = wr0 < nr ? pos0 + (int)fdiv((uint32_t)(r0 + wr1), a.group) : -1;
+
+    float m_lo = -CUDART_INF_F, m_hi = -CUDART_INF_F, l_lo = 0.f, l_hi = 0.f;
+    float acc[HD / 8][4];
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+
+    for (int kt = 0; kt < nt; ++kt) {
+      const int buf = kt & 1;
+      if (kt + 1 < nt) {
+        __syncthreads();  // the other buffer is free
+        load(buf ^ 1);
+        if (kt + 2 < nt) lookup(kt + 2);
+      }
+      cp_async_commit();
+      cp_async_wait<1>();
+      __syncthreads();
+      // keys of the tile: numbers x0 .. x0 + KT - 1; its window part is contiguous in keys
+      const int x0 = kt * KT, key_last = x0 + KT - 1 < nsink ? x0 + KT - 1 : lo + (x0 + KT - 1 - nsink);
+      const int key_first = x0 < nsink ? x0 : lo + (x0 - nsink);
+      const bool has_sink = x0 < nsink;
+      if (key_first > wpos_last || (window > 0 && !has_sink && key_last <= wpos_first - window && key_first >= sinks))
+        continue;  // no row of this warp sees a key of it
+      unsigned all = 0xffffffffu, okw[KT / 32];
+#pragma unroll
+      for (int i = 0; i < KT / 32; ++i) all &= okw[i] = __ballot_sync(0xffffffffu, okr[buf][i * 32 + lane] != 0);
+      const bool edge = all != 0xffffffffu || key_last > wpos_first || has_sink ||
+                        (window > 0 && key_first <= wpos_last - window);
+      const T* kt_s = Ks + buf * TILE;
+      const T* vt_s = Vs + buf * TILE;
+      float s[KT / 8][4];
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+        for (int np = 0; np < KT / 16; ++np) {
+          uint32_t kf[4];
+          const int r = np * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
+          ldsm_x4(kf, kt_s + r * HD + row_swz<HD>(r, ch) * 8);
+          mma16<T>(s[2 * np], qf[ks], kf[0], kf[1]);
+          mma16<T>(s[2 * np + 1], qf[ks], kf[2], kf[3]);
+        }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) {
+          const unsigned ok = okw[i >> 2] >> ((i & 3) * 8);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = 2 * t4 + e, x = x0 + i * 8 + j, key = x < nsink ? x : lo + (x - nsink);
+            const bool in = (ok >> j) & 1;
+            if (!(in && key <= pos_lo && (window == 0 || key > pos_lo - window || key < sinks))) s[i][e] = -CUDART_INF_F;
+            if (!(in && key <= pos_hi && (window == 0 || key > pos_hi - window || key < sinks))) s[i][2 + e] = -CUDART_INF_F;
+          }
+        }
+      }
+      float mt_lo = -CUDART_INF_F, mt_hi = -CUDART_INF_F;
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i) {
+        mt_lo = fmax3(mt_lo, s[i][0], s[i][1]);
+        mt_hi = fmax3(mt_hi, s[i][2], s[i][3]);
+      }
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) {
+        mt_lo = fmaxf(mt_lo, __shfl_xor_sync(0xffffffffu, mt_lo, o));
+        mt_hi = fmaxf(mt_hi, __shfl_xor_sync(0xffffffffu, mt_hi, o));
+      }
+      // (-inf + 8 stays -inf: a row's first key always moves its maximum)
+      const bool mv_lo = mt_lo > m_lo + thr, mv_hi = mt_hi > m_hi + thr;
+      if (__any_sync(0xffffffffu, mv_lo || mv_hi)) {
+        const float n_lo = mv_lo ? mt_lo : m_lo, n_hi = mv_hi ? mt_hi : m_hi;
+        // before a row's first key O and l are zero and any finite factor will do
+        const float f_lo = mv_lo && m_lo != -CUDART_INF_F ? ex2_f32((m_lo - n_lo) * c) : 1.f;
+        const float f_hi = mv_hi && m_hi != -CUDART_INF_F ? ex2_f32((m_hi - n_hi) * c) : 1.f;
+        l_lo *= f_lo;
+        l_hi *= f_hi;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          acc[i][0] *= f_lo; acc[i][1] *= f_lo;
+          acc[i][2] *= f_hi; acc[i][3] *= f_hi;
+        }
+        m_lo = n_lo;
+        m_hi = n_hi;
+      }
+      // rows without a key yet subtract 0: 2^-inf = 0
+      const float sub_lo = m_lo == -CUDART_INF_F ? 0.f : -m_lo * c, sub_hi = m_hi == -CUDART_INF_F ? 0.f : -m_hi * c;
+      const uint64_t c2 = f2_dup(c), b_lo = f2_dup(sub_lo), b_hi = f2_dup(sub_hi), one2 = f2_dup(1.f);
+      uint64_t rs_lo = 0, rs_hi = 0;
+      uint32_t pf[KT / 16][4];
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i) {
+        const uint64_t x = f2_fma(f2_pack(s[i][0], s[i][1]), c2, b_lo), y = f2_fma(f2_pack(s[i][2], s[i][3]), c2, b_hi);
+        const float p0 = ex2_f32(f2_lo(x)), p1 = ex2_f32(f2_hi(x)), p2 = ex2_f32(f2_lo(y)), p3 = ex2_f32(f2_hi(y));
+        rs_lo = f2_fma(f2_pack(p0, p1), one2, rs_lo);
+        rs_hi = f2_fma(f2_pack(p2, p3), one2, rs_hi);
+        pf[i >> 1][(i & 1) * 2 + 0] = pack2<T>(p0, p1);
+        pf[i >> 1][(i & 1) * 2 + 1] = pack2<T>(p2, p3);
+      }
+      l_lo += f2_lo(rs_lo) + f2_hi(rs_lo);
+      l_hi += f2_lo(rs_hi) + f2_hi(rs_hi);
+#pragma unroll
+      for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+        for (int dp = 0; dp < HD / 16; ++dp) {
+          uint32_t vf[4];
+          const int r = kk * 16 + (lane & 15), ch = dp * 2 + (lane >> 4);
+          ldsm_x4_t(vf, vt_s + r * HD + row_swz<HD>(r, ch) * 8);
+          mma16<T>(acc[2 * dp], pf[kk], vf[0], vf[1]);
+          mma16<T>(acc[2 * dp + 1], pf[kk], vf[2], vf[3]);
+        }
+    }
+    cp_async_wait<0>();
+    bool nan[2] = {false, false};
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+      l_lo += __shfl_xor_sync(0xffffffffu, l_lo, o);
+      l_hi += __shfl_xor_sync(0xffffffffu, l_hi, o);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = rr + 8 * h;
+      if (r < nr) {
+        const uint32_t x = (uint32_t)(r0 + r), t = fdiv(x, a.group), gi = x - t * G;
+        T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + gi) * HD;
+        const float l = h ? l_hi : l_lo, inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          const float u = acc[i][2 * h] * inv, w = acc[i][2 * h + 1] * inv;
+          nan[h] |= u != u || w != w;
+          T pair[2] = {round_f<T>(u), round_f<T>(w)};
+          *reinterpret_cast<uint32_t*>(op + i * 8 + 2 * t4) = *reinterpret_cast<uint32_t*>(pair);
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      unsigned again = __ballot_sync(0xffffffffu, nan[h]);
+      while (again) {
+        const int q = (__ffs(again) - 1) >> 2;  // the lane quad of a row
+        again &= ~(15u << (4 * q));
+        const uint32_t x = (uint32_t)(r0 + warp * 16 + 8 * h + q), t = fdiv(x, a.group), gi = x - t * G;
+        prefill_row_again<T, HD>(a, b, hk, a.q + (first + t) * a.q_ts + (int64_t)(hk * G + gi) * a.q_hs, pos0 + (int)t,
+                                 a.o + ((first + t) * Hq + (int64_t)hk * G + gi) * HD);
+      }
+    }
+  }
+}
+
+template <typename T, int HD>
+static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
+  constexpr int W = 4, KT = 64;
+  constexpr int smem = 4 * KT * HD * 2;
+  auto* kern = paged_prefill_mma_kernel<T, HD, W, KT>;
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status();
+  const int64_t tiles = ((int64_t)max_q * a.group.d + W * 16 - 1) / (W * 16);
+  kern<<<dim3((unsigned)tiles, a.kv_heads, B), W * 32, smem, s>>>(a);
+  return launch_status();
+}
+
 template <typename T, int HD>
 static int launch_prefill(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
+  if constexpr (sizeof(T) == 2) return launch_prefill_mma<T, HD>(a, B, max_q, s);
   constexpr int QT = 64, KT = 32, LD = HD + 4;
   const int smem = ((QT + 2 * KT) * LD + QT * (KT + 1)) * 4;
   auto* kern = paged_prefill_vec_kernel<T, HD>;
