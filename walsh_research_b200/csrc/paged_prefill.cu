@@ -255,6 +255,10 @@ __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArg
 // grown by more than 8 powers of two since it was last moved (P <= 2^8).
 // With 16 channels the exponentials bound it (16 per clock and SM), with 32
 // they and the MMAs take the same time.
+template <typename T> __device__ __forceinline__ uint32_t pack_p(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack_p<__half>(float lo, float hi) { return pack_f16(lo, hi); }
+template <> __device__ __forceinline__ uint32_t pack_p<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
+
 template <int HD>
 __device__ __forceinline__ int row_swz(int r, int c) {  // 16-byte piece c of row r: its place in the row
   if constexpr (HD == 16) return c ^ ((r >> 2) & 1);
@@ -262,13 +266,13 @@ __device__ __forceinline__ int row_swz(int r, int c) {  // 16-byte piece c of ro
   else return c ^ (r & 7);
 }
 
-template <typename T, int HD, int W, int KT>
-__global__ void __launch_bounds__(W * 32) paged_prefill_mma_kernel(const PrefillArgs<T> a) {
-  constexpr int QT = W * 16, NT = W * 32, CH = HD / 8, TILE = KT * HD;
+template <typename T, int HD, int W, int KS, int MINB>
+__global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const PrefillArgs<T> a) {
+  constexpr int QT = W * 16, NT = W * 32, CH = HD / 8, STAGE = KS * HD, KT = 64;
   extern __shared__ __align__(16) unsigned char smb[];
-  T* Ks = reinterpret_cast<T*>(smb);  // [2][KT][HD]
-  T* Vs = Ks + 2 * TILE;              // [2][KT][HD]
-  __shared__ uint8_t okr[2][KT];  // rows that hold a key (not past the end, not of a bad page)
+  T* Ks = reinterpret_cast<T*>(smb);  // [2][KS][HD]
+  T* Vs = Ks + 2 * STAGE;             // [2][KS][HD]
+  __shared__ uint8_t okr[2][KS];      // rows that hold a key; only read in stages with a bad page
   const int b = blockIdx.z, hk = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
   int64_t first;
@@ -288,43 +292,52 @@ __global__ void __launch_bounds__(W * 32) paged_prefill_mma_kernel(const Prefill
     const int nr = (int)min64(QT, nrows - r0);
     const int pos_first = pos0 + (int)fdiv((uint32_t)r0, a.group);
     const int pos_last = pos0 + (int)fdiv((uint32_t)(r0 + nr - 1), a.group);
+    // the tile's keys are numbered: sinks before the first row's window, then lo .. pos_last.
+    // In these numbers a row at pos sees x < end and (x >= beg or x < sinks), with
+    // end = pos + 1 - shift and beg = pos + 1 - window - shift, shift = lo - nsink.
     const int lo = window > 0 ? max(0, pos_first + 1 - window) : 0;
-    const int nsink = min(sinks, lo), n = nsink + max(0, pos_last + 1 - lo);
-    const int nt = (n + KT - 1) / KT;
+    const int nsink = min(sinks, lo), n = nsink + max(0, pos_last + 1 - lo), shift = lo - nsink;
+    const int nst = (n + KS - 1) / KS;
 
-    // this thread's rows of a tile: page lookups for tile kt
-    constexpr int RPT = (KT * CH + NT - 1) / NT;  // 16-byte pieces per thread and matrix
+    constexpr int RPT = (KS * CH + NT - 1) / NT;  // 16-byte pieces per thread and matrix
+    static_assert(KS * CH % NT == 0 || RPT == 1, "whole pieces");
     int64_t off[RPT];
-    auto lookup = [&](int kt) {
+    auto lookup = [&](int st) {
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
-        const int x = kt * KT + (tid + i * NT) / CH;
+        const int x = st * KS + (tid + i * NT) / CH;
         off[i] = -1;
-        if ((tid + i * NT) < KT * CH && x < n) off[i] = key_offset(a.pg, trow, x < nsink ? x : lo + (x - nsink));
+        if ((tid + i * NT) < KS * CH && x < n) off[i] = key_offset(a.pg, trow, x < nsink ? x : x + shift);
       }
     };
-    auto load = [&](int buf) {
+    // starts the copies of stage st; returns whether one of its keys lies in a bad page
+    auto load = [&](int st) {
+      const int buf = st & 1;
+      bool bad = false;
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
         const int p = tid + i * NT, r = p / CH, ch = p - r * CH;
-        if (RPT * NT != KT * CH && p >= KT * CH) break;
-        const int64_t o = off[i] < 0 ? 0 : off[i];
-        const int at = buf * TILE + r * HD + row_swz<HD>(r, ch) * 8;
-        cp_async16(Ks + at, kb + o + ch * 8, off[i] < 0 ? 0 : 16);
-        cp_async16(Vs + at, vb + o + ch * 8, off[i] < 0 ? 0 : 16);
-        if (ch == 0) okr[buf][r] = off[i] >= 0;
+        if (RPT == 1 && p >= KS * CH) break;
+        const bool in = off[i] >= 0;
+        const int64_t o = in ? off[i] : 0;
+        const int at = buf * STAGE + r * HD + row_swz<HD>(r, ch) * 8;
+        cp_async16(Ks + at, kb + o + ch * 8, in ? 16 : 0);
+        cp_async16(Vs + at, vb + o + ch * 8, in ? 16 : 0);
+        if (ch == 0) okr[buf][r] = in;
+        bad |= !in && st * KS + r < n;
       }
+      cp_async_commit();
+      return bad;
     };
     __syncthreads();  // the buffers of the turn before are free
     lookup(0);
-    load(0);
-    cp_async_commit();
-    if (nt > 1) lookup(1);
+    bool bad_next = load(0);
+    if (nst > 1) lookup(1);
 
-    // Q fragments, this thread's two rows
+    // Q fragments and bounds of this thread's two rows
     const int rr = warp * 16 + g;
     uint32_t qf[HD / 16][4];
-    int pos_lo, pos_hi;
+    int end_lo, end_hi;
     {
       const uint32_t* qp[2];
       int ps[2];
@@ -336,128 +349,159 @@ __global__ void __launch_bounds__(W * 32) paged_prefill_mma_kernel(const Prefill
         qp[h] = r < nr ? reinterpret_cast<const uint32_t*>(a.q + (first + t) * a.q_ts + (int64_t)(hk * G + gi) * a.q_hs)
                        : nullptr;
       }
-      pos_lo = ps[0];
-      pos_hi = ps[1];
+      end_lo = ps[0] < 0 ? 0 : ps[0] + 1 - shift;
+      end_hi = ps[1] < 0 ? 0 : ps[1] + 1 - shift;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
         for (int j = 0; j < 4; ++j) qf[ks][j] = qp[j & 1] ? __ldg(qp[j & 1] + ks * 8 + t4 + (j >> 1) * 4) : 0u;
     }
-    // positions of the warp's rows: which tiles it needs and which of them need masks
+    // numbers that every row of the warp sees: beg_all <= x < end_all (and x < sinks); that some row sees: beg_any, end_any
     const int wr0 = warp * 16, wr1 = min(nr, wr0 + 16) - 1;
-    const int wpos_first = wr0 < nr ? pos0 + (int)fdiv((uint32_t)(r0 + wr0), a.group) : -1;
-    const int wpos_last = wr0 < nr ? pos0 + (int)fdiv((uint32_t)(r0 + wr1), a.group) : -1;
+    int beg_any = 0, end_any = 0, beg_all = 0, end_all = 0;
+    if (wr0 < nr) {
+      end_all = max(0, pos0 + (int)fdiv((uint32_t)(r0 + wr0), a.group) + 1 - shift);
+      end_any = max(0, pos0 + (int)fdiv((uint32_t)(r0 + wr1), a.group) + 1 - shift);
+      if (window > 0) {
+        beg_any = end_all - window;
+        beg_all = end_any - window;
+      }
+    }
 
     float m_lo = -CUDART_INF_F, m_hi = -CUDART_INF_F, l_lo = 0.f, l_hi = 0.f;
     float acc[HD / 8][4];
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
 
-    for (int kt = 0; kt < nt; ++kt) {
-      const int buf = kt & 1;
-      if (kt + 1 < nt) {
-        __syncthreads();  // the other buffer is free
-        load(buf ^ 1);
-        if (kt + 2 < nt) lookup(kt + 2);
+    for (int st = 0; st < nst; ++st) {
+      const int buf = st & 1;
+      const bool bad_mine = bad_next;
+      if (st + 1 < nst) {
+        if (st > 0) __syncthreads();  // the other buffer is free
+        bad_next = load(st + 1);
+        if (st + 2 < nst) lookup(st + 2);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
       }
-      cp_async_commit();
-      cp_async_wait<1>();
-      __syncthreads();
-      // keys of the tile: numbers x0 .. x0 + KT - 1; its window part is contiguous in keys
-      const int x0 = kt * KT, key_last = x0 + KT - 1 < nsink ? x0 + KT - 1 : lo + (x0 + KT - 1 - nsink);
-      const int key_first = x0 < nsink ? x0 : lo + (x0 - nsink);
-      const bool has_sink = x0 < nsink;
-      if (key_first > wpos_last || (window > 0 && !has_sink && key_last <= wpos_first - window && key_first >= sinks))
-        continue;  // no row of this warp sees a key of it
-      unsigned all = 0xffffffffu, okw[KT / 32];
+      const bool bad = __syncthreads_or(bad_mine);
+#pragma unroll 1
+      for (int x0 = st * KS; x0 < min(n, (st + 1) * KS); x0 += KT) {
+        // no row of this warp sees a key of the step
+        if (x0 >= end_any || (x0 + KT <= beg_any && x0 >= sinks)) continue;
+        const int row0 = x0 - st * KS;
+        const T* kt_s = Ks + buf * STAGE + row0 * HD;
+        const T* vt_s = Vs + buf * STAGE + row0 * HD;
+        float s[KT / 8][4];
 #pragma unroll
-      for (int i = 0; i < KT / 32; ++i) all &= okw[i] = __ballot_sync(0xffffffffu, okr[buf][i * 32 + lane] != 0);
-      const bool edge = all != 0xffffffffu || key_last > wpos_first || has_sink ||
-                        (window > 0 && key_first <= wpos_last - window);
-      const T* kt_s = Ks + buf * TILE;
-      const T* vt_s = Vs + buf * TILE;
-      float s[KT / 8][4];
+        for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
 #pragma unroll
-      for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+        for (int ks = 0; ks < HD / 16; ++ks)
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
+          for (int np = 0; np < KT / 16; ++np) {
+            uint32_t kf[4];
+            const int r = np * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
+            ldsm_x4(kf, kt_s + r * HD + row_swz<HD>(r, ch) * 8);
+            mma16<T>(s[2 * np], qf[ks], kf[0], kf[1]);
+            mma16<T>(s[2 * np + 1], qf[ks], kf[2], kf[3]);
+          }
+        if (x0 + KT > end_all || (window > 0 && x0 < beg_all)) {
+          // masks: two bounds per row, and the sinks where the step holds some
+          const int e_lo = end_lo - x0 - 2 * t4, e_hi = end_hi - x0 - 2 * t4;
+          if (window == 0) {
 #pragma unroll
-        for (int np = 0; np < KT / 16; ++np) {
-          uint32_t kf[4];
-          const int r = np * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
-          ldsm_x4(kf, kt_s + r * HD + row_swz<HD>(r, ch) * 8);
-          mma16<T>(s[2 * np], qf[ks], kf[0], kf[1]);
-          mma16<T>(s[2 * np + 1], qf[ks], kf[2], kf[3]);
-        }
-      if (edge) {
+            for (int i = 0; i < KT / 8; ++i)
 #pragma unroll
-        for (int i = 0; i < KT / 8; ++i) {
-          const unsigned ok = okw[i >> 2] >> ((i & 3) * 8);
+              for (int e = 0; e < 2; ++e) {
+                if (i * 8 + e >= e_lo) s[i][e] = -CUDART_INF_F;
+                if (i * 8 + e >= e_hi) s[i][2 + e] = -CUDART_INF_F;
+              }
+          } else {
+            const int b_lo = e_lo - window, b_hi = e_hi - window, sk = sinks - x0 - 2 * t4;
+            if (x0 < sinks) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int j = 2 * t4 + e, x = x0 + i * 8 + j, key = x < nsink ? x : lo + (x - nsink);
-            const bool in = (ok >> j) & 1;
-            if (!(in && key <= pos_lo && (window == 0 || key > pos_lo - window || key < sinks))) s[i][e] = -CUDART_INF_F;
-            if (!(in && key <= pos_hi && (window == 0 || key > pos_hi - window || key < sinks))) s[i][2 + e] = -CUDART_INF_F;
+              for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int j = i * 8 + e;
+                  if (j >= e_lo || (j < b_lo && j >= sk)) s[i][e] = -CUDART_INF_F;
+                  if (j >= e_hi || (j < b_hi && j >= sk)) s[i][2 + e] = -CUDART_INF_F;
+                }
+            } else {
+#pragma unroll
+              for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  const int j = i * 8 + e;
+                  if ((unsigned)(j - b_lo) >= (unsigned)window) s[i][e] = -CUDART_INF_F;
+                  if ((unsigned)(j - b_hi) >= (unsigned)window) s[i][2 + e] = -CUDART_INF_F;
+                }
+            }
           }
         }
-      }
-      float mt_lo = -CUDART_INF_F, mt_hi = -CUDART_INF_F;
+        if (bad) {
 #pragma unroll
-      for (int i = 0; i < KT / 8; ++i) {
-        mt_lo = fmax3(mt_lo, s[i][0], s[i][1]);
-        mt_hi = fmax3(mt_hi, s[i][2], s[i][3]);
-      }
+          for (int i = 0; i < KT / 8; ++i)
 #pragma unroll
-      for (int o = 1; o <= 2; o <<= 1) {
-        mt_lo = fmaxf(mt_lo, __shfl_xor_sync(0xffffffffu, mt_lo, o));
-        mt_hi = fmaxf(mt_hi, __shfl_xor_sync(0xffffffffu, mt_hi, o));
-      }
-      // (-inf + 8 stays -inf: a row's first key always moves its maximum)
-      const bool mv_lo = mt_lo > m_lo + thr, mv_hi = mt_hi > m_hi + thr;
-      if (__any_sync(0xffffffffu, mv_lo || mv_hi)) {
-        const float n_lo = mv_lo ? mt_lo : m_lo, n_hi = mv_hi ? mt_hi : m_hi;
-        // before a row's first key O and l are zero and any finite factor will do
-        const float f_lo = mv_lo && m_lo != -CUDART_INF_F ? ex2_f32((m_lo - n_lo) * c) : 1.f;
-        const float f_hi = mv_hi && m_hi != -CUDART_INF_F ? ex2_f32((m_hi - n_hi) * c) : 1.f;
-        l_lo *= f_lo;
-        l_hi *= f_hi;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-          acc[i][0] *= f_lo; acc[i][1] *= f_lo;
-          acc[i][2] *= f_hi; acc[i][3] *= f_hi;
+            for (int e = 0; e < 2; ++e)
+              if (!okr[buf][row0 + i * 8 + 2 * t4 + e]) s[i][e] = s[i][2 + e] = -CUDART_INF_F;
         }
-        m_lo = n_lo;
-        m_hi = n_hi;
-      }
-      // rows without a key yet subtract 0: 2^-inf = 0
-      const float sub_lo = m_lo == -CUDART_INF_F ? 0.f : -m_lo * c, sub_hi = m_hi == -CUDART_INF_F ? 0.f : -m_hi * c;
-      const uint64_t c2 = f2_dup(c), b_lo = f2_dup(sub_lo), b_hi = f2_dup(sub_hi), one2 = f2_dup(1.f);
-      uint64_t rs_lo = 0, rs_hi = 0;
-      uint32_t pf[KT / 16][4];
+        float mt_lo = -CUDART_INF_F, mt_hi = -CUDART_INF_F;
 #pragma unroll
-      for (int i = 0; i < KT / 8; ++i) {
-        const uint64_t x = f2_fma(f2_pack(s[i][0], s[i][1]), c2, b_lo), y = f2_fma(f2_pack(s[i][2], s[i][3]), c2, b_hi);
-        const float p0 = ex2_f32(f2_lo(x)), p1 = ex2_f32(f2_hi(x)), p2 = ex2_f32(f2_lo(y)), p3 = ex2_f32(f2_hi(y));
-        rs_lo = f2_fma(f2_pack(p0, p1), one2, rs_lo);
-        rs_hi = f2_fma(f2_pack(p2, p3), one2, rs_hi);
-        pf[i >> 1][(i & 1) * 2 + 0] = pack2<T>(p0, p1);
-        pf[i >> 1][(i & 1) * 2 + 1] = pack2<T>(p2, p3);
-      }
-      l_lo += f2_lo(rs_lo) + f2_hi(rs_lo);
-      l_hi += f2_lo(rs_hi) + f2_hi(rs_hi);
-#pragma unroll
-      for (int kk = 0; kk < KT / 16; ++kk)
-#pragma unroll
-        for (int dp = 0; dp < HD / 16; ++dp) {
-          uint32_t vf[4];
-          const int r = kk * 16 + (lane & 15), ch = dp * 2 + (lane >> 4);
-          ldsm_x4_t(vf, vt_s + r * HD + row_swz<HD>(r, ch) * 8);
-          mma16<T>(acc[2 * dp], pf[kk], vf[0], vf[1]);
-          mma16<T>(acc[2 * dp + 1], pf[kk], vf[2], vf[3]);
+        for (int i = 0; i < KT / 8; ++i) {
+          mt_lo = fmax3(mt_lo, s[i][0], s[i][1]);
+          mt_hi = fmax3(mt_hi, s[i][2], s[i][3]);
         }
+        // the maximum moves when a row exceeds it by more than the slack; each
+        // quad's lanes decide together (-inf + slack stays -inf: a row's first key always moves it)
+        if (__any_sync(0xffffffffu, mt_lo > m_lo + thr || mt_hi > m_hi + thr)) {
+#pragma unroll
+          for (int o = 1; o <= 2; o <<= 1) {
+            mt_lo = fmaxf(mt_lo, __shfl_xor_sync(0xffffffffu, mt_lo, o));
+            mt_hi = fmaxf(mt_hi, __shfl_xor_sync(0xffffffffu, mt_hi, o));
+          }
+          const float n_lo = fmaxf(mt_lo, m_lo), n_hi = fmaxf(mt_hi, m_hi);
+          // before a row's first key O and l are zero and any finite factor will do
+          const float f_lo = m_lo != -CUDART_INF_F ? ex2_f32((m_lo - n_lo) * c) : 1.f;
+          const float f_hi = m_hi != -CUDART_INF_F ? ex2_f32((m_hi - n_hi) * c) : 1.f;
+          l_lo *= f_lo;
+          l_hi *= f_hi;
+#pragma unroll
+          for (int i = 0; i < HD / 8; ++i) {
+            acc[i][0] *= f_lo; acc[i][1] *= f_lo;
+            acc[i][2] *= f_hi; acc[i][3] *= f_hi;
+          }
+          m_lo = n_lo;
+          m_hi = n_hi;
+        }
+        // rows without a key yet subtract 0: 2^-inf = 0
+        const float sub_lo = m_lo == -CUDART_INF_F ? 0.f : -m_lo * c, sub_hi = m_hi == -CUDART_INF_F ? 0.f : -m_hi * c;
+        const uint64_t c2 = f2_dup(c), b_lo = f2_dup(sub_lo), b_hi = f2_dup(sub_hi), one2 = f2_dup(1.f);
+        uint64_t rs_lo = 0, rs_hi = 0;
+        uint32_t pf[KT / 16][4];
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) {
+          const uint64_t x = f2_fma(f2_pack(s[i][0], s[i][1]), c2, b_lo), y = f2_fma(f2_pack(s[i][2], s[i][3]), c2, b_hi);
+          const float p0 = ex2_f32(f2_lo(x)), p1 = ex2_f32(f2_hi(x)), p2 = ex2_f32(f2_lo(y)), p3 = ex2_f32(f2_hi(y));
+          rs_lo = f2_fma(f2_pack(p0, p1), one2, rs_lo);
+          rs_hi = f2_fma(f2_pack(p2, p3), one2, rs_hi);
+          pf[i >> 1][(i & 1) * 2 + 0] = pack_p<T>(p0, p1);
+          pf[i >> 1][(i & 1) * 2 + 1] = pack_p<T>(p2, p3);
+        }
+        l_lo += f2_lo(rs_lo) + f2_hi(rs_lo);
+        l_hi += f2_lo(rs_hi) + f2_hi(rs_hi);
+#pragma unroll
+        for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+          for (int dp = 0; dp < HD / 16; ++dp) {
+            uint32_t vf[4];
+            const int r = kk * 16 + (lane & 15), ch = dp * 2 + (lane >> 4);
+            ldsm_x4_t(vf, vt_s + r * HD + row_swz<HD>(r, ch) * 8);
+            mma16<T>(acc[2 * dp], pf[kk], vf[0], vf[1]);
+            mma16<T>(acc[2 * dp + 1], pf[kk], vf[2], vf[3]);
+          }
+      }
     }
-    cp_async_wait<0>();
     bool nan[2] = {false, false};
 #pragma unroll
     for (int o = 1; o <= 2; o <<= 1) {
@@ -494,16 +538,30 @@ __global__ void __launch_bounds__(W * 32) paged_prefill_mma_kernel(const Prefill
   }
 }
 
-template <typename T, int HD>
-static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
-  constexpr int W = 4, KT = 64;
-  constexpr int smem = 4 * KT * HD * 2;
-  auto* kern = paged_prefill_mma_kernel<T, HD, W, KT>;
+template <typename T, int HD, int W, int KS, int MINB>
+static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
+  constexpr int smem = 4 * KS * HD * 2;
+  auto* kern = paged_prefill_mma_kernel<T, HD, W, KS, MINB>;
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
   const int64_t tiles = ((int64_t)max_q * a.group.d + W * 16 - 1) / (W * 16);
   kern<<<dim3((unsigned)tiles, a.kv_heads, B), W * 32, smem, s>>>(a);
   return launch_status();
+}
+#ifndef PF_W16
+#define PF_W16 4
+#define PF_S16 128
+#define PF_B16 5
+#define PF_W32 4
+#define PF_S32 128
+#define PF_B32 4
+#endif
+template <typename T, int HD>
+static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
+  if constexpr (HD == 16) return launch_prefill_tile<T, HD, PF_W16, PF_S16, PF_B16>(a, B, max_q, s);
+  else if constexpr (HD == 32) return launch_prefill_tile<T, HD, PF_W32, PF_S32, PF_B32>(a, B, max_q, s);
+  else if constexpr (HD == 64) return launch_prefill_tile<T, HD, 4, 64, 3>(a, B, max_q, s);
+  else return launch_prefill_tile<T, HD, 4, 64, 2>(a, B, max_q, s);
 }
 
 template <typename T, int HD>
