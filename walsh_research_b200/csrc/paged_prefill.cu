@@ -272,7 +272,8 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
   extern __shared__ __align__(16) unsigned char smb[];
   T* Ks = reinterpret_cast<T*>(smb);  // [2][KS][HD]
   T* Vs = Ks + 2 * STAGE;             // [2][KS][HD]
-  __shared__ uint8_t okr[2][KS];      // rows that hold a key; only read in stages with a bad page
+  // offsets of a stage's key rows (-1: none, or in a bad page), looked up a stage ahead, one row per thread
+  __shared__ int64_t offs[3][KS];
   const int b = blockIdx.z, hk = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t4 = lane & 3;
   int64_t first;
@@ -299,31 +300,28 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
     const int nsink = min(sinks, lo), n = nsink + max(0, pos_last + 1 - lo), shift = lo - nsink;
     const int nst = (n + KS - 1) / KS;
 
-    constexpr int RPT = (KS * CH + NT - 1) / NT;  // 16-byte pieces per thread and matrix
-    static_assert(KS * CH % NT == 0 || RPT == 1, "whole pieces");
-    int64_t off[RPT];
     auto lookup = [&](int st) {
-#pragma unroll
-      for (int i = 0; i < RPT; ++i) {
-        const int x = st * KS + (tid + i * NT) / CH;
-        off[i] = -1;
-        if ((tid + i * NT) < KS * CH && x < n) off[i] = key_offset(a.pg, trow, x < nsink ? x : x + shift);
+      for (int r = tid; r < KS; r += NT) {
+        const int x = st * KS + r;
+        offs[st % 3][r] = x < n ? key_offset(a.pg, trow, x < nsink ? x : x + shift) : -1;
       }
     };
     // starts the copies of stage st; returns whether one of its keys lies in a bad page
+    constexpr int RPT = KS * CH / NT;  // 16-byte pieces per thread and matrix
+    static_assert(KS * CH % NT == 0 && NT % CH == 0, "whole pieces");
+    const int pr = tid / CH, pc = tid - pr * CH;
     auto load = [&](int st) {
       const int buf = st & 1;
       bool bad = false;
 #pragma unroll
       for (int i = 0; i < RPT; ++i) {
-        const int p = tid + i * NT, r = p / CH, ch = p - r * CH;
-        if (RPT == 1 && p >= KS * CH) break;
-        const bool in = off[i] >= 0;
-        const int64_t o = in ? off[i] : 0;
-        const int at = buf * STAGE + r * HD + row_swz<HD>(r, ch) * 8;
-        cp_async16(Ks + at, kb + o + ch * 8, in ? 16 : 0);
-        cp_async16(Vs + at, vb + o + ch * 8, in ? 16 : 0);
-        if (ch == 0) okr[buf][r] = in;
+        const int r = pr + i * (NT / CH);
+        const int64_t off = offs[st % 3][r];
+        const bool in = off >= 0;
+        const int64_t o = (in ? off : 0) + pc * 8;
+        const int at = buf * STAGE + r * HD + row_swz<HD>(r, pc) * 8;
+        cp_async16(Ks + at, kb + o, in ? 16 : 0);
+        cp_async16(Vs + at, vb + o, in ? 16 : 0);
         bad |= !in && st * KS + r < n;
       }
       cp_async_commit();
@@ -331,8 +329,9 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
     };
     __syncthreads();  // the buffers of the turn before are free
     lookup(0);
+    lookup(1);
+    __syncthreads();
     bool bad_next = load(0);
-    if (nst > 1) lookup(1);
 
     // Q fragments and bounds of this thread's two rows
     const int rr = warp * 16 + g;
@@ -379,7 +378,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
       if (st + 1 < nst) {
         if (st > 0) __syncthreads();  // the other buffer is free
         bad_next = load(st + 1);
-        if (st + 2 < nst) lookup(st + 2);
+        lookup(st + 2);
         cp_async_wait<1>();
       } else {
         cp_async_wait<0>();
@@ -405,38 +404,35 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
             mma16<T>(s[2 * np], qf[ks], kf[0], kf[1]);
             mma16<T>(s[2 * np + 1], qf[ks], kf[2], kf[3]);
           }
-        if (x0 + KT > end_all || (window > 0 && x0 < beg_all)) {
-          // masks: two bounds per row, and the sinks where the step holds some
+        if (x0 + KT > end_all) {  // keys after some row
           const int e_lo = end_lo - x0 - 2 * t4, e_hi = end_hi - x0 - 2 * t4;
-          if (window == 0) {
+#pragma unroll
+          for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              if (i * 8 + e >= e_lo) s[i][e] = -CUDART_INF_F;
+              if (i * 8 + e >= e_hi) s[i][2 + e] = -CUDART_INF_F;
+            }
+        }
+        if (window > 0 && x0 < beg_all) {  // keys before some row's window; sinks stay
+          const int b_lo = end_lo - window - x0 - 2 * t4, b_hi = end_hi - window - x0 - 2 * t4;
+          const int sk = sinks - x0 - 2 * t4;
+          if (x0 < sinks) {
 #pragma unroll
             for (int i = 0; i < KT / 8; ++i)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                if (i * 8 + e >= e_lo) s[i][e] = -CUDART_INF_F;
-                if (i * 8 + e >= e_hi) s[i][2 + e] = -CUDART_INF_F;
+                if (i * 8 + e < b_lo && i * 8 + e >= sk) s[i][e] = -CUDART_INF_F;
+                if (i * 8 + e < b_hi && i * 8 + e >= sk) s[i][2 + e] = -CUDART_INF_F;
               }
           } else {
-            const int b_lo = e_lo - window, b_hi = e_hi - window, sk = sinks - x0 - 2 * t4;
-            if (x0 < sinks) {
 #pragma unroll
-              for (int i = 0; i < KT / 8; ++i)
+            for (int i = 0; i < KT / 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int j = i * 8 + e;
-                  if (j >= e_lo || (j < b_lo && j >= sk)) s[i][e] = -CUDART_INF_F;
-                  if (j >= e_hi || (j < b_hi && j >= sk)) s[i][2 + e] = -CUDART_INF_F;
-                }
-            } else {
-#pragma unroll
-              for (int i = 0; i < KT / 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  const int j = i * 8 + e;
-                  if ((unsigned)(j - b_lo) >= (unsigned)window) s[i][e] = -CUDART_INF_F;
-                  if ((unsigned)(j - b_hi) >= (unsigned)window) s[i][2 + e] = -CUDART_INF_F;
-                }
-            }
+              for (int e = 0; e < 2; ++e) {
+                if (i * 8 + e < b_lo) s[i][e] = -CUDART_INF_F;
+                if (i * 8 + e < b_hi) s[i][2 + e] = -CUDART_INF_F;
+              }
           }
         }
         if (bad) {
@@ -444,7 +440,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
           for (int i = 0; i < KT / 8; ++i)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              if (!okr[buf][row0 + i * 8 + 2 * t4 + e]) s[i][e] = s[i][2 + e] = -CUDART_INF_F;
+              if (offs[st % 3][row0 + i * 8 + 2 * t4 + e] < 0) s[i][e] = s[i][2 + e] = -CUDART_INF_F;
         }
         float mt_lo = -CUDART_INF_F, mt_hi = -CUDART_INF_F;
 #pragma unroll
