@@ -41,7 +41,7 @@ __device__ __forceinline__ void split_range(int n, int chunk, int nsplit, int c,
 }
 
 // ---------------------------------------------------------------------------
-// CUDA-core form, any type.  LPK lanes share one key, 16 bytes of it each; a
+// CUDA-core form for float32.  LPK lanes share one key, 16 bytes of it each; a
 // warp step covers 32 / LPK keys and KPT steps are in flight.
 // ---------------------------------------------------------------------------
 template <typename T, int HD, int GH, int W>
@@ -179,6 +179,253 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
   }
 }
 
+// ---------------------------------------------------------------------------
+// Tensor-core form for 16-bit types.  A CTA of W warps takes one range of one
+// (sequence, key/value head); each warp streams its slice through its own ring
+// of NS stages of KT keys (16-byte asynchronous copies; no CTA barrier until
+// the join), page lookups made a stage ahead, one key row per lane.  The heads
+// of the group are the rows of the MMAs: S = Q K^T and O += P V (m16n8k16).
+// With up to 8 heads the rows 8 - 15 carry what rounding P to 16 bits left over
+// in rows 0 - 7, so P keeps 16 (bf16) to 22 bits at no cost; with 9 to 16 heads
+// P is rounded once, which moves an output by about as much as its own rounding.
+// ---------------------------------------------------------------------------
+template <int HD>
+__device__ __forceinline__ int dec_swz(int r, int c) {  // 16-byte piece c of row r: its place in the row
+  if constexpr (HD == 16) return c ^ ((r >> 2) & 1);
+  else if constexpr (HD == 32) return c ^ ((r >> 1) & 3);
+  else return c ^ (r & 7);
+}
+template <typename T> __device__ __forceinline__ uint32_t dec_pack(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t dec_pack<__half>(float lo, float hi) { return pack_f16(lo, hi); }
+template <> __device__ __forceinline__ uint32_t dec_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
+
+// RH: halves of the 16 MMA rows in use (1: up to 8 heads, 2: up to 16)
+template <typename T, int HD, int RH, int W, int KT, int NS>
+__global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeArgs<T> a) {
+  constexpr int CH = HD / 8, STAGE = 2 * KT * HD, RI = 32 / CH;  // RI: rows per copy instruction
+  constexpr int OL = HD + 4;                                     // padded row of the join buffer
+  extern __shared__ __align__(16) unsigned char smb[];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+  int unit = blockIdx.x;
+  const int c = unit % a.nsplit;
+  unit /= a.nsplit;
+  const int gt = unit % a.gtiles;
+  unit /= a.gtiles;
+  const int hk = unit % a.kv_heads, b = unit / a.kv_heads;
+  const int len = seq_len(a.pg, b);
+  const Visible vis = visible_keys(len - 1, a.pg.window, a.pg.sinks);
+  int beg, end;
+  split_range(vis.n, a.chunk, a.nsplit, c, &beg, &end);
+  if (beg >= end && c > 0) return;
+  const int ng = min(8 * RH, a.group - gt * 8 * RH), h0 = hk * a.group + gt * 8 * RH;
+  const int per = ((end - beg + W - 1) / W + 15) / 16 * 16;
+  const int wbeg = min(end, beg + warp * per), n = min(end, wbeg + per) - wbeg;  // this warp's keys
+  const int nst = (n + KT - 1) / KT;
+  T* ring = reinterpret_cast<T*>(smb) + warp * (NS * STAGE);  // a warp's own
+  const int* trow = a.pg.table + (int64_t)b * a.pg.table_stride;
+  const T* kb = a.pg.k + (int64_t)hk * a.pg.head_stride + (lane % CH) * 8;
+  const T* vb = a.pg.v + (int64_t)hk * a.pg.head_stride + (lane % CH) * 8;
+
+  constexpr int RL = (KT + 31) / 32;  // rows looked up per lane
+  int64_t off[RL];
+  auto lookup = [&](int st) {
+#pragma unroll
+    for (int i = 0; i < RL; ++i) {
+      const int x = st * KT + i * 32 + lane;
+      off[i] = -1;
+      if ((KT >= 32 || lane < KT) && x < n) off[i] = key_offset(a.pg, trow, vis.key(wbeg + x));
+    }
+  };
+  // bit r: row r of the stage holds a key
+  uint32_t okq[NS][RL];
+  auto load = [&](int st, int buf) {
+    T* dst = ring + buf * STAGE;
+#pragma unroll
+    for (int i = 0; i < KT / RI; ++i) {
+      const int r = i * RI + lane / CH, ch = lane % CH;
+      const int64_t o = __shfl_sync(0xffffffffu, off[(i * RI) / 32], r % 32);
+      const int at = r * HD + dec_swz<HD>(r, ch) * 8;
+      cp_async16(dst + at, kb + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
+      cp_async16(dst + KT * HD + at, vb + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
+    }
+    (void)st;
+  };
+#pragma unroll
+  for (int i = 0; i < NS; ++i)
+#pragma unroll
+    for (int j = 0; j < RL; ++j) okq[i][j] = 0;
+  if (n > 0) {
+    lookup(0);
+#pragma unroll
+    for (int s = 0; s < NS - 1; ++s) {
+      if (s < nst) load(s, s);
+#pragma unroll
+      for (int j = 0; j < RL; ++j) okq[s][j] = __ballot_sync(0xffffffffu, s < nst && off[j] >= 0);
+      cp_async_commit();
+      lookup(s + 1);
+    }
+  }
+  // Q fragments; rows past the tile's heads are zero
+  uint32_t qf[HD / 16][4];
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int r = g + (j & 1) * 8;
+      qf[ks][j] = 0u;
+      if (r < ng)
+        qf[ks][j] = __ldg(reinterpret_cast<const uint32_t*>(a.q + (int64_t)b * a.q_bs + (int64_t)(h0 + r) * a.q_hs) +
+                          ks * 8 + t4 + (j >> 1) * 4);
+    }
+  float m[2] = {-CUDART_INF_F, -CUDART_INF_F}, l[2] = {0.f, 0.f}, acc[HD / 8][4];
+#pragma unroll
+  for (int i = 0; i < HD / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+  const float sc = a.scale_log2;
+  auto compute = [&](const T* kt_s, const uint32_t* ok) {
+    const T* vt_s = kt_s + KT * HD;
+    float s[KT / 8][4];
+#pragma unroll
+    for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+      for (int np = 0; np < KT / 16; ++np) {
+        uint32_t kf[4];
+        const int r = np * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
+        ldsm_x4(kf, kt_s + r * HD + dec_swz<HD>(r, ch) * 8);
+        mma16<T>(s[2 * np], qf[ks], kf[0], kf[1]);
+        mma16<T>(s[2 * np + 1], qf[ks], kf[2], kf[3]);
+      }
+    bool full = true;
+#pragma unroll
+    for (int j = 0; j < RL; ++j) full &= ok[j] == (KT >= 32 ? 0xffffffffu : (1u << (KT & 31)) - 1u);
+    if (!full) {
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (!((ok[i >> 2] >> ((i & 3) * 8 + 2 * t4 + e)) & 1u)) s[i][e] = s[i][2 + e] = -CUDART_INF_F;
+    }
+    uint32_t pf[KT / 16][4];
+#pragma unroll
+    for (int h = 0; h < RH; ++h) {
+      float mt = -CUDART_INF_F;
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i) mt = fmax3(mt, s[i][2 * h], s[i][2 * h + 1]);
+#pragma unroll
+      for (int o = 1; o <= 2; o <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+      const float mn = fmaxf(m[h], mt), sub = mn == -CUDART_INF_F ? 0.f : mn * sc;
+      const float corr = ex2_f32(m[h] * sc - sub);
+      m[h] = mn;
+      float rs = 0.f;
+#pragma unroll
+      for (int i = 0; i < KT / 8; ++i) {
+        const float p0 = ex2_f32(fmaf(s[i][2 * h], sc, -sub)), p1 = ex2_f32(fmaf(s[i][2 * h + 1], sc, -sub));
+        rs += p0 + p1;
+        const uint32_t hi = dec_pack<T>(p0, p1);
+        pf[i >> 1][(i & 1) * 2 + h] = hi;
+        if constexpr (RH == 1) {
+          const float2 hf = unpack2<T>(hi);
+          pf[i >> 1][(i & 1) * 2 + 1] = dec_pack<T>(p0 - hf.x, p1 - hf.y);
+        }
+      }
+      l[h] = l[h] * corr + rs;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) {
+        acc[i][2 * h] *= corr, acc[i][2 * h + 1] *= corr;
+        if constexpr (RH == 1) acc[i][2] *= corr, acc[i][3] *= corr;
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+      for (int dp = 0; dp < HD / 16; ++dp) {
+        uint32_t vf[4];
+        const int r = kk * 16 + (lane & 15), ch = dp * 2 + (lane >> 4);
+        ldsm_x4_t(vf, vt_s + r * HD + dec_swz<HD>(r, ch) * 8);
+        mma16<T>(acc[2 * dp], pf[kk], vf[0], vf[1]);
+        mma16<T>(acc[2 * dp + 1], pf[kk], vf[2], vf[3]);
+      }
+  };
+  for (int st0 = 0; st0 < nst; st0 += NS) {
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {  // stage st0 + u lies in buffer u
+      const int st = st0 + u;
+      if (st >= nst) break;
+      // the buffer that the stage before this one left takes stage st + NS - 1
+      constexpr int NB = NS - 1;
+      const int nb = (u + NB) % NS;
+      if (st + NB < nst) load(st + NB, nb);
+#pragma unroll
+      for (int j = 0; j < RL; ++j) okq[nb][j] = __ballot_sync(0xffffffffu, st + NB < nst && off[j] >= 0);
+      cp_async_commit();
+      lookup(st + NS);
+      cp_async_wait<NS - 1>();
+      __syncwarp();
+      compute(ring + u * STAGE, okq[u]);
+      __syncwarp();
+    }
+  }
+  cp_async_wait<0>();
+#pragma unroll
+  for (int h = 0; h < RH; ++h)
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], o);
+  if constexpr (RH == 1) {  // the leftovers' part (an infinite sum is complete without it)
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (fabsf(acc[i][e]) < CUDART_INF_F) acc[i][e] += acc[i][2 + e];
+  }
+  // join the warps: rows of the ring are free
+  float* jo = reinterpret_cast<float*>(smb);             // [W][8 RH][OL]
+  float* jm = jo + W * 8 * RH * OL;                      // [W][8 RH][2]
+  if constexpr (W > 1) __syncthreads();
+#pragma unroll
+  for (int h = 0; h < RH; ++h) {
+    const int r = g + 8 * h;
+    if (r < ng) {
+      float* row = jo + (warp * 8 * RH + r) * OL;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i)
+        *reinterpret_cast<float2*>(row + i * 8 + 2 * t4) = make_float2(acc[i][2 * h], acc[i][2 * h + 1]);
+      if (t4 == 0) {
+        jm[(warp * 8 * RH + r) * 2] = m[h] * sc;
+        jm[(warp * 8 * RH + r) * 2 + 1] = l[h];
+      }
+    }
+  }
+  if constexpr (W > 1) __syncthreads();
+  else __syncwarp();
+  const int64_t Hq = (int64_t)a.kv_heads * a.group;
+  const bool whole = vis.n <= a.chunk || a.nsplit == 1;  // this range is all there is
+  for (int i = threadIdx.x; i < ng * HD; i += W * 32) {
+    const int r = i / HD, d = i - r * HD;
+    float M = -CUDART_INF_F;
+#pragma unroll
+    for (int w = 0; w < W; ++w) M = fmaxf(M, jm[(w * 8 * RH + r) * 2]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float mw = jm[(w * 8 * RH + r) * 2];
+      const float f = mw == -CUDART_INF_F ? 0.f : ex2_f32(mw - M);
+      L = fmaf(jm[(w * 8 * RH + r) * 2 + 1], f, L);
+      O = fmaf(jo[(w * 8 * RH + r) * OL + d], f, O);
+    }
+    const int64_t row = (int64_t)b * Hq + h0 + r;
+    if (whole) {
+      a.o[row * HD + d] = round_f<T>(L == 0.f ? 0.f : O / L);  // no visible key: zeros
+    } else {
+      a.part_o[(row * a.nsplit + c) * HD + d] = O;
+      if (d == 0) {
+        a.part_ml[(row * a.nsplit + c) * 2] = M;
+        a.part_ml[(row * a.nsplit + c) * 2 + 1] = L;
+      }
+    }
+  }
+}
+
 // Joins the ranges of each (sequence, head): one warp per row.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs<T> a) {
@@ -216,15 +463,35 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs<T> a) 
     for (int k = 0; k < HD / DP; ++k) a.o[row * HD + k * DP + d0] = round_f<T>(L == 0.f ? 0.f : O[k] / L);
 }
 
-template <typename T, int HD>
-static int launch_decode(DecodeArgs<T> a, cudaStream_t s) {
-  constexpr int W = 4;
+template <typename T, int HD, int RH, int W>
+static int launch_decode_mma(const DecodeArgs<T>& a, int64_t ctas, cudaStream_t s) {
+  // 8 KB of K and V per stage (4 KB for 16 channels)
+  constexpr int KT = HD <= 32 ? 64 : HD == 64 ? 32 : 16;
+  // two stages in flight and the warps' number cover the latency; the smaller
+  // ring leaves room for more warps (256 x 1024 keys, 16 channels: 2 stages
+  // 49.4 us, 3 50.7, 4 58.4; 12 x 32768, 64 channels: 82.3, 89.4, 94.8)
+  constexpr int NS = 2;
+  constexpr int ring = W * NS * 2 * KT * HD * 2, join = W * 8 * RH * (HD + 4 + 2) * 4;
+  constexpr int smem = ring > join ? ring : join;
+  auto* kern = paged_decode_mma_kernel<T, HD, RH, W, KT, NS>;
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status();
+  kern<<<(unsigned)ctas, W * 32, smem, s>>>(a);
+  return launch_status();
+}
+
+template <typename T, int HD, int W>
+static int launch_decode(const DecodeArgs<T>& a, cudaStream_t s) {
   const int64_t ctas = (int64_t)a.B * a.kv_heads * a.gtiles * a.nsplit;
-  if (a.group == 1)
-    paged_decode_vec_kernel<T, HD, 1, W><<<(unsigned)ctas, W * 32, 0, s>>>(a);
-  else
-    paged_decode_vec_kernel<T, HD, 4, W><<<(unsigned)ctas, W * 32, 0, s>>>(a);
-  if (const int r = launch_status()) return r;
+  int r;
+  if constexpr (sizeof(T) == 2) {
+    r = a.group <= 8 ? launch_decode_mma<T, HD, 1, W>(a, ctas, s) : launch_decode_mma<T, HD, 2, W>(a, ctas, s);
+  } else {
+    if (a.group == 1) paged_decode_vec_kernel<T, HD, 1, W><<<(unsigned)ctas, W * 32, 0, s>>>(a);
+    else paged_decode_vec_kernel<T, HD, 4, W><<<(unsigned)ctas, W * 32, 0, s>>>(a);
+    r = launch_status();
+  }
+  if (r) return r;
   if (a.nsplit > 1) {
     const int64_t rows = (int64_t)a.B * a.kv_heads * a.group;
     paged_join_kernel<T, HD><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a);
@@ -233,24 +500,31 @@ static int launch_decode(DecodeArgs<T> a, cudaStream_t s) {
   return WALSH_OK;
 }
 
-// How a call is cut: enough ranges to fill the GPU when there are few (sequence,
-// head) units, none shorter than 256 keys.
+// How a call is cut: `warps` per CTA, `nsplit` ranges of `chunk` visible keys.
 struct DecodePlan {
-  int gtiles, nsplit, chunk;
+  int warps, gtiles, nsplit, chunk;
 };
+constexpr int kDecodeWarps = 148 * 16;  // wanted in all
+constexpr int kDecodeMinKeys = 128;     // of one warp
 static DecodePlan decode_plan(const walsh_paged_kv* kv, int B, int q_heads, int max_len) {
-  const int group = q_heads / kv->kv_heads;
+  const int group = q_heads / kv->kv_heads, tile = kv->dtype == WALSH_F32 ? 4 : group <= 8 ? 8 : 16;
   DecodePlan p;
-  p.gtiles = group == 1 ? 1 : (group + 3) / 4;
+  p.gtiles = group == 1 ? 1 : (group + tile - 1) / tile;
   const int64_t units = (int64_t)B * kv->kv_heads * p.gtiles;
   int64_t n = max_len;
   if (kv->window > 0) n = min64(n, (int64_t)kv->window + kv->sinks);
-  const int64_t want = (148 * 8 + units - 1) / units;
-  p.nsplit = (int)(n < 256 ? 1 : min64(want, n / 256));
-  if (p.nsplit < 1) p.nsplit = 1;
+  const int64_t want = (kDecodeWarps + units - 1) / units, most = n / kDecodeMinKeys;
+  const int64_t per_unit = most < 1 ? 1 : min64(most, want);
+  p.warps = per_unit >= 4 ? 4 : 1;
+  p.nsplit = (int)((per_unit + p.warps - 1) / p.warps);
   p.chunk = (int)((n + p.nsplit - 1) / p.nsplit);
   if (p.chunk < 1) p.chunk = 1;
   return p;
+}
+
+template <typename T, int HD>
+static int launch_decode_warps(const DecodeArgs<T>& a, int warps, cudaStream_t s) {
+  return warps == 1 ? launch_decode<T, HD, 1>(a, s) : launch_decode<T, HD, 4>(a, s);
 }
 
 }  // namespace walsh
@@ -293,10 +567,10 @@ extern "C" walsh_status walsh_paged_attn_fwd(const walsh_paged_kv* kv, const voi
     a.scale_log2 = kv->scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
     switch (kv->head_dim) {
-      case 16: return launch_decode<ET, 16>(a, s);
-      case 32: return launch_decode<ET, 32>(a, s);
-      case 64: return launch_decode<ET, 64>(a, s);
-      default: return launch_decode<ET, 128>(a, s);
+      case 16: return launch_decode_warps<ET, 16>(a, p.warps, s);
+      case 32: return launch_decode_warps<ET, 32>(a, p.warps, s);
+      case 64: return launch_decode_warps<ET, 64>(a, p.warps, s);
+      default: return launch_decode_warps<ET, 128>(a, p.warps, s);
     }
   }());
 }

@@ -10,6 +10,8 @@
 // key/value heads are read once for their whole group.
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "mma.cuh"
 #include "paged.cuh"
 
@@ -266,9 +268,29 @@ __device__ __forceinline__ int row_swz(int r, int c) {  // 16-byte piece c of ro
   else return c ^ (r & 7);
 }
 
-template <typename T, int HD, int W, int KS, int MINB>
+// d = a b + (c_lo, c_lo, c_hi, c_hi)
+template <typename T> __device__ __forceinline__ void mma_rowc(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo, float c_hi);
+template <> __device__ __forceinline__ void mma_rowc<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo, float c_hi) {
+  mma_f16_rowc(d, a, b0, b1, c_lo, c_hi);
+}
+template <> __device__ __forceinline__ void mma_rowc<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo, float c_hi) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%11,%11};\n"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c_lo), "f"(c_hi));
+}
+
+template <typename T, int HD, int W, int MT, int KT, int KS, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const PrefillArgs<T> a) {
-  constexpr int QT = W * 16, NT = W * 32, CH = HD / 8, STAGE = KS * HD, KT = 64;
+  constexpr int QT = W * MT * 16, NT = W * 32, CH = HD / 8, STAGE = KS * HD;
+  // c q as two 16-bit terms (22 bits together), so that the MMAs give c s - m
+  #ifndef NOFOLD
+  constexpr bool FOLD = HD == 16;
+#else
+  constexpr bool FOLD = false;
+#endif
+  constexpr int QF = FOLD ? 2 : 1;
   extern __shared__ __align__(16) unsigned char smb[];
   T* Ks = reinterpret_cast<T*>(smb);  // [2][KS][HD]
   T* Vs = Ks + 2 * STAGE;             // [2][KS][HD]
@@ -285,7 +307,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
   const int* trow = a.pg.table + (int64_t)b * a.pg.table_stride;
   const T* kb = a.pg.k + (int64_t)hk * a.pg.head_stride;
   const T* vb = a.pg.v + (int64_t)hk * a.pg.head_stride;
-  const float c = a.scale_log2, thr = 8.f / c;
+  const float c = a.scale_log2, slack = 8.f / c;
   const int64_t tiles = (nrows + QT - 1) / QT;
   // the grid covers max_q tokens, latest (longest) tiles first; tiles of a longer span follow in further turns
   for (int64_t turn = blockIdx.x; turn < tiles; turn += gridDim.x) {
@@ -294,8 +316,8 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
     const int pos_first = pos0 + (int)fdiv((uint32_t)r0, a.group);
     const int pos_last = pos0 + (int)fdiv((uint32_t)(r0 + nr - 1), a.group);
     // the tile's keys are numbered: sinks before the first row's window, then lo .. pos_last.
-    // In these numbers a row at pos sees x < end and (x >= beg or x < sinks), with
-    // end = pos + 1 - shift and beg = pos + 1 - window - shift, shift = lo - nsink.
+    // In these numbers a row at pos sees x < end and (x >= end - window or x < sinks), with
+    // end = pos + 1 - shift, shift = lo - nsink.
     const int lo = window > 0 ? max(0, pos_first + 1 - window) : 0;
     const int nsink = min(sinks, lo), n = nsink + max(0, pos_last + 1 - lo), shift = lo - nsink;
     const int nst = (n + KS - 1) / KS;
@@ -333,31 +355,28 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
     __syncthreads();
     bool bad_next = load(0);
 
-    // Q fragments and bounds of this thread's two rows
-    const int rr = warp * 16 + g;
-    uint32_t qf[HD / 16][4];
-    int end_lo, end_hi;
-    {
-      const uint32_t* qp[2];
-      int ps[2];
+    // Q fragments and bounds of this thread's rows: tile mt of the warp, halves g and g + 8
+    uint32_t qf[MT][HD / 16][4];
+    int end[MT][2];
+    const int wr0 = warp * MT * 16;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = rr + 8 * h;
+        const int r = wr0 + mt * 16 + g + 8 * h;
         const uint32_t x = (uint32_t)(r0 + min(r, nr - 1)), t = fdiv(x, a.group), gi = x - t * G;
-        ps[h] = r < nr ? pos0 + (int)t : -1;
-        qp[h] = r < nr ? reinterpret_cast<const uint32_t*>(a.q + (first + t) * a.q_ts + (int64_t)(hk * G + gi) * a.q_hs)
-                       : nullptr;
+        const uint32_t* qp =
+            reinterpret_cast<const uint32_t*>(a.q + (first + t) * a.q_ts + (int64_t)(hk * G + gi) * a.q_hs);
+        const int pos = pos0 + (int)t;
+        end[mt][h] = r < nr && pos >= 0 ? pos + 1 - shift : 0;
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) qf[mt][ks][2 * j + h] = r < nr ? __ldg(qp + ks * 8 + t4 + j * 4) : 0u;
       }
-      end_lo = ps[0] < 0 ? 0 : ps[0] + 1 - shift;
-      end_hi = ps[1] < 0 ? 0 : ps[1] + 1 - shift;
-#pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) qf[ks][j] = qp[j & 1] ? __ldg(qp[j & 1] + ks * 8 + t4 + (j >> 1) * 4) : 0u;
-    }
     // numbers that every row of the warp sees: beg_all <= x < end_all (and x < sinks); that some row sees: beg_any, end_any
-    const int wr0 = warp * 16, wr1 = min(nr, wr0 + 16) - 1;
-    int beg_any = 0, end_any = 0, beg_all = 0, end_all = 0;
+    const int wr1 = min(nr, wr0 + MT * 16) - 1;
+    int beg_any = 0, end_any = 0, beg_all = -1, end_all = 0;
     if (wr0 < nr) {
       end_all = max(0, pos0 + (int)fdiv((uint32_t)(r0 + wr0), a.group) + 1 - shift);
       end_any = max(0, pos0 + (int)fdiv((uint32_t)(r0 + wr1), a.group) + 1 - shift);
@@ -367,13 +386,154 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
       }
     }
 
-    float m_lo = -CUDART_INF_F, m_hi = -CUDART_INF_F, l_lo = 0.f, l_hi = 0.f;
-    float acc[HD / 8][4];
+    // nm: minus the score a row's exponents refer to.  It is the MMAs' addend, so
+    // scores come out relative to it; 0 until the row's first key (thr = -inf)
+    float nm[MT][2], thr[MT][2], thr_min = -CUDART_INF_F, l[MT][2], acc[MT][HD / 8][4];
 #pragma unroll
-    for (int i = 0; i < HD / 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) nm[mt][h] = l[mt][h] = 0.f, thr[mt][h] = -CUDART_INF_F;
+#pragma unroll
+      for (int i = 0; i < HD / 8; ++i) acc[mt][i][0] = acc[mt][i][1] = acc[mt][i][2] = acc[mt][i][3] = 0.f;
+    }
 
+    // this lane's ldmatrix rows within 16 keys, in bytes from a step's first row
+    uint32_t k_lane[HD / 16], v_lane[HD / 16];
+#pragma unroll
+    for (int i = 0; i < HD / 16; ++i) {
+      const int kr = (lane & 7) + ((lane >> 4) << 3), vr = lane & 15;
+      k_lane[i] = (kr * HD + row_swz<HD>(kr, i * 2 + ((lane >> 3) & 1)) * 8) * 2;
+      v_lane[i] = (vr * HD + row_swz<HD>(vr, i * 2 + (lane >> 4)) * 8) * 2;
+    }
+    const uint64_t c2 = f2_dup(c), one2 = f2_dup(1.f);
+    // one step of KT keys from number x0; EDGE: some row does not see all of them
+    auto step = [&](auto edge_tag, const int x0, const int st, const bool bad) {
+      constexpr bool EDGE = decltype(edge_tag)::value;
+      const int row0 = x0 - st * KS;
+      const unsigned char* kt_s = smb + ((st & 1) * STAGE + row0 * HD) * 2;
+      const unsigned char* vt_s = kt_s + 2 * STAGE * 2;
+      float s[MT][KT / 8][4];
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+#pragma unroll
+        for (int np = 0; np < KT / 16; ++np) {
+          uint32_t kf[4];
+          ldsm_x4(kf, kt_s + k_lane[ks] + np * 16 * HD * 2);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float* d = s[mt][2 * np + j];
+              if (ks == 0) mma_rowc<T>(d, qf[mt][0], kf[2 * j], kf[2 * j + 1], nm[mt][0], nm[mt][1]);
+              else mma16<T>(d, qf[mt][ks], kf[2 * j], kf[2 * j + 1]);
+            }
+        }
+      if constexpr (EDGE) {
+        if (x0 + KT > end_all) {  // keys after some row
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const int e_lo = end[mt][0] - x0 - 2 * t4, e_hi = end[mt][1] - x0 - 2 * t4;
+#pragma unroll
+            for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (i * 8 + e >= e_lo) s[mt][i][e] = -CUDART_INF_F;
+                if (i * 8 + e >= e_hi) s[mt][i][2 + e] = -CUDART_INF_F;
+              }
+          }
+        }
+        if (window > 0 && x0 < beg_all) {  // keys before some row's window; sinks stay
+          const int sk = max(sinks - x0, 0) - 2 * t4;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const int b_lo = end[mt][0] - window - x0 - 2 * t4, b_hi = end[mt][1] - window - x0 - 2 * t4;
+#pragma unroll
+            for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                if (i * 8 + e < b_lo && i * 8 + e >= sk) s[mt][i][e] = -CUDART_INF_F;
+                if (i * 8 + e < b_hi && i * 8 + e >= sk) s[mt][i][2 + e] = -CUDART_INF_F;
+              }
+          }
+        }
+        if (bad) {
+#pragma unroll
+          for (int i = 0; i < KT / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (offs[st % 3][row0 + i * 8 + 2 * t4 + e] < 0) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) s[mt][i][e] = s[mt][i][2 + e] = -CUDART_INF_F;
+              }
+        }
+      }
+      // a row's reference moves when its maximum is more than the slack above it
+      float mx[MT][2], top = -CUDART_INF_F;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mx[mt][0] = mx[mt][1] = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) {
+          mx[mt][0] = fmax3(mx[mt][0], s[mt][i][0], s[mt][i][1]);
+          mx[mt][1] = fmax3(mx[mt][1], s[mt][i][2], s[mt][i][3]);
+        }
+        top = fmax3(top, mx[mt][0], mx[mt][1]);
+      }
+      if (__any_sync(0xffffffffu, top > thr_min)) {
+        thr_min = CUDART_INF_F;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x = mx[mt][h];
+#pragma unroll
+            for (int o = 1; o <= 2; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            const bool mv = x > thr[mt][h], fresh = thr[mt][h] == -CUDART_INF_F;
+            const float d = mv ? x : 0.f;
+            // before a row's first key O and l are zero and any finite factor will do
+            const float f = mv && !fresh ? ex2_f32(-d * c) : 1.f;
+            l[mt][h] *= f;
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) acc[mt][i][2 * h] *= f, acc[mt][i][2 * h + 1] *= f;
+#pragma unroll
+            for (int i = 0; i < KT / 8; ++i) s[mt][i][2 * h] -= d, s[mt][i][2 * h + 1] -= d;
+            if (mv) {
+              nm[mt][h] -= d;
+              thr[mt][h] = slack;
+            }
+            thr_min = fminf(thr_min, thr[mt][h]);
+          }
+      }
+      uint32_t pf[MT][KT / 16][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint64_t rs0 = 0, rs1 = 0;
+#pragma unroll
+        for (int i = 0; i < KT / 8; ++i) {
+          const uint64_t x = f2_mul(f2_pack(s[mt][i][0], s[mt][i][1]), c2), y = f2_mul(f2_pack(s[mt][i][2], s[mt][i][3]), c2);
+          const float p0 = ex2_f32(f2_lo(x)), p1 = ex2_f32(f2_hi(x)), p2 = ex2_f32(f2_lo(y)), p3 = ex2_f32(f2_hi(y));
+          rs0 = f2_fma(f2_pack(p0, p1), one2, rs0);
+          rs1 = f2_fma(f2_pack(p2, p3), one2, rs1);
+          pf[mt][i >> 1][(i & 1) * 2 + 0] = pack_p<T>(p0, p1);
+          pf[mt][i >> 1][(i & 1) * 2 + 1] = pack_p<T>(p2, p3);
+        }
+        l[mt][0] += f2_lo(rs0) + f2_hi(rs0);
+        l[mt][1] += f2_lo(rs1) + f2_hi(rs1);
+      }
+#pragma unroll
+      for (int kk = 0; kk < KT / 16; ++kk)
+#pragma unroll
+        for (int dp = 0; dp < HD / 16; ++dp) {
+          uint32_t vf[4];
+          ldsm_x4_t(vf, vt_s + v_lane[dp] + kk * 16 * HD * 2);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            mma16<T>(acc[mt][2 * dp], pf[mt][kk], vf[0], vf[1]);
+            mma16<T>(acc[mt][2 * dp + 1], pf[mt][kk], vf[2], vf[3]);
+          }
+        }
+    };
     for (int st = 0; st < nst; ++st) {
-      const int buf = st & 1;
       const bool bad_mine = bad_next;
       if (st + 1 < nst) {
         if (st > 0) __syncthreads();  // the other buffer is free
@@ -384,180 +544,71 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
         cp_async_wait<0>();
       }
       const bool bad = __syncthreads_or(bad_mine);
+      // steps some row of the warp sees: from its rows' windows (or the sinks) to their ends
+      const int x_end = min(end_any, (st + 1) * KS);
 #pragma unroll 1
-      for (int x0 = st * KS; x0 < min(n, (st + 1) * KS); x0 += KT) {
-        // no row of this warp sees a key of the step
-        if (x0 >= end_any || (x0 + KT <= beg_any && x0 >= sinks)) continue;
-        const int row0 = x0 - st * KS;
-        const T* kt_s = Ks + buf * STAGE + row0 * HD;
-        const T* vt_s = Vs + buf * STAGE + row0 * HD;
-        float s[KT / 8][4];
+      for (int x0 = st * KS; x0 < x_end; x0 += KT) {
+        if (x0 + KT <= beg_any && x0 >= sinks) continue;
+        if (x0 + KT > end_all || x0 < beg_all || bad) step(std::true_type{}, x0, st, bad);
+        else step(std::false_type{}, x0, st, false);
+      }
+    }
 #pragma unroll
-        for (int i = 0; i < KT / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int ks = 0; ks < HD / 16; ++ks)
+      for (int h = 0; h < 2; ++h) {
+        float L = l[mt][h];
 #pragma unroll
-          for (int np = 0; np < KT / 16; ++np) {
-            uint32_t kf[4];
-            const int r = np * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
-            ldsm_x4(kf, kt_s + r * HD + row_swz<HD>(r, ch) * 8);
-            mma16<T>(s[2 * np], qf[ks], kf[0], kf[1]);
-            mma16<T>(s[2 * np + 1], qf[ks], kf[2], kf[3]);
-          }
-        if (x0 + KT > end_all) {  // keys after some row
-          const int e_lo = end_lo - x0 - 2 * t4, e_hi = end_hi - x0 - 2 * t4;
-#pragma unroll
-          for (int i = 0; i < KT / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              if (i * 8 + e >= e_lo) s[i][e] = -CUDART_INF_F;
-              if (i * 8 + e >= e_hi) s[i][2 + e] = -CUDART_INF_F;
-            }
-        }
-        if (window > 0 && x0 < beg_all) {  // keys before some row's window; sinks stay
-          const int b_lo = end_lo - window - x0 - 2 * t4, b_hi = end_hi - window - x0 - 2 * t4;
-          const int sk = sinks - x0 - 2 * t4;
-          if (x0 < sinks) {
-#pragma unroll
-            for (int i = 0; i < KT / 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (i * 8 + e < b_lo && i * 8 + e >= sk) s[i][e] = -CUDART_INF_F;
-                if (i * 8 + e < b_hi && i * 8 + e >= sk) s[i][2 + e] = -CUDART_INF_F;
-              }
-          } else {
-#pragma unroll
-            for (int i = 0; i < KT / 8; ++i)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                if (i * 8 + e < b_lo) s[i][e] = -CUDART_INF_F;
-                if (i * 8 + e < b_hi) s[i][2 + e] = -CUDART_INF_F;
-              }
-          }
-        }
-        if (bad) {
-#pragma unroll
-          for (int i = 0; i < KT / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if (offs[st % 3][row0 + i * 8 + 2 * t4 + e] < 0) s[i][e] = s[i][2 + e] = -CUDART_INF_F;
-        }
-        float mt_lo = -CUDART_INF_F, mt_hi = -CUDART_INF_F;
-#pragma unroll
-        for (int i = 0; i < KT / 8; ++i) {
-          mt_lo = fmax3(mt_lo, s[i][0], s[i][1]);
-          mt_hi = fmax3(mt_hi, s[i][2], s[i][3]);
-        }
-        // the maximum moves when a row exceeds it by more than the slack; each
-        // quad's lanes decide together (-inf + slack stays -inf: a row's first key always moves it)
-        if (__any_sync(0xffffffffu, mt_lo > m_lo + thr || mt_hi > m_hi + thr)) {
-#pragma unroll
-          for (int o = 1; o <= 2; o <<= 1) {
-            mt_lo = fmaxf(mt_lo, __shfl_xor_sync(0xffffffffu, mt_lo, o));
-            mt_hi = fmaxf(mt_hi, __shfl_xor_sync(0xffffffffu, mt_hi, o));
-          }
-          const float n_lo = fmaxf(mt_lo, m_lo), n_hi = fmaxf(mt_hi, m_hi);
-          // before a row's first key O and l are zero and any finite factor will do
-          const float f_lo = m_lo != -CUDART_INF_F ? ex2_f32((m_lo - n_lo) * c) : 1.f;
-          const float f_hi = m_hi != -CUDART_INF_F ? ex2_f32((m_hi - n_hi) * c) : 1.f;
-          l_lo *= f_lo;
-          l_hi *= f_hi;
+        for (int o = 1; o <= 2; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        const int r = wr0 + mt * 16 + g + 8 * h;
+        bool nan = false;
+        if (r < nr) {
+          const uint32_t x = (uint32_t)(r0 + r), t = fdiv(x, a.group), gi = x - t * G;
+          T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + gi) * HD;
+          const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
           for (int i = 0; i < HD / 8; ++i) {
-            acc[i][0] *= f_lo; acc[i][1] *= f_lo;
-            acc[i][2] *= f_hi; acc[i][3] *= f_hi;
+            const float u = acc[mt][i][2 * h] * inv, w = acc[mt][i][2 * h + 1] * inv;
+            nan |= u != u || w != w;
+            T pair[2] = {round_f<T>(u), round_f<T>(w)};
+            *reinterpret_cast<uint32_t*>(op + i * 8 + 2 * t4) = *reinterpret_cast<uint32_t*>(pair);
           }
-          m_lo = n_lo;
-          m_hi = n_hi;
         }
-        // rows without a key yet subtract 0: 2^-inf = 0
-        const float sub_lo = m_lo == -CUDART_INF_F ? 0.f : -m_lo * c, sub_hi = m_hi == -CUDART_INF_F ? 0.f : -m_hi * c;
-        const uint64_t c2 = f2_dup(c), b_lo = f2_dup(sub_lo), b_hi = f2_dup(sub_hi), one2 = f2_dup(1.f);
-        uint64_t rs_lo = 0, rs_hi = 0;
-        uint32_t pf[KT / 16][4];
-#pragma unroll
-        for (int i = 0; i < KT / 8; ++i) {
-          const uint64_t x = f2_fma(f2_pack(s[i][0], s[i][1]), c2, b_lo), y = f2_fma(f2_pack(s[i][2], s[i][3]), c2, b_hi);
-          const float p0 = ex2_f32(f2_lo(x)), p1 = ex2_f32(f2_hi(x)), p2 = ex2_f32(f2_lo(y)), p3 = ex2_f32(f2_hi(y));
-          rs_lo = f2_fma(f2_pack(p0, p1), one2, rs_lo);
-          rs_hi = f2_fma(f2_pack(p2, p3), one2, rs_hi);
-          pf[i >> 1][(i & 1) * 2 + 0] = pack_p<T>(p0, p1);
-          pf[i >> 1][(i & 1) * 2 + 1] = pack_p<T>(p2, p3);
-        }
-        l_lo += f2_lo(rs_lo) + f2_hi(rs_lo);
-        l_hi += f2_lo(rs_hi) + f2_hi(rs_hi);
-#pragma unroll
-        for (int kk = 0; kk < KT / 16; ++kk)
-#pragma unroll
-          for (int dp = 0; dp < HD / 16; ++dp) {
-            uint32_t vf[4];
-            const int r = kk * 16 + (lane & 15), ch = dp * 2 + (lane >> 4);
-            ldsm_x4_t(vf, vt_s + r * HD + row_swz<HD>(r, ch) * 8);
-            mma16<T>(acc[2 * dp], pf[kk], vf[0], vf[1]);
-            mma16<T>(acc[2 * dp + 1], pf[kk], vf[2], vf[3]);
-          }
-      }
-    }
-    bool nan[2] = {false, false};
-#pragma unroll
-    for (int o = 1; o <= 2; o <<= 1) {
-      l_lo += __shfl_xor_sync(0xffffffffu, l_lo, o);
-      l_hi += __shfl_xor_sync(0xffffffffu, l_hi, o);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = rr + 8 * h;
-      if (r < nr) {
-        const uint32_t x = (uint32_t)(r0 + r), t = fdiv(x, a.group), gi = x - t * G;
-        T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + gi) * HD;
-        const float l = h ? l_hi : l_lo, inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int i = 0; i < HD / 8; ++i) {
-          const float u = acc[i][2 * h] * inv, w = acc[i][2 * h + 1] * inv;
-          nan[h] |= u != u || w != w;
-          T pair[2] = {round_f<T>(u), round_f<T>(w)};
-          *reinterpret_cast<uint32_t*>(op + i * 8 + 2 * t4) = *reinterpret_cast<uint32_t*>(pair);
+        unsigned again = __ballot_sync(0xffffffffu, nan);
+        while (again) {
+          const int q = (__ffs(again) - 1) >> 2;  // the lane quad of a row
+          again &= ~(15u << (4 * q));
+          const uint32_t x = (uint32_t)(r0 + wr0 + mt * 16 + 8 * h + q), t = fdiv(x, a.group), gi = x - t * G;
+          prefill_row_again<T, HD>(a, b, hk, a.q + (first + t) * a.q_ts + (int64_t)(hk * G + gi) * a.q_hs, pos0 + (int)t,
+                                   a.o + ((first + t) * Hq + (int64_t)hk * G + gi) * HD);
         }
       }
-    }
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      unsigned again = __ballot_sync(0xffffffffu, nan[h]);
-      while (again) {
-        const int q = (__ffs(again) - 1) >> 2;  // the lane quad of a row
-        again &= ~(15u << (4 * q));
-        const uint32_t x = (uint32_t)(r0 + warp * 16 + 8 * h + q), t = fdiv(x, a.group), gi = x - t * G;
-        prefill_row_again<T, HD>(a, b, hk, a.q + (first + t) * a.q_ts + (int64_t)(hk * G + gi) * a.q_hs, pos0 + (int)t,
-                                 a.o + ((first + t) * Hq + (int64_t)hk * G + gi) * HD);
-      }
-    }
   }
 }
 
-template <typename T, int HD, int W, int KS, int MINB>
+template <typename T, int HD, int W, int MT, int KT, int KS, int MINB>
 static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
   constexpr int smem = 4 * KS * HD * 2;
-  auto* kern = paged_prefill_mma_kernel<T, HD, W, KS, MINB>;
+  auto* kern = paged_prefill_mma_kernel<T, HD, W, MT, KT, KS, MINB>;
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
-  const int64_t tiles = ((int64_t)max_q * a.group.d + W * 16 - 1) / (W * 16);
+  const int64_t tiles = ((int64_t)max_q * a.group.d + W * MT * 16 - 1) / (W * MT * 16);
   kern<<<dim3((unsigned)tiles, a.kv_heads, B), W * 32, smem, s>>>(a);
   return launch_status();
 }
-#ifndef PF_W16
-#define PF_W16 4
-#define PF_S16 128
-#define PF_B16 5
-#define PF_W32 4
-#define PF_S32 128
-#define PF_B32 4
-#endif
+
+// Warps, 16-row tiles per warp, keys per step and per stage, CTAs per SM.
+// Measured on one GPU: 16 channels (8 x 2048 tokens, 32 heads, window 512):
+// (4, 1, 64, 128, 5) 149 us, (8, 1, 32, 256, 3) 148, (4, 2, 32, 128, 5) 148,
+// (8, 1, 64, 128, 2) 177, and 4.4 against 5.1 - 5.5 us for a few short
+// prompts; 32 channels (3 later parts of 3500, 64 heads, window 1024): (4, 2,
+// 32, 256, 3) 199 us, (4, 2, 32, 128, 4) 208, (4, 1, 64, 128, 4) 213.
 template <typename T, int HD>
 static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
-  if constexpr (HD == 16) return launch_prefill_tile<T, HD, PF_W16, PF_S16, PF_B16>(a, B, max_q, s);
-  else if constexpr (HD == 32) return launch_prefill_tile<T, HD, PF_W32, PF_S32, PF_B32>(a, B, max_q, s);
-  else if constexpr (HD == 64) return launch_prefill_tile<T, HD, 4, 64, 3>(a, B, max_q, s);
-  else return launch_prefill_tile<T, HD, 4, 64, 2>(a, B, max_q, s);
+  if constexpr (HD == 16) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 5>(a, B, max_q, s);
+  else if constexpr (HD == 32) return launch_prefill_tile<T, HD, 4, 2, 32, 256, 3>(a, B, max_q, s);
+  else if constexpr (HD == 64) return launch_prefill_tile<T, HD, 4, 1, 64, 64, 3>(a, B, max_q, s);
+  else return launch_prefill_tile<T, HD, 4, 1, 64, 64, 2>(a, B, max_q, s);
 }
 
 template <typename T, int HD>
