@@ -1,7 +1,5 @@
 """What the serving entry points refuse, on the host before any launch (no
 GPU: the pointers are never used)."""
-import ctypes
-
 import pytest
 import torch
 
@@ -10,12 +8,16 @@ from walsh_research_b200 import _lib, ops
 P16 = 1 << 12  # a 16-byte aligned address that is never dereferenced
 
 
+KV_FIELDS = ("k_pages", "v_pages", "dtype", "n_pages", "kv_heads", "page_size", "head_dim", "page_stride", "head_stride",
+             "row_stride", "page_table", "table_stride", "table_cols", "kv_lens", "window", "sinks", "scale", "err")
+
+
 def kv(**kw):
     d = dict(k_pages=P16, v_pages=P16, dtype=2, n_pages=4, kv_heads=2, page_size=16, head_dim=32, page_stride=1024,
              head_stride=512, row_stride=32, page_table=P16, table_stride=3, table_cols=3, kv_lens=P16, window=0,
              sinks=0, scale=0.25, err=None)
     d.update(kw)
-    return ctypes.byref(_lib.PagedKV(*[d[n] for n, _ in _lib.PagedKV._fields_]))
+    return _lib.PAGED_KV.pack(*[d[n] or 0 for n in KV_FIELDS])
 
 
 def attn(k, q=P16, q_bs=128, q_hs=32, B=2, hq=4, max_len=48, scratch=P16, o=P16):

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from ctypes import c_float, c_int, c_int64, c_void_p
 
 import torch
@@ -122,12 +123,12 @@ class MoeRouting(ctypes.Structure):
     _fields_ = [("mode", c_int), ("min_experts", c_int), ("threshold", c_float)]
 
 
-class PagedKV(ctypes.Structure):
-    """walsh_paged_kv: one layer of a paged key/value cache."""
-    _fields_ = [("k_pages", P), ("v_pages", P), ("dtype", c_int), ("n_pages", c_int), ("kv_heads", c_int),
-                ("page_size", c_int), ("head_dim", c_int), ("page_stride", c_int64), ("head_stride", c_int64),
-                ("row_stride", c_int64), ("page_table", P), ("table_stride", c_int64), ("table_cols", c_int),
-                ("kv_lens", P), ("window", c_int), ("sinks", c_int), ("scale", c_float), ("err", P)]
+# walsh_paged_kv, one layer of a paged key/value cache, packed to bytes (passed
+# where its pointer is expected): k_pages, v_pages, dtype, n_pages, kv_heads,
+# page_size, head_dim, page_stride, head_stride, row_stride, page_table,
+# table_stride, table_cols, kv_lens, window, sinks, scale, err.  Packing costs
+# a few hundred nanoseconds where filling a ctypes structure costs microseconds.
+PAGED_KV = struct.Struct("@PPiiiiiqqqPqiPiifP")
 
 
 class WalshError(RuntimeError):
@@ -181,14 +182,14 @@ def ptr(t):
     return t.data_ptr()
 
 
+_DCODE = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
+
+
 def dcode(dtype: torch.dtype) -> int:
-    if dtype == torch.float32:
-        return F32
-    if dtype == torch.bfloat16:
-        return BF16
-    if dtype == torch.float16:
-        return F16
-    raise TypeError(f"walsh kernels take float32, bfloat16 or float16 activations, got {dtype}")
+    code = _DCODE.get(dtype)
+    if code is None:
+        raise TypeError(f"walsh kernels take float32, bfloat16 or float16 activations, got {dtype}")
+    return code
 
 
 def inner_dtype(stream_dtype: torch.dtype) -> torch.dtype:

@@ -8,6 +8,7 @@ anything on the host.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -578,82 +579,104 @@ def rmsnorm(x, w, eps=1e-6, out_dtype=None):
 # serving: paged key/value cache and token sampling
 # ---------------------------------------------------------------------------
 
-def _call_on(t, name, *args):
-    """call(name, *args, stream) on t's device and its current stream."""
-    if t.device.index == torch._C._cuda_getDevice():
-        return call(name, *args, stream())
-    with torch.cuda.device(t.device):
-        return call(name, *args, stream())
-
-
-def _same_device(first, *tensors):
-    require_cuda(first, *tensors)
+def _device_of(first, *tensors):
+    """Index of the CUDA device that holds all the given tensors (None skipped)."""
+    dev = first.get_device()
     for t in tensors:
-        if t is not None and t.device != first.device:
+        if t is not None and t.get_device() != dev:
+            require_cuda(first, t)
             raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+    if dev < 0:
+        require_cuda(first)
+    return dev
+
+
+def _call_on(dev, name, *args):
+    """call(name, *args, stream) on device ``dev`` and its current stream."""
+    if dev < 0 or dev == torch._C._cuda_getDevice():
+        return call(name, *args, stream())
+    with torch.cuda.device(dev):
+        return call(name, *args, stream())
 
 
 def _head_rows(x, heads, hd, dtype, what):
-    """x [N, heads, hd] and its token and head strides, copied when a row is
-    not contiguous or not on 16-byte boundaries."""
-    if x.dim() != 3 or x.shape[2] != hd or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{what} has shape {tuple(x.shape)}; expected [N, {heads or 'heads'}, {hd}]")
+    """x [N, heads, hd] with its address, token and head strides, copied when a
+    row is not contiguous or not on 16-byte boundaries."""
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != hd or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{what} has shape {tuple(shape)}; expected [N, {heads or 'heads'}, {hd}]")
     if x.dtype != dtype:
         raise ValueError(f"{what} is {x.dtype}; the pages are {dtype}")
-    vec = 16 // x.element_size()
-    n, h, _ = x.shape
+    mask = 3 if dtype == torch.float32 else 7
     st, sh, sd = x.stride()
-    if sd != 1 or (st % vec and n > 1) or (sh % vec and h > 1):
+    if shape[0] <= 1:
+        st = 0
+    if shape[1] <= 1:
+        sh = 0
+    if sd != 1 or (st | sh) & mask:
         x = x.contiguous()
-        st, sh, sd = x.stride()
-    if x.data_ptr() % 16:
+        st, sh = (shape[1] * hd if shape[0] > 1 else 0), (hd if shape[1] > 1 else 0)
+    p = x.data_ptr()
+    if p & 15:
         x = x.clone(memory_format=torch.contiguous_format)
-        st, sh, sd = x.stride()
-    return x, (st if n > 1 else 0), (sh if h > 1 else 0)
+        st, sh, p = (shape[1] * hd if shape[0] > 1 else 0), (hd if shape[1] > 1 else 0), x.data_ptr()
+    return x, p, st, sh
 
 
-def _index_vector(x, n, what, dtypes=(torch.int32,)):
-    if x.dtype not in dtypes or x.dim() != 1 or x.shape[0] != n:
+_INT32 = (torch.int32,)
+_INTS = (torch.int32, torch.int64)
+
+
+def _index_vector(x, n, what, dtypes=_INT32):
+    if x.dtype not in dtypes or x.shape != (n,):
         raise ValueError(f"{what} must be {' or '.join(str(d)[6:] for d in dtypes)} [{n}], got {x.dtype} {tuple(x.shape)}")
     return _c(x)
 
 
 def _out_rows(out, like, shape):
-    if out is None:
-        return torch.empty(shape, dtype=like.dtype, device=like.device)
+    if out is None:  # (of a view, empty_like would keep the strides)
+        return torch.empty_like(like) if like.is_contiguous() else torch.empty(shape, dtype=like.dtype, device=like.device)
     if out.shape != shape or out.dtype != like.dtype or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {like.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
     return out
 
 
 def _paged_kv(k_pages, v_pages, page_table=None, kv_lens=None, window=0, sinks=0, scale=None, err=None):
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+    """walsh_paged_kv of the given tensors, as bytes (see _lib.PAGED_KV)."""
+    shape, strides, dtype = k_pages.shape, k_pages.stride(), k_pages.dtype
+    if len(shape) != 4 or shape != v_pages.shape or dtype != v_pages.dtype:
         raise ValueError(f"k_pages and v_pages must be alike [n_pages, kv_heads, page_size, hd], got "
-                         f"{tuple(k_pages.shape)} {k_pages.dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
-    if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+                         f"{tuple(shape)} {dtype} and {tuple(v_pages.shape)} {v_pages.dtype}")
+    if strides != v_pages.stride() or strides[3] != 1:
         raise ValueError("k_pages and v_pages must have the same strides and contiguous rows")
-    n, h, ps, hd = k_pages.shape
-    sp, sh, sr, _ = k_pages.stride()
-    kv = _lib.PagedKV(k_pages.data_ptr(), v_pages.data_ptr(), dcode(k_pages.dtype), n, h, ps, hd,
-                      sp if n > 1 else 0, sh if h > 1 else 0, sr if ps > 1 else hd)
+    n, h, ps, hd = shape
+    sp, sh, sr, _ = strides
+    e = 0
     if err is not None:
         if err.dtype != torch.int32 or err.numel() != 1:
             raise ValueError("err must be one int32")
-        kv.err = err.data_ptr()
+        e = err.data_ptr()
+    tab = ts = cols = lens = 0
     if page_table is not None:
-        if page_table.dtype != torch.int32 or page_table.dim() != 2 or (page_table.shape[1] > 1
-                                                                       and page_table.stride(1) != 1):
-            raise ValueError(f"page_table must be int32 [B, columns] with contiguous rows, got {page_table.dtype} "
-                             f"{tuple(page_table.shape)}")
+        size = page_table.shape
+        if page_table.dtype != torch.int32 or len(size) != 2:
+            raise ValueError(f"page_table must be int32 [B, columns], got {page_table.dtype} {tuple(size)}")
+        rows, cols = size
+        ts, tc = page_table.stride()
+        if cols > 1 and tc != 1:
+            raise ValueError("page_table must have contiguous rows")
+        if kv_lens.dtype != torch.int32 or kv_lens.shape != size[:1] or not kv_lens.is_contiguous():
+            raise ValueError(f"kv_lens must be contiguous int32 [{rows}], got {kv_lens.dtype} {tuple(kv_lens.shape)}")
         if window < 0 or sinks < 0:
             raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
-        kv.page_table = page_table.data_ptr()
-        kv.table_stride = page_table.stride(0) if page_table.shape[0] > 1 else 0
-        kv.table_cols = page_table.shape[1]
-        kv.kv_lens = kv_lens.data_ptr()
-        kv.window, kv.sinks = int(window), int(sinks)
-        kv.scale = hd ** -0.5 if scale is None else float(scale)
-    return kv
+        tab, lens = page_table.data_ptr(), kv_lens.data_ptr()
+        if rows <= 1:
+            ts = 0
+        if scale is None:
+            scale = hd ** -0.5
+    return _lib.PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), dcode(dtype), n, h, ps, hd,
+                              sp if n > 1 else 0, sh if h > 1 else 0, sr if ps > 1 else hd, tab, ts, cols, lens,
+                              min(window, 0x7fffffff), min(sinks, 0x7fffffff), scale or 0.0, e)
 
 
 def paged_append(q, k, v, k_pages, v_pages, slots, positions=None, rope=None, q_norm=None, k_norm=None, eps=1e-6,
@@ -668,44 +691,56 @@ def paged_append(q, k, v, k_pages, v_pages, slots, positions=None, rope=None, q_
     q|k|v, or head-major).  Slots must be distinct.  ``err`` (int32 [1])
     becomes nonzero when a slot or position is out of range; such a token is
     not stored and its q_out row is zero (for a position).  One launch."""
-    _same_device(k_pages, v_pages, q, k, v, slots, positions, q_norm, k_norm, q_out, err)
+    dev = _device_of(k_pages, v_pages, q, k, v, slots, positions, q_norm, k_norm, q_out, err)
     kv = _paged_kv(k_pages, v_pages, err=err)
-    hk, hd, dt = k_pages.shape[1], k_pages.shape[3], k_pages.dtype
-    k, k_ts, k_hs = _head_rows(k, hk, hd, dt, "k")
-    v, v_ts, v_hs = _head_rows(v, hk, hd, dt, "v")
+    _, hk, _, hd = k_pages.shape
+    dt = k_pages.dtype
+    k, kp, k_ts, k_hs = _head_rows(k, hk, hd, dt, "k")
+    v, vp, v_ts, v_hs = _head_rows(v, hk, hd, dt, "v")
     n = k.shape[0]
     hq = q_ts = q_hs = 0
+    qp = None
     if q is not None:
-        q, q_ts, q_hs = _head_rows(q, None, hd, dt, "q")
+        q, qp, q_ts, q_hs = _head_rows(q, None, hd, dt, "q")
         hq = q.shape[1]
-        q_out = _out_rows(q_out, q, (n, hq, hd))
+        q_out = _out_rows(q_out, q, (q.shape[0], hq, hd))
     elif q_out is not None or q_norm is not None:
         raise ValueError("q_out and q_norm need q")
     if v.shape[0] != n or (q is not None and q.shape[0] != n):
         raise ValueError("q, k and v must have the same number of tokens")
-    slots = _index_vector(slots, n, "slots", (torch.int32, torch.int64))
+    slots = _index_vector(slots, n, "slots", _INTS)
     cos = sin = None
+    n_pos = 0
     if (positions is None) != (rope is None):
         raise ValueError("positions and rope go together")
     if positions is not None:
-        positions = _index_vector(positions, n, "positions", (torch.int32, torch.int64))
+        positions = _index_vector(positions, n, "positions", _INTS)
         if positions.dtype != slots.dtype:
             positions = positions.to(slots.dtype)
         cos, sin = rope
-        _same_device(k_pages, cos, sin)
+        _device_of(k_pages, cos, sin)
         if (cos.dim() != 2 or cos.shape[1] != hd // 2 or cos.shape != sin.shape or cos.dtype != torch.float32
                 or sin.dtype != torch.float32):
             raise ValueError(f"rope must be two float32 [n_pos, {hd // 2}] tables")
         cos, sin = _c(cos), _c(sin)
+        n_pos = cos.shape[0]
     for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
         if w is not None and (w.dtype != torch.float32 or w.shape != (hd,) or not w.is_contiguous()):
             raise ValueError(f"{what} must be contiguous float32 [{hd}]")
     if n == 0:
         return q_out
-    _call_on(k_pages, "walsh_paged_append", ctypes.byref(kv), ptr(q), q_ts, q_hs, ptr(k), k_ts, k_hs, ptr(v), v_ts,
-             v_hs, n, hq, ptr(slots), ptr(positions), 1 if slots.dtype == torch.int64 else 0, ptr(cos), ptr(sin),
-             0 if cos is None else cos.shape[0], ptr(q_norm), ptr(k_norm), float(eps), ptr(q_out))
+    _call_on(dev, "walsh_paged_append", kv, qp, q_ts, q_hs, kp, k_ts, k_hs, vp, v_ts, v_hs, n, hq, slots.data_ptr(),
+             ptr(positions), slots.dtype == torch.int64, ptr(cos), ptr(sin), n_pos, ptr(q_norm), ptr(k_norm), eps,
+             ptr(q_out))
     return q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _attn_scratch_bytes(dtype_code, kv_heads, hd, window, sinks, B, hq, max_len):
+    """walsh_paged_attn_scratch_bytes, which depends on these alone (the pages of
+    the description passed on are never looked at)."""
+    kv = _lib.PAGED_KV.pack(16, 16, dtype_code, 1, kv_heads, 1, hd, 0, 0, hd, 16, 0, 1, 16, window, sinks, 1.0, 0)
+    return call("walsh_paged_attn_scratch_bytes", kv, B, hq, max_len)
 
 
 def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, window=0, sinks=0, scale=None, out=None,
@@ -720,23 +755,21 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, wind
     Sequences of length 0 give zeros.  ``err`` (int32 [1]) becomes nonzero
     when a page id or length is out of range; keys of such a page are not
     seen."""
-    _same_device(k_pages, v_pages, q, page_table, kv_lens, out, err)
+    dev = _device_of(k_pages, v_pages, q, page_table, kv_lens, out, err)
     kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
-    q, q_bs, q_hs = _head_rows(q, None, k_pages.shape[3], k_pages.dtype, "q")
-    B, hq, _ = q.shape
-    _index_vector(kv_lens, B, "kv_lens")
-    if page_table.shape[0] != B or not kv_lens.is_contiguous():
-        raise ValueError(f"{B} queries, a page table of {page_table.shape[0]} rows and kv_lens of stride "
-                         f"{kv_lens.stride(0)}")
-    out = _out_rows(out, q, q.shape)
+    _, hk, ps, hd = k_pages.shape
+    q, qp, q_bs, q_hs = _head_rows(q, None, hd, k_pages.dtype, "q")
+    B, hq, _ = shape = q.shape
+    if page_table.shape[0] != B:
+        raise ValueError(f"{B} queries and a page table of {page_table.shape[0]} rows")
+    out = _out_rows(out, q, shape)
     if B == 0:
         return out
     if max_len is None:
-        max_len = page_table.shape[1] * k_pages.shape[2]
-    nbytes = call("walsh_paged_attn_scratch_bytes", ctypes.byref(kv), B, hq, int(max_len))
+        max_len = page_table.shape[1] * ps
+    nbytes = _attn_scratch_bytes(dcode(q.dtype), hk, hd, window, sinks, B, hq, max_len)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
-    _call_on(q, "walsh_paged_attn_fwd", ctypes.byref(kv), ptr(q), q_bs, q_hs, B, hq, int(max_len), ptr(scratch),
-             ptr(out))
+    _call_on(dev, "walsh_paged_attn_fwd", kv, qp, q_bs, q_hs, B, hq, max_len, ptr(scratch), out.data_ptr())
     return out
 
 
@@ -748,20 +781,17 @@ def paged_prefill_attention(q, q_offsets, k_pages, v_pages, page_table, kv_lens,
     kv_len - T + t).  Pages, lengths, window, sinks, scale and err as in
     paged_attention; ``max_q`` bounds the spans on the host (default N).  Rows
     of ``out`` outside every span are left as they are."""
-    _same_device(k_pages, v_pages, q, q_offsets, page_table, kv_lens, out, err)
+    dev = _device_of(k_pages, v_pages, q, q_offsets, page_table, kv_lens, out, err)
     kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
-    q, q_ts, q_hs = _head_rows(q, None, k_pages.shape[3], k_pages.dtype, "q")
-    n, hq, _ = q.shape
+    q, qp, q_ts, q_hs = _head_rows(q, None, k_pages.shape[3], k_pages.dtype, "q")
+    n, hq, _ = shape = q.shape
     B = page_table.shape[0]
-    _index_vector(kv_lens, B, "kv_lens")
     q_offsets = _index_vector(q_offsets, B + 1, "q_offsets")
-    if not kv_lens.is_contiguous():
-        raise ValueError("kv_lens must be contiguous")
-    out = _out_rows(out, q, q.shape)
+    out = _out_rows(out, q, shape)
     if n == 0 or B == 0:
         return out
-    _call_on(q, "walsh_paged_prefill_fwd", ctypes.byref(kv), ptr(q), q_ts, q_hs, n, ptr(q_offsets), B, hq,
-             n if max_q is None else min(int(max_q), n), ptr(out))
+    _call_on(dev, "walsh_paged_prefill_fwd", kv, qp, q_ts, q_hs, n, q_offsets.data_ptr(), B, hq,
+             n if max_q is None else min(max_q, n), out.data_ptr())
     return out
 
 
@@ -792,7 +822,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     kv, kr = _row_param(top_k, rows, torch.int32, "top_k")
     pv, pr = _row_param(top_p, rows, torch.float32, "top_p")
     mv, mr = _row_param(min_p, rows, torch.float32, "min_p")
-    _same_device(logits, uniforms, tr, kr, pr, mr)
+    dev = _device_of(logits, uniforms, tr, kr, pr, mr)
     if not tv >= 0 or pv != pv or mv != mv:
         raise ValueError(f"temperature must be >= 0 and top_p, min_p numbers, got {tv}, {pv}, {mv}")
     if uniforms.dtype != torch.float32 or uniforms.shape != (rows,):
@@ -801,8 +831,8 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
         logits = logits.contiguous()
     uniforms = _c(uniforms)
     ids = torch.empty(rows, dtype=torch.int64, device=logits.device)
-    logp = torch.empty(rows, dtype=torch.float32, device=logits.device) if want_logprob else None
-    _call_on(logits, "walsh_sample_tokens", ptr(logits), dcode(logits.dtype), logits.stride(0) if rows > 1 else 0,
-             rows, vocab, ptr(uniforms), float(tv), max(0, min(int(kv), vocab)), float(pv), float(mv), ptr(tr), ptr(kr),
-             ptr(pr), ptr(mr), ptr(ids), ptr(logp))
+    logp = torch.empty_like(uniforms) if want_logprob else None
+    _call_on(dev, "walsh_sample_tokens", logits.data_ptr(), dcode(logits.dtype), logits.stride(0) if rows > 1 else 0,
+             rows, vocab, uniforms.data_ptr(), tv, max(0, min(kv, vocab)), pv, mv, ptr(tr), ptr(kr), ptr(pr), ptr(mr),
+             ids.data_ptr(), ptr(logp))
     return (ids, logp) if want_logprob else ids
