@@ -16,6 +16,8 @@
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "mma.cuh"
 #include "paged.cuh"
@@ -84,28 +86,31 @@ __device__ __forceinline__ u64 fixed(double w) { return __double2ull_rn(w * kWei
 
 constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kBins = 1024;      // bins of the mass histogram
-constexpr int kCands = 512;      // tokens resolved one by one at a top-p border
-constexpr int kList = 2048;      // tokens of a top-k list (sorted in shared memory)
+constexpr int kCands = 256;      // tokens resolved one by one at a top-p border
+constexpr int kList = 1024;      // tokens of a top-k list
 constexpr int kListTopK = 512;   // largest top_k that goes by the list
+constexpr int kPairs = 256;      // lists up to this long are ranked by comparing all pairs, longer ones sorted
 
 struct SampleShared {
   union {
     struct {
-      uint32_t maxima[2 * kSampleThreads];
+      uint32_t maxima[2 * kSampleThreads];  // of the halves of a thread's chunks
+      uint32_t warp_max[kSampleWarps], oct_max[4 * kSampleWarps];
       u64 list[kList];
     } k;
     struct {
-      uint32_t hist[kBins];
-      u64 cand[kCands], all[kCands];
-      uint8_t from[kCands];
+      float queue[kSampleWarps][64];
+      u64 cand[kCands];  // this CTA's tokens at the border
+      union {
+        uint32_t hist[kBins];
+        struct {
+          u64 all[kCands], wt[kCands];  // the whole row's
+        };
+        u64 mass[256];
+      };
     } p;
-    struct {
-      u64 mass[256];
-      uint32_t count[256];
-    } r;
   };
-  float queue[kSampleWarps][64];
-  u64 w_keep[kSampleWarps], w_all[kSampleWarps], scratch[kSampleWarps];
+  u64 w_keep[kSampleWarps], w_all[kSampleWarps], scratch[kSampleWarps], step[32], add[8];
   double w_sum[kSampleWarps], w_err[kSampleWarps];
   // what other CTAs of the cluster read
   u64 cta_keep, cta_all, cta_ties;
@@ -113,7 +118,14 @@ struct SampleShared {
   uint32_t cta_max, n;
   // what the CTA that finds it writes into every CTA
   int tie_index, uncertain;
+  u64 thr;
 };
+
+// bits of two or one -inf values
+template <typename T> __device__ __forceinline__ uint32_t neg_inf_word();
+template <> __device__ __forceinline__ uint32_t neg_inf_word<float>() { return 0xff800000u; }
+template <> __device__ __forceinline__ uint32_t neg_inf_word<__half>() { return 0xfc00fc00u; }
+template <> __device__ __forceinline__ uint32_t neg_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
 
 // One cluster of CS CTAs per row, each holding a contiguous part of the row in
 // shared memory; each warp owns a contiguous part of that, so index order is
@@ -141,6 +153,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   int top_k = a.top_k_r ? a.top_k_r[row] : a.top_k;
   if (top_k <= 0 || top_k > V) top_k = V;
   const bool greedy = !(temp > 0.0) || top_k == 1;
+  const bool by_list = top_k < V && top_k <= kListTopK, by_mass = top_k == V && top_p < 1.0;
   const double c = temp > 0.0 ? 1.4426950408889634074 / temp : 1.0;
   const float cf = fminf(fmaxf((float)c, 1.2e-38f), 3e38f);
 
@@ -149,7 +162,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   const int mis = (int)(((uintptr_t)lg & 15) / sizeof(T));
   const int chunks = (mis + V + VEC - 1) / VEC, per_cta = (chunks + CS - 1) / CS;
   const int c0 = rank * per_cta, nch = max(0, min(per_cta, chunks - c0));
-  const int per_warp = (nch + NW - 1) / NW;
+  const int per_warp = max(1, (nch + NW - 1) / NW);
   const int wbeg = min(nch, warp * per_warp), wend = min(nch, wbeg + per_warp);
   const int base = c0 * VEC - mis;  // token of the part's first element (negative: before the row)
   float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
@@ -191,13 +204,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       }
     }
   }
-  // f(value, token) for this lane's elements of the warp's part, in order of the
-  // warp's steps; every lane makes the same number of calls (in = false: no element)
+  // 16 bytes of the part; past a warp's chunks (and around the row) -inf
+  auto chunk = [&](int ch, int end) -> uint4 {
+    if (ch < end) return *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
+    const uint32_t w = neg_inf_word<T>();
+    return make_uint4(w, w, w, w);
+  };
+  // f(value, token, is one) for the elements of the warp's chunks; every lane makes the same number of calls
   auto each = [&](auto f) {
     for (int ch0 = wbeg; ch0 < wend; ch0 += 32) {
       const int ch = ch0 + lane;
-      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-      if (ch < wend) raw = *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
+      const uint4 raw = chunk(ch, wend);
       const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -207,19 +224,82 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
   };
   auto composite = [](float v, int t) { return ((u64)float_key(v + 0.f) << 32) | (0xffffffffu - (unsigned)t); };
+  auto warp_sum64 = [&](u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto warp_sumd = [&](double v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  // sums over the block of one value per thread
+  auto block_sum = [&](u64 v) {
+    v = warp_sum64(v);
+    __syncthreads();
+    if (lane == 0) sh.scratch[warp] = v;
+    __syncthreads();
+    v = sh.scratch[lane % NW];
+#pragma unroll
+    for (int o = NW / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto block_sum32 = [&](unsigned v) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if (lane == 0) sh.scratch[warp] = v;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, lane < NW ? (unsigned)sh.scratch[lane] : 0u);
+  };
+  // inclusive prefix sum over the block's threads
+  auto block_scan = [&](u64 v, u64* total) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh.scratch[warp] = v;
+    __syncthreads();
+    u64 s = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      if (w == warp) before = s;
+      s += sh.scratch[w];
+    }
+    *total = s;
+    return v + before;
+  };
 
-  // ---- maximum of the row
+  // ---- maximum of the row, and for top-p a lower bound of Z
   const uint32_t mk0 = float_key(mx0 + 0.f), mk1 = float_key(mx1 + 0.f);
   {
     const uint32_t wm = __reduce_max_sync(0xffffffffu, max(mk0, mk1));
-    sh.k.maxima[tid] = mk0;
-    sh.k.maxima[NT + tid] = mk1;
+    if (by_list) {
+      sh.k.maxima[tid] = mk0;
+      sh.k.maxima[NT + tid] = mk1;
+      const uint32_t om = __reduce_max_sync(0xffu << (lane & 24), max(mk0, mk1));
+      if ((lane & 7) == 0) sh.k.oct_max[tid >> 3] = om;
+      if (lane == 0) sh.k.warp_max[warp] = wm;
+    }
     if (lane == 0) sh.scratch[warp] = wm;
     if (tid == 0) sh.n = 0, sh.uncertain = 0;
+    if (tid < 8) sh.add[tid] = 0;
     __syncthreads();
-    if (warp == 0) {
-      const uint32_t cm = __reduce_max_sync(0xffffffffu, lane < NW ? (uint32_t)sh.scratch[lane] : 0u);
-      if (lane == 0) sh.cta_max = cm;
+    const uint32_t cm = __reduce_max_sync(0xffffffffu, (uint32_t)sh.scratch[lane % NW]);
+    if (tid == 0) sh.cta_max = cm;
+    if (by_mass) {  // the sum of the threads' largest weights, relative to this part's largest
+      const float f = key_float(cm);
+      float z = f > -CUDART_INF_F && f < CUDART_INF_F ? ex2_f32((mx0 - f) * cf) + ex2_f32((mx1 - f) * cf) : 0.f;
+      z = warp_sum(z);
+      if (lane == 0) sh.w_sum[warp] = z;
+      __syncthreads();
+      if (tid == 0) {
+        double s = 0.0;
+        for (int w = 0; w < NW; ++w) s += sh.w_sum[w];
+        sh.cta_sum = s;
+      }
     }
   }
   all_sync();
@@ -235,16 +315,28 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     all_sync();
     return;
   }
+  bool general = top_k < V && !by_list;
+  float z_low = 0.f, z_high = (float)V;
+  if (by_mass) {
+#pragma unroll
+    for (int r = 0; r < CS; ++r) {
+      const float f = key_float(peer(r)->cta_max);
+      if (f > -CUDART_INF_F) z_low += (float)peer(r)->cta_sum * ex2_f32((f - m) * cf);
+    }
+    // Z is at most that sum times the elements behind one of the maxima
+    z_high = fminf(z_high, fmaxf(z_low, 1.f) * 1.001f * (float)((per_warp + 31) / 32 * (VEC / 2)));
+    z_low = fmaxf(z_low * 0.999f, 1.f);
+  }
   if (m == CUDART_INF_F && !greedy) {  // the +inf logits share the weight, nothing else has any
+    all_sync();
     for (int i = tid; i < nch * VEC; i += NT)
       seg[i] = to_f(seg[i]) == CUDART_INF_F ? round_f<T>(0.f) : round_f<T>(-CUDART_INF_F);
     m = 0.f;
     kmax = float_key(0.f);
-    const bool i0 = mx0 == CUDART_INF_F, i1 = mx1 == CUDART_INF_F;
-    all_sync();
-    sh.k.maxima[tid] = float_key(i0 ? 0.f : -CUDART_INF_F);
-    sh.k.maxima[NT + tid] = float_key(i1 ? 0.f : -CUDART_INF_F);
-    all_sync();
+    z_low = 1.f;
+    z_high = (float)V;
+    general |= top_k < V;  // (the list's maxima are of the logits as they were)
+    __syncthreads();
   }
   const double u = (double)a.u[row];
   auto finish = [&](int id, double w, double z) {
@@ -273,37 +365,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     return;
   }
 
-  // sum over the block of one value per thread
-  auto block_sum = [&](u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    __syncthreads();
-    if (lane == 0) sh.scratch[warp] = v;
-    __syncthreads();
-    u64 s = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) s += sh.scratch[w];
-    return s;
-  };
-  // inclusive prefix sum over the block's threads
-  auto block_scan = [&](u64 v, u64* total) {
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += y;
-    }
-    __syncthreads();
-    if (lane == 31) sh.scratch[warp] = v;
-    __syncthreads();
-    u64 s = 0, before = 0;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      if (w == warp) before = s;
-      s += sh.scratch[w];
-    }
-    *total = s;
-    return v + before;
-  };
   auto drawn_mass = [&](u64 z) {  // the running mass that the drawn token is the first to exceed
     const double uz = u * (double)z;
     const u64 t = uz > 0.0 ? (uz < 9.2e18 ? (u64)uz : z - 1) : 0;
@@ -311,36 +372,56 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   };
 
   // -----------------------------------------------------------------------
-  // top-k by a list: a lower bound t of the k-th largest logit comes from the
-  // maxima of half chunks (k of those reach t, so k logits do), the logits from
-  // t up are gathered and sorted, and everything else happens on the list.
+  // top-k by a list: a lower bound t of the k-th largest logit is the k-th
+  // largest maximum over disjoint groups of the row (k groups reach it, so k
+  // logits do; with at least 2 k groups few more).  The logits from t up are
+  // gathered in one CTA, which ranks them and does everything else.
   // -----------------------------------------------------------------------
-  bool general = top_k < V;
-  if (top_k < V && top_k <= kListTopK) {
+  if (by_list && !general) {
     uint32_t t = 0;
     if (V > kList) {
-      uint32_t keys[2 * CS];
-#pragma unroll
-      for (int r = 0; r < CS; ++r) {
-        keys[2 * r] = peer(r)->k.maxima[tid];
-        keys[2 * r + 1] = peer(r)->k.maxima[NT + tid];
-      }
-      uint32_t lo = 0, hi = kmax;  // count(>= lo) >= k; wanted: not many more
-      const unsigned enough = (unsigned)top_k + max(16, top_k / 4);
-      while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo + 1) / 2;
-        unsigned n = 0;
-#pragma unroll
-        for (int i = 0; i < 2 * CS; ++i) n += keys[i] >= mid;
-        n = (unsigned)block_sum(n);
-        if (n >= (unsigned)top_k) {
-          lo = mid;
-          if (n <= enough) break;
-        } else {
-          hi = mid - 1;
+      const int groups = 2 * top_k <= NW * CS ? NW : 2 * top_k <= 4 * NW * CS ? 4 * NW : 0;  // of a CTA
+      if (groups) {
+        uint32_t* vals = reinterpret_cast<uint32_t*>(sh.k.list);
+        const int all = groups * CS;
+        if (tid < all) {
+          const SampleShared* q = peer(tid / groups);
+          vals[tid] = groups == NW ? q->k.warp_max[tid % NW] : q->k.oct_max[tid % (4 * NW)];
         }
+        __syncthreads();
+        const int gs = NT / all, i = tid / gs;  // threads per value (all divides NT)
+        const uint32_t mine = vals[i];
+        unsigned n = 0;  // values above, and at least, mine
+        for (int j = tid % gs; j < all; j += gs) n += (vals[j] > mine) + ((unsigned)(vals[j] >= mine) << 16);
+        for (int o = 1; o < min(gs, 32); o <<= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        if ((int)(n & 0xffffu) < top_k && top_k <= (int)(n >> 16)) sh.tie_index = (int)mine;
+        __syncthreads();
+        t = (uint32_t)sh.tie_index;
+      } else {
+        uint32_t keys[2 * CS];
+#pragma unroll
+        for (int r = 0; r < CS; ++r) {
+          keys[2 * r] = peer(r)->k.maxima[tid];
+          keys[2 * r + 1] = peer(r)->k.maxima[NT + tid];
+        }
+        uint32_t lo = 0, hi = kmax;  // count(>= lo) >= k; wanted: not many more
+        const unsigned enough = (unsigned)top_k + max(16, top_k / 4);
+        while (lo < hi) {
+          const uint32_t mid = lo + (hi - lo + 1) / 2;
+          unsigned n = 0;
+#pragma unroll
+          for (int i = 0; i < 2 * CS; ++i) n += keys[i] >= mid;
+          n = block_sum32(n);
+          if (n >= (unsigned)top_k) {
+            lo = mid;
+            if (n <= enough) break;
+          } else {
+            hi = mid - 1;
+          }
+        }
+        t = lo;
       }
-      t = lo;
+      __syncthreads();  // (the list takes the place of vals)
     }
     each([&](float v, int tok, bool in) {
       const bool take = in && float_key(v + 0.f) >= t;
@@ -358,9 +439,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     for (int r = 0; r < CS; ++r) n += peer(r)->n;
     if (n <= kList) {
       if (rank == 0) {
-        u64* s = reinterpret_cast<u64*>(dyn);  // the part itself is no longer needed
-        const unsigned size = n <= 64 ? 64 : 1u << (32 - __clz(n - 1));
-        __syncthreads();
+        u64* s = reinterpret_cast<u64*>(dyn);  // [kList]; the part itself is no longer needed
+        u64* ws = s + kList;                   // [kList]
         unsigned at = 0;
         for (int r = 0; r < CS; ++r) {
           const SampleShared* q = peer(r);
@@ -368,87 +448,93 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
           for (unsigned i = tid; i < k; i += NT) s[at + i] = q->k.list[i];
           at += k;
         }
-        for (unsigned i = n + tid; i < size; i += NT) s[i] = 0;
-        auto sort_down = [&](unsigned size) {  // bitonic, descending
-          for (unsigned k = 2; k <= size; k <<= 1)
-            for (unsigned j = k >> 1; j > 0; j >>= 1) {
-              __syncthreads();
-              for (unsigned i = tid; i < size / 2; i += NT) {
-                const unsigned x = 2 * i - (i & (j - 1)), y = x + j;
-                const u64 p = s[x], q = s[y];
-                if (((x & k) == 0) == (p < q)) s[x] = q, s[y] = p;
-              }
-            }
-          __syncthreads();
-        };
-        sort_down(size);
         const unsigned k = min(n, (unsigned)top_k);
-        constexpr int PER = kListTopK / NT;  // ranks per thread, consecutive
-        u64 w[PER], mine = 0, z;
-        double wd[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const unsigned r = tid * PER + i;
-          wd[i] = r < k ? weight(key_float((uint32_t)(s[r] >> 32)), m, c) : 0.0;
-          w[i] = fixed(wd[i]);
-          mine += w[i];
-        }
-        u64 before = block_scan(mine, &z) - mine;
-        const double reach = top_p < 1.0 ? top_p * (double)z : 2.0 * (double)z;
-        unsigned kept = 0;
-        u64 entry[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const unsigned r = tid * PER + i;
-          const bool keep = r < k && (r == 0 || ((double)before < reach && wd[i] >= min_p));
-          kept += keep;
-          // for the order by index: token in the upper half (its complement sorts it), rank below
-          entry[i] = keep ? (s[r] << 32) | r : 0;
-          before += w[i];
-        }
-        kept = (unsigned)block_sum(kept);
-        __syncthreads();
-        u64* wr = sh.k.list;  // weights by rank; every CTA's list has been read
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          s[tid * PER + i] = entry[i];
-          wr[tid * PER + i] = w[i];
-        }
-        // the kept are the leading ranks
-        const unsigned size2 = kept <= 64 ? 64 : 1u << (32 - __clz(kept - 1));
-        sort_down(size2);  // descending complement of the index: ascending index
-        mine = 0;
-        u64 wi[PER];
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const unsigned r = tid * PER + i;
-          wi[i] = r < kept ? wr[(uint32_t)s[r]] : 0;
-          mine += wi[i];
-        }
-        before = block_scan(mine, &z) - mine;
-        const u64 target = drawn_mass(z);
-#pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const unsigned r = tid * PER + i;
-          if (r < kept && target >= before && target < before + wi[i]) {
-            const int tok = (int)(0xffffffffu - (uint32_t)(s[r] >> 32));
-            finish(tok, (double)wi[i], (double)z);
+        if (n <= kPairs) {
+          __syncthreads();
+          for (unsigned i = tid; i < n; i += NT) ws[i] = fixed(weight(key_float((uint32_t)(s[i] >> 32)), m, c));
+          __syncthreads();
+          // gs threads per entry: its rank and the mass before it
+          unsigned gs = 32;
+          while (NT / gs < n) gs >>= 1;
+          const unsigned i = tid / gs, part = tid % gs;
+          const bool have = i < n;
+          const u64 mine = have ? s[i] : 0, w = have ? ws[i] : 0;
+          unsigned rk = 0;
+          u64 before = 0;
+          for (unsigned j = part; j < n; j += gs)
+            if (s[j] > mine) ++rk, before += ws[j];
+          for (unsigned o = 1; o < gs; o <<= 1) {
+            rk += __shfl_xor_sync(0xffffffffu, rk, o);
+            before += __shfl_xor_sync(0xffffffffu, before, o);
           }
-          before += wi[i];
+          bool keep = have && rk < k;
+          const u64 zk = block_sum(keep && part == 0 ? w : 0);
+          if (keep && rk > 0) {
+            if (top_p < 1.0) keep = (double)before < top_p * (double)zk;
+            if (min_p > 0.0) keep = keep && weight(key_float((uint32_t)(mine >> 32)), m, c) >= min_p;
+          }
+          __syncthreads();
+          if (part == 0 && have) ws[i] = keep ? w : 0;
+          const u64 z = block_sum(keep && part == 0 ? w : 0);  // (its barriers order ws)
+          // the mass before it by index: a smaller index has a larger complement
+          before = 0;
+          for (unsigned j = part; j < n; j += gs)
+            if ((uint32_t)s[j] > (uint32_t)mine) before += ws[j];
+          for (unsigned o = 1; o < gs; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+          const u64 target = drawn_mass(z);
+          if (keep && part == 0 && target >= before && target < before + w)
+            finish((int)(0xffffffffu - (uint32_t)mine), (double)w, (double)z);
+        } else {
+          const unsigned size = 1u << (32 - __clz(n - 1));
+          for (unsigned i = n + tid; i < size; i += NT) s[i] = 0;
+          auto sort_down = [&](unsigned size) {  // bitonic, descending
+            for (unsigned k = 2; k <= size; k <<= 1)
+              for (unsigned j = k >> 1; j > 0; j >>= 1) {
+                __syncthreads();
+                for (unsigned i = tid; i < size / 2; i += NT) {
+                  const unsigned x = 2 * i - (i & (j - 1)), y = x + j;
+                  const u64 p = s[x], q = s[y];
+                  if (((x & k) == 0) == (p < q)) s[x] = q, s[y] = p;
+                }
+              }
+            __syncthreads();
+          };
+          sort_down(size);
+          static_assert(kListTopK == NT, "one rank per thread");
+          const unsigned r = tid;
+          u64 z;
+          const double wd = r < k ? weight(key_float((uint32_t)(s[r] >> 32)), m, c) : 0.0;
+          const u64 w = fixed(wd);
+          u64 before = block_scan(w, &z) - w;
+          const double reach = top_p < 1.0 ? top_p * (double)z : 2.0 * (double)z;
+          const bool keep = r < k && (r == 0 || ((double)before < reach && wd >= min_p));
+          // for the order by index: the complement of the token in the upper half, the rank below
+          const u64 entry = keep ? (s[r] << 32) | r : 0;
+          const unsigned kept = block_sum32(keep);  // the kept are the leading ranks
+          __syncthreads();
+          s[r] = entry;
+          ws[r] = w;
+          sort_down(max(64u, 1u << (32 - __clz(max(kept, 2u) - 1))));
+          const u64 wi = r < kept ? ws[(uint32_t)s[r]] : 0;
+          before = block_scan(wi, &z) - wi;
+          const u64 target = drawn_mass(z);
+          if (r < kept && target >= before && target < before + wi)
+            finish((int)(0xffffffffu - (uint32_t)(s[r] >> 32)), (double)wi, (double)z);
         }
       }
       all_sync();
       return;
     }
+    general = true;  // too many equal logits
   }
 
   // f(value) for the values for which want(value, token) holds, 32 at a time: they are
   // packed in the warp's queue, since the exact weights cost about 60 instructions each
   auto packed = [&](auto want, auto f) {
     int fill = 0;
-    float* q = sh.queue[warp];
+    float* q = sh.p.queue[warp];
     each([&](float v, int t, bool in) {
-      const bool take = in && want(v, t);
+      const bool take = want(v, t) && in;
       const unsigned bal = __ballot_sync(0xffffffffu, take);
       if (take) q[fill + __popc(bal & ((1u << lane) - 1))] = v;
       fill += __popc(bal);
@@ -465,83 +551,94 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     if (lane < fill) f(q[lane]);
     __syncwarp();
   };
-  auto warp_sum64 = [&](u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  };
 
   // The last step of every path below: sh.w_keep holds each warp's kept mass and
-  // keep_of[r] each CTA's; the warp that holds the drawn mass walks its part.
-  // w_of(value, token) is a token's kept mass; slack the uncertainty of the sums
-  // (0: exact).  Returns true when the draw is certain (the same in every CTA).
-  auto draw = [&](const u64* keep_of, auto w_of, u64 slack) -> bool {
-    u64 z = 0, mine0 = 0;
+  // keep_of[r] each CTA's.  In the CTA that holds the drawn mass all warps share
+  // the steps of the part that holds it.  sel(value, token): kept; w_of(value):
+  // its mass; slack: the uncertainty of the sums (0: exact).  Returns true when
+  // the draw is certain (the same in every CTA).
+  auto draw = [&](const u64* keep_of, auto sel, auto w_of, u64 slack) -> bool {
+    u64 z = 0, mine0 = 0, mine = 0;
 #pragma unroll
     for (int r = 0; r < CS; ++r) {
-      if (r == rank) mine0 = z;
+      if (r == rank) mine0 = z, mine = keep_of[r];
       z += keep_of[r];
     }
     const u64 target = drawn_mass(z);
-    if (target >= mine0 && target < mine0 + keep_of[rank]) {
-      u64 acc = mine0;
-      for (int w = 0; w < warp; ++w) acc += sh.w_keep[w];
-      if (target >= acc && target < acc + sh.w_keep[warp]) {
-        bool done = false;
-        for (int ch0 = wbeg; ch0 < wend && !done; ch0 += 32) {
-          const int ch = ch0 + lane;
-          uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-          if (ch < wend) raw = *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
-          const T* e = reinterpret_cast<const T*>(&raw);
-          u64 w[VEC], s = 0;
+    if (target >= mine0 && target < mine0 + mine) {
+      auto find = [&](u64 v, u64* at) {  // first lane whose running sum from *at exceeds the target (32: none)
+        u64 incl = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, *at + incl > target);
+        if (!hit) return 32;
+        const int l = __ffs(hit) - 1;
+        *at += __shfl_sync(0xffffffffu, incl - v, l);
+        return l;
+      };
+      u64 at = mine0;
+      const int hw = find(lane < NW ? sh.w_keep[lane] : 0, &at);
+      const int hb = min(nch, hw * per_warp), he = min(nch, hb + per_warp);
+      const int steps = (he - hb + 31) / 32;
+      u64 w[VEC], sum = 0;
+      auto weigh = [&](int s) {
+        const int ch = hb + 32 * s + lane;
+        const uint4 raw = chunk(ch, he);
+        const T* e = reinterpret_cast<const T*>(&raw);
+        sum = 0;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const int t = base + ch * VEC + j;
+          const bool is = ch < he && (unsigned)t < (unsigned)V && sel(to_f(e[j]), t);
+          w[j] = 0;
+          if (__any_sync(0xffffffffu, is)) w[j] = is ? w_of(to_f(e[j])) : 0;
+          sum += w[j];
+        }
+      };
+      int last = -1;
+      for (int s = warp; s < steps; s += NW) {
+        weigh(s);
+        last = s;
+        const u64 t = warp_sum64(sum);
+        if (lane == 0) sh.step[s] = t;
+      }
+      __syncthreads();
+      const int hs = find(lane < steps ? sh.step[lane] : 0, &at);
+      if (hs == 32 || hw == 32) {  // the approximate sums of the two walks differ by their rounding
+        if (tid == 0)
+          for (int r = 0; r < CS; ++r) peer(r)->uncertain = 1;
+      } else if (hs % NW == warp) {
+        if (last != hs) weigh(hs);
+        const int l = find(sum, &at);
+        if (lane == l) {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const int t = base + ch * VEC + j;
-            w[j] = ch < wend && (unsigned)t < (unsigned)V ? w_of(to_f(e[j]), t) : 0;
-            s += w[j];
-          }
-          u64 incl = s;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const u64 y = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += y;
-          }
-          const unsigned hit = __ballot_sync(0xffffffffu, acc + incl > target);
-          if (hit) {
-            done = true;
-            if (lane == __ffs(hit) - 1) {
-              u64 b = acc + incl - s;
-#pragma unroll
-              for (int j = 0; j < VEC; ++j) {
-                if (target >= b && target < b + w[j]) {
-                  const bool sure = slack == 0 || (target >= b + slack && target + slack < b + w[j]);
-                  if (sure) {
-                    finish(base + ch * VEC + j, (double)w[j], (double)z);
-                  } else {
-                    for (int r = 0; r < CS; ++r) peer(r)->uncertain = 1;
-                  }
-                }
-                b += w[j];
+            if (target >= at && target < at + w[j]) {
+              if (slack == 0 || (target >= at + slack && target + slack < at + w[j])) {
+                finish(base + (hb + 32 * hs + lane) * VEC + j, (double)w[j], (double)z);
+              } else {
+                for (int r = 0; r < CS; ++r) peer(r)->uncertain = 1;
               }
             }
+            at += w[j];
           }
-          acc += __shfl_sync(0xffffffffu, incl, 31);
         }
-        if (!done && lane == 0)  // the approximate sums of the two walks may differ by their rounding
-          for (int r = 0; r < CS; ++r) peer(r)->uncertain = 1;
       }
     }
     all_sync();
     return sh.uncertain == 0;
   };
   // exact draw among the tokens with composite >= thr and weight >= min_p
+  auto exact_of = [&](float v) -> u64 {
+    const double w = weight(v, m, c);
+    return w >= min_p ? fixed(w) : 0;
+  };
   auto draw_exact = [&](u64 thr) {
     u64 acc = 0;
-    packed([&](float v, int t) { return composite(v, t) >= thr; },
-           [&](float v) {
-             const double w = weight(v, m, c);
-             if (w >= min_p) acc += fixed(w);
-           });
+    packed([&](float v, int t) { return composite(v, t) >= thr; }, [&](float v) { acc += exact_of(v); });
     acc = warp_sum64(acc);
     if (lane == 0) sh.w_keep[warp] = acc;
     __syncthreads();
@@ -554,20 +651,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     u64 keep_of[CS];
 #pragma unroll
     for (int r = 0; r < CS; ++r) keep_of[r] = peer(r)->cta_keep;
-    draw(keep_of,
-         [&](float v, int t) -> u64 {
-           if (composite(v, t) < thr) return 0;
-           const double w = weight(v, m, c);
-           return w >= min_p ? fixed(w) : 0;
-         },
-         0);
+    draw(keep_of, [&](float v, int t) { return composite(v, t) >= thr; }, exact_of, 0);
   };
 
-  // Sum of the weights in float32 (ex2.approx, at most 2 ulp): Z~, and a bound of
-  // its error: x = (m - l) c carries 3 roundings, each moving the weight by
-  // x 2^-24 ln 2; the exponential 2^-22; sums of VEC weights VEC roundings.
+  // A weight in float32 (ex2.approx, at most 2 ulp) errs relatively by at most
+  // err_1 + x err_x: x = (m - l) c carries 3 roundings, each moving the weight by
+  // x 2^-24 ln 2, the exponential 2^-22, and sums of VEC weights VEC roundings.
   const float err_x = 3.f * 0.7f * 5.9604645e-8f, err_1 = (4.f + VEC) * 5.9604645e-8f;
-  if (!general && !(top_p < 1.0)) {
+  if (!general && !by_mass) {
     // ---------------------------------------------------------------------
     // no top-k, no top-p: draw from the float32 masses when the drawn mass is
     // farther from the token's borders than their error, else from exact ones;
@@ -581,7 +672,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     double sum = 0.0, err = 0.0;
     bool border = false;
     for (int ch = wbeg + lane; ch < wend; ch += 32) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
+      const uint4 raw = chunk(ch, wend);
       const T* e = reinterpret_cast<const T*>(&raw);
       float s = 0.f, se = 0.f;
 #pragma unroll
@@ -590,17 +681,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const float w = x <= x_min ? ex2_f32(-x) : 0.f;
         border |= x_min < CUDART_INF_F && fabsf(x - x_min) <= 1e-6f * (x_min + 1.f);
         s += w;
-        if (w > 0.f) se = fmaf(w, fmaf(x, err_x, err_1), se);
+        se = fmaf(w, fmaf(fminf(x, 200.f), err_x, err_1), se);
       }
       sum += (double)s;
       err += (double)se;
     }
     if (border) atomicOr(&sh.uncertain, 1);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      err += __shfl_xor_sync(0xffffffffu, err, o);
-    }
+    sum = warp_sumd(sum);
+    err = warp_sumd(err);
     if (lane == 0) {
       sh.w_keep[warp] = fixed(sum);
       sh.w_err[warp] = err;
@@ -628,12 +716,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     // warp's mass is rounded to the fixed point
     const u64 slack = (u64)(2.0 * e * kWeightOne) + (u64)V + 64;
     if (sure)
-      sure = draw(keep_of,
-                  [&](float v, int) -> u64 {
-                    const float x = (m - v) * cf;
-                    return x <= x_min ? fixed((double)ex2_f32(-x)) : 0;
-                  },
-                  slack);
+      sure = draw(keep_of, [&](float v, int) { return (m - v) * cf <= x_min; },
+                  [&](float v) { return fixed((double)ex2_f32((v - m) * cf)); }, slack);
     else
       all_sync();  // every CTA has read the sums before they are written again
     if (!sure) draw_exact(0);
@@ -643,28 +727,36 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   u64 thr = 0;  // kept: composite >= thr
   if (!general) {
     // ---------------------------------------------------------------------
-    // top-p.  Z~ bounds the weights that can stay (a token below (1 - p) Z / V
-    // cannot: all tokens from it down would have less than (1 - p) Z); a
-    // histogram of their float32 masses over x gives a few bins that hold the
-    // border; the masses above those bins are summed exactly, the tail in
+    // top-p.  With z_low <= Z a token below (1 - p) z_low / V cannot stay (all
+    // tokens from it down have less than (1 - p) Z).  One pass sums the float32
+    // weights to Z~ and makes a histogram over x of the masses that can; the
+    // border lies in the one or few bins where the running mass passes p Z~.
+    // The next pass sums the masses above those bins exactly and the tail in
     // float32 with its error bound, and the tokens of the bins are taken one
     // by one.  Where the error could move the border, the tail is summed
     // exactly as well.
     // ---------------------------------------------------------------------
+    const float rest = fmaxf((float)(1.0 - top_p), 1e-17f);
+    const float x_end = fmaxf(log2f((float)V / z_low) - log2f(rest), 0.f) + 0.02f;
+    const float bin_scale = (float)kBins / x_end, unit = 2147483648.0f / z_high * (1.f - 1e-3f);
+    auto bin_at = [&](float v) { return (m - v) * cf * bin_scale; };  // falls with v; its floor is the bin
+    for (int i = tid; i < kBins; i += NT) sh.p.hist[i] = 0;
+    __syncthreads();
     double sum = 0.0;
     for (int ch = wbeg + lane; ch < wend; ch += 32) {
-      const uint4 raw = *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
+      const uint4 raw = chunk(ch, wend);
       const T* e = reinterpret_cast<const T*>(&raw);
       float s = 0.f;
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) s += ex2_f32((to_f(e[j]) - m) * cf);
+      for (int j = 0; j < VEC; ++j) {
+        const float x = (m - to_f(e[j])) * cf, w = ex2_f32(-x), b = x * bin_scale;
+        s += w;
+        if (b < (float)kBins) atomicAdd(&sh.p.hist[(int)b], __float2uint_rn(w * unit));
+      }
       sum += (double)s;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    sum = warp_sumd(sum);
     if (lane == 0) sh.w_sum[warp] = sum;
-    // (the maxima of the union are not read any more: no list was made)
-    for (int i = tid; i < kBins; i += NT) sh.p.hist[i] = 0;
     __syncthreads();
     if (tid == 0) {
       double s = 0.0;
@@ -672,92 +764,113 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       sh.cta_sum = s;
     }
     all_sync();
-    double z = 0.0;
-#pragma unroll
-    for (int r = 0; r < CS; ++r) z += peer(r)->cta_sum;
-    const double rest = fmax(1.0 - top_p, 1e-17);
-    const float x_end = (float)fmax(log2((double)V / (rest * z)), 0.0) + 0.01f;
-    const float bin_scale = (float)kBins / x_end, unit = (float)(2147483648.0 / z * (1.0 - 1e-4));
-    auto bin_of = [&](float v) { return min((m - v) * cf * bin_scale, (float)kBins + 1.f); };  // monotone in v
-    each([&](float v, int, bool in) {
-      const float b = bin_of(v);
-      if (in && b < (float)kBins) atomicAdd(&sh.p.hist[(int)b], __float2uint_rn(ex2_f32((v - m) * cf) * unit));
-    });
-    all_sync();
     int blo, bhi;
     {
       static_assert(kBins == 2 * NT, "two bins per thread");
-      u64 h0 = 0, h1 = 0, total;
+      double z = 0.0;
+      uint32_t h0 = 0, h1 = 0;
 #pragma unroll
       for (int r = 0; r < CS; ++r) {
-        h0 += peer(r)->p.hist[2 * tid];
-        h1 += peer(r)->p.hist[2 * tid + 1];
+        z += peer(r)->cta_sum;
+        const uint2 h = *reinterpret_cast<const uint2*>(&peer(r)->p.hist[2 * tid]);
+        h0 += h.x;
+        h1 += h.y;
       }
-      const u64 incl = block_scan(h0 + h1, &total);
-      const double reach = top_p * z * unit, margin = 0.5 * V + 3e-5 * z * unit;
-      // number of bins whose running mass stays at or below either bound
-      const unsigned n_lo = ((double)(incl - h1) <= reach - margin) + ((double)incl <= reach - margin);
-      const unsigned n_hi = ((double)(incl - h1) < reach + margin) + ((double)incl < reach + margin);
-      const u64 both = block_sum(((u64)n_hi << 32) | n_lo);
-      blo = min((int)(both & 0xffffffffu), kBins - 1);
-      bhi = min((int)(both >> 32), kBins - 1);
-    }
-    all_sync();  // every CTA has read the histograms: the union is free
-    const float edge_lo = (float)blo, edge_hi = (float)(bhi + 1);
-    bool exact_tail = false, resolved = false;
-    u64 keep_of[CS];
-    for (;;) {
-      if (tid == 0) sh.n = 0;
-      __syncthreads();
-      u64 acc_keep = 0, acc_all = 0, acc_tail = 0;
-      double tail = 0.0, tail_err = 0.0;
-      packed(
-          [&](float v, int t) {
-            const float b = bin_of(v);
-            if (b >= edge_lo && b < edge_hi) {
-              const unsigned at = atomicAdd(&sh.n, 1u);
-              if (at < kCands) sh.p.cand[at] = composite(v, t);
-            }
-            return b < edge_lo || (exact_tail && b >= edge_hi);
-          },
-          [&](float v) {
-            const double w = weight(v, m, c);
-            const u64 f = fixed(w);
-            if (bin_of(v) < edge_lo) {
-              acc_all += f;
-              if (w >= min_p) acc_keep += f;
-            } else {
-              acc_tail += f;
-            }
-          });
-      if (!exact_tail) {
-        for (int ch = wbeg + lane; ch < wend; ch += 32) {
-          const uint4 raw = *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
-          const T* e = reinterpret_cast<const T*>(&raw);
-          float s = 0.f, se = 0.f;
+      // inclusive prefix sums of 32 bits: the masses are below 2^31 in all
+      uint32_t incl = h0 + h1;
 #pragma unroll
-          for (int j = 0; j < VEC; ++j) {
-            const float v = to_f(e[j]), x = (m - v) * cf;
-            const float w = bin_of(v) >= edge_hi ? ex2_f32(-x) : 0.f;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      if (lane == 31) sh.step[warp] = incl;
+      __syncthreads();
+      incl += __reduce_add_sync(0xffffffffu, lane < warp ? (uint32_t)sh.step[lane] : 0u);
+      const double reach = top_p * z * unit, margin = 0.5 * V + 3e-5 * z * unit;
+      const long long below = (long long)floor(reach - margin), past = (long long)ceil(reach + margin);
+      // number of bins whose running mass stays at or below either bound
+      const unsigned n_lo = ((long long)(incl - h1) <= below) + ((long long)incl <= below);
+      const unsigned n_hi = ((long long)(incl - h1) < past) + ((long long)incl < past);
+      const unsigned both = block_sum32((n_hi << 16) | n_lo);
+      blo = min((int)(both & 0xffffu), kBins - 1);
+      bhi = min((int)(both >> 16), kBins - 1);
+    }
+    const float edge_lo = (float)blo, edge_hi = (float)(bhi + 1);
+    u64 keep_of[CS];
+    u64 acc_keep, acc_all, acc_tail;
+    double tail, tail_err;
+    // the pass over the part: masses above the bins (exact), the bins' tokens, the tail
+    auto tally = [&](auto exact_tag) {
+      constexpr bool EXACT = decltype(exact_tag)::value;
+      acc_keep = acc_all = acc_tail = 0;
+      tail = tail_err = 0.0;
+      int fill = 0;
+      float* q = sh.p.queue[warp];
+      auto take_one = [&](float v) {
+        const double w = weight(v, m, c);
+        const u64 f = fixed(w);
+        if (!EXACT || bin_at(v) < edge_lo) {
+          acc_all += f;
+          if (w >= min_p) acc_keep += f;
+        } else {
+          acc_tail += f;
+        }
+      };
+      for (int ch0 = wbeg; ch0 < wend; ch0 += 32) {
+        const int ch = ch0 + lane;
+        const uint4 raw = chunk(ch, wend);
+        const T* e = reinterpret_cast<const T*>(&raw);
+        float s = 0.f, se = 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+          const float v = to_f(e[j]), x = (m - v) * cf, b = x * bin_scale;
+          const bool in_tail = !(b < edge_hi);
+          if (!EXACT) {
+            const float w = in_tail ? ex2_f32(-x) : 0.f;
             s += w;
-            if (w > 0.f) se = fmaf(w, fmaf(x, err_x, err_1), se);
+            se = fmaf(w, fmaf(fminf(x, 200.f), err_x, err_1), se);
           }
+          const bool take = b < edge_lo || (EXACT && in_tail);
+          if (b >= edge_lo && !in_tail) {
+            const unsigned at = atomicAdd(&sh.n, 1u);
+            if (at < kCands) sh.p.cand[at] = composite(v, base + ch * VEC + j);
+          }
+          const unsigned bal = __ballot_sync(0xffffffffu, take);
+          if (bal) {
+            if (take) q[fill + __popc(bal & ((1u << lane) - 1))] = v;
+            fill += __popc(bal);
+            if (fill >= 32) {
+              __syncwarp();
+              const float y0 = q[lane], y1 = q[32 + lane];
+              __syncwarp();
+              q[lane] = y1;
+              fill -= 32;
+              take_one(y0);
+            }
+          }
+        }
+        if (!EXACT) {
           tail += (double)s;
           tail_err += (double)se;
         }
       }
+      __syncwarp();
+      if (lane < fill) take_one(q[lane]);
+      __syncwarp();
+    };
+    bool resolved = false;
+    for (int pass = 0; pass < 2; ++pass) {
+      const bool exact_tail = pass == 1;
+      if (exact_tail) tally(std::true_type{});
+      else tally(std::false_type{});
       acc_keep = warp_sum64(acc_keep);
       acc_all = warp_sum64(acc_all);
-      acc_tail = warp_sum64(acc_tail);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        tail += __shfl_xor_sync(0xffffffffu, tail, o);
-        tail_err += __shfl_xor_sync(0xffffffffu, tail_err, o);
-      }
+      tail = exact_tail ? (double)warp_sum64(acc_tail) / kWeightOne : warp_sumd(tail);
+      tail_err = warp_sumd(tail_err);
       if (lane == 0) {
         sh.w_keep[warp] = acc_keep;
         sh.w_all[warp] = acc_all;
-        sh.w_sum[warp] = exact_tail ? (double)acc_tail / kWeightOne : tail;
+        sh.w_sum[warp] = tail;
         sh.w_err[warp] = tail_err;
       }
       __syncthreads();
@@ -771,6 +884,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       u64 above = 0;
       double tl = 0.0, te = 0.0;
       unsigned n = 0;
+      int src = -1;
+      u64 own = 0;
 #pragma unroll
       for (int r = 0; r < CS; ++r) {
         const SampleShared* q = peer(r);
@@ -778,89 +893,73 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         above += q->cta_all;
         tl += q->cta_sum;
         te += q->cta_err;
-        n += q->n;
+        const unsigned k = q->n;
+        if (tid >= n && tid < n + k && k <= kCands) own = q->p.cand[tid - n], src = r;
+        n += k;
       }
       if (n == 0 || n > kCands) break;  // too many tokens at the border: the general way
-      unsigned at = 0;
-      for (int r = 0; r < CS; ++r) {
-        const SampleShared* q = peer(r);
-        const unsigned k = q->n;
-        for (unsigned i = tid; i < k; i += NT) {
-          sh.p.all[at + i] = q->p.cand[i];
-          sh.p.from[at + i] = (uint8_t)r;
-        }
-        at += k;
+      // thread i < n holds token i of the border: its weight for the others
+      const double own_w = src >= 0 ? weight(key_float((uint32_t)(own >> 32)), m, c) : 0.0;
+      if (src >= 0) {
+        sh.p.all[tid] = own;
+        sh.p.wt[tid] = fixed(own_w);
       }
       __syncthreads();
-      // this thread's candidate: the mass before it
-      static_assert(kCands == NT, "one candidate per thread");
-      const bool have = tid < n;
-      const u64 mine = have ? sh.p.all[tid] : 0;
-      const double wd = have ? weight(key_float((uint32_t)(mine >> 32)), m, c) : 0.0;
-      const u64 wf = fixed(wd);
-      u64 before = above;
-      const u64 cands = block_sum(wf);
-      for (unsigned i0 = 0; i0 < n; i0 += 32) {
-        // 32 candidates at a time, their weights computed by this warp's lanes
-        const u64 other = i0 + lane < n ? sh.p.all[i0 + lane] : 0;
-        const u64 ow = other ? fixed(weight(key_float((uint32_t)(other >> 32)), m, c)) : 0;
-#pragma unroll 4
-        for (int i = 0; i < 32; ++i) {
-          const u64 oc = __shfl_sync(0xffffffffu, other, i), w = __shfl_sync(0xffffffffu, ow, i);
-          if (oc > mine) before += w;
-        }
+      // gs threads per token: its rank in the bins and the mass before it
+      unsigned gs = 16;
+      while (NT / gs < n) gs >>= 1;
+      const unsigned i = tid / gs, part = tid % gs;
+      const bool have = i < n;
+      const u64 mine = have ? sh.p.all[i] : 0;
+      unsigned rk = 0;
+      u64 before = 0, cands = 0;
+      for (unsigned j = part; j < n; j += gs) {
+        const u64 w = sh.p.wt[j];
+        cands += w;
+        if (sh.p.all[j] > mine) ++rk, before += w;
       }
+      for (unsigned o = 1; o < gs; o <<= 1) {
+        rk += __shfl_xor_sync(0xffffffffu, rk, o);
+        before += __shfl_xor_sync(0xffffffffu, before, o);
+        cands += __shfl_xor_sync(0xffffffffu, cands, o);
+      }
+      const bool first = above == 0 && rk == 0;  // the most likely token stays
+      before += above;
       const double zx = (double)(above + cands);
-      const double reach_lo = top_p * (zx + (tl - te) * kWeightOne * (1.0 - 1e-9) - V);
-      const double reach_hi = top_p * (zx + (tl + te) * kWeightOne * (1.0 + 1e-9) + V);
       const double reach = top_p * (zx + tl * kWeightOne);
-      const bool first = before == 0 && mine >> 32 == kmax;  // the most likely token stays
-      bool keep = have && (first || (double)before < reach);
+      const bool keep = have && (first || (double)before < reach);
       if (!exact_tail) {
+        const double reach_lo = top_p * (zx + (tl - te) * kWeightOne * (1.0 - 1e-9) - V);
+        const double reach_hi = top_p * (zx + (tl + te) * kWeightOne * (1.0 + 1e-9) + V);
         const bool unsure = have && ((double)before < reach_lo) != ((double)before < reach_hi);
         if (__syncthreads_or(unsure)) {
-          exact_tail = true;
           all_sync();  // the lists and sums have been read by every CTA
+          if (tid == 0) sh.n = 0;
+          __syncthreads();
           continue;
         }
       }
-      // threshold: the last kept candidate, or just above the first of them
-      u64 lowest = keep ? mine : ~0ull, highest = mine;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        lowest = min(lowest, __shfl_xor_sync(0xffffffffu, lowest, o));
-        highest = max(highest, __shfl_xor_sync(0xffffffffu, highest, o));
+      // the border does lie in these bins (their histogram is approximate)
+      if (!((above == 0 || (double)above < reach) && zx >= reach)) break;
+      // threshold: the last kept token, or just above the first of them
+      const unsigned kept = block_sum32(keep && part == 0);
+      if (part == 0 && have && (kept ? rk == kept - 1 : rk == 0)) sh.thr = kept ? mine : mine + 1;
+      // the kept join the masses of their CTAs and of this CTA's warps
+      __syncthreads();
+      thr = sh.thr;
+      if (src >= 0 && own >= thr && own_w >= min_p) {
+        const u64 f = fixed(own_w);
+        atomicAdd(&sh.add[src], f);
+        if (src == rank) atomicAdd(&sh.w_keep[(((int)(0xffffffffu - (uint32_t)own) - base) / VEC) / per_warp], f);
       }
       __syncthreads();
-      if (lane == 0) sh.scratch[warp] = lowest;
-      __syncthreads();
-      for (int w = 0; w < NW; ++w) lowest = min(lowest, sh.scratch[w]);
-      __syncthreads();
-      if (lane == 0) sh.scratch[warp] = highest;
-      __syncthreads();
-      for (int w = 0; w < NW; ++w) highest = max(highest, sh.scratch[w]);
-      thr = lowest != ~0ull ? lowest : highest + 1;
-      // the kept candidates join the masses of their CTAs and of this CTA's warps
-      const bool counts = keep && wd >= min_p;
-      const int src = have ? sh.p.from[tid] : -1;
 #pragma unroll
-      for (int r = 0; r < CS; ++r) keep_of[r] += block_sum(counts && src == r ? wf : 0);
-      if (counts && src == rank) {
-        const int t = (int)(0xffffffffu - (uint32_t)mine);
-        atomicAdd(&sh.w_keep[((t - base) / VEC) / per_warp], wf);
-      }
-      __syncthreads();
+      for (int r = 0; r < CS; ++r) keep_of[r] += sh.add[r];
       resolved = true;
       break;
     }
     if (resolved) {
-      draw(keep_of,
-           [&](float v, int t) -> u64 {
-             if (composite(v, t) < thr) return 0;
-             const double w = weight(v, m, c);
-             return w >= min_p ? fixed(w) : 0;
-           },
-           0);
+      draw(keep_of, [&](float v, int t) { return composite(v, t) >= thr; }, exact_of, 0);
       return;
     }
     all_sync();
@@ -871,13 +970,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   // (top-k) and masses (top-p); then the place of the last kept token among
   // those of the border key
   // -----------------------------------------------------------------------
-  // largest K with sum over keys >= K reaching `target` (of counts, or of masses
-  // while the running value is below it); *above = the sum over keys > K
-  auto select = [&](bool by_mass, double target, u64* above) -> uint32_t {
+  // largest K with the sum over keys >= K reaching `target`; *above = the sum over keys > K
+  auto select = [&](bool by_weight, double target, u64* above) -> uint32_t {
     uint32_t prefix = 0;
     u64 run = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
-      for (int i = tid; i < 256; i += NT) sh.r.mass[i] = 0;
+      for (int i = tid; i < 256; i += NT) sh.p.mass[i] = 0;
       __syncthreads();
       each([&](float v, int, bool in) {
         const uint32_t k = float_key(v + 0.f);
@@ -885,34 +983,35 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const unsigned act = __ballot_sync(0xffffffffu, take);
         if (!act) return;
         u64 w = 0;
-        if (take) w = by_mass ? fixed(weight(v, m, c)) : 1;
+        if (take) w = by_weight ? fixed(weight(v, m, c)) : 1;
         const int b = (k >> shift) & 255, lead = __shfl_sync(0xffffffffu, b, __ffs(act) - 1);
         if (__all_sync(0xffffffffu, !take || b == lead)) {  // one bin: one addition
           w = warp_sum64(w);
-          if (lane == 0) atomicAdd(&sh.r.mass[lead], w);
+          if (lane == 0) atomicAdd(&sh.p.mass[lead], w);
         } else if (take) {
-          atomicAdd(&sh.r.mass[b], w);
+          atomicAdd(&sh.p.mass[b], w);
         }
       });
       all_sync();
       // bins from the top: thread t holds bin 255 - t
       u64 h = 0, total;
       if (tid < 256)
-        for (int r = 0; r < CS; ++r) h += peer(r)->r.mass[255 - tid];
+        for (int r = 0; r < CS; ++r) h += peer(r)->p.mass[255 - tid];
       const u64 incl = block_scan(h, &total);
       // bins passed before the target is reached
       const bool passed = tid < 256 && (double)(run + incl) < target;
-      const unsigned np = min((unsigned)block_sum(passed), 255u);
+      const unsigned np = min(block_sum32(passed), 255u);
       __syncthreads();
-      if (tid == np) sh.scratch[0] = run + incl - h;
+      if (tid == np) sh.thr = run + incl - h;
       __syncthreads();
-      run = sh.scratch[0];
+      run = sh.thr;
       prefix |= (255u - np) << shift;
       all_sync();  // the histograms have been read
     }
     *above = run;
     return prefix;
   };
+  all_sync();  // (a list that was too long has been counted by every CTA)
   uint32_t K = 0;
   u64 ties = ~0ull, above = 0, zk;
   if (top_k < V) {
@@ -973,11 +1072,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       u64 run = total;
       for (int ch0 = wbeg; ch0 < wend; ch0 += 32) {
         const int ch = ch0 + lane;
+        const uint4 raw = chunk(ch, wend);
+        const T* e = reinterpret_cast<const T*>(&raw);
         unsigned n = 0, eq = 0;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const int t = base + ch * VEC + j;
-          const bool is = ch < wend && (unsigned)t < (unsigned)V && float_key(to_f(seg[(int64_t)ch * VEC + j]) + 0.f) == K;
+          const bool is = ch < wend && (unsigned)t < (unsigned)V && float_key(to_f(e[j]) + 0.f) == K;
           eq |= (unsigned)is << j;
           n += is;
         }
@@ -1007,7 +1108,7 @@ template <typename T, int CS>
 static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int per_cta = ((VEC - 1 + a.vocab + VEC - 1) / VEC + CS - 1) / CS;
-  const int smem = max(per_cta * 16, kList * 8);
+  const int smem = max(per_cta * 16, kList * 16);  // a list takes the part's place, with its weights
   auto* kern = sample_kernel<T, CS>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
@@ -1026,13 +1127,14 @@ static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
   return launch_status();
 }
 
-// CTAs per row: as many as keep a part at 56 KB (three CTAs per SM), then more
-// while the rows alone do not fill the GPU and a thread still has eight tokens.
+// CTAs per row: as few as keep a part within 100 KB (two CTAs per SM: the
+// barriers and scalar steps of a row are paid per CTA), then more while the
+// rows alone do not fill the GPU and a thread still has four tokens.
 template <typename T>
 static int sample_cluster(int64_t rows, int vocab) {
   int cs = 1;
-  while (cs < 8 && (int64_t)vocab * (int)sizeof(T) > cs * 57344ll) cs *= 2;
-  while (cs < 8 && rows * cs < 148 * 2 && vocab / cs > kSampleThreads * 8) cs *= 2;
+  while (cs < 8 && (int64_t)vocab * (int)sizeof(T) > cs * 101000ll) cs *= 2;
+  while (cs < 8 && rows * cs < 148 && vocab / cs > kSampleThreads * 8) cs *= 2;
   return cs;
 }
 
