@@ -111,11 +111,11 @@ struct SampleShared {
     } p;
   };
   u64 w_keep[kSampleWarps], w_all[kSampleWarps], scratch[kSampleWarps], step[32], add[8];
-  double w_sum[kSampleWarps], w_err[kSampleWarps];
+  double w_sum[kSampleWarps];
   // what other CTAs of the cluster read
   u64 cta_keep, cta_all, cta_ties;
-  double cta_sum, cta_err;
-  uint32_t cta_max, n;
+  double cta_sum;
+  uint32_t cta_max, n, key_lo, key_hi;  // key_lo, key_hi: of the tokens at the border
   // what the CTA that finds it writes into every CTA
   int tie_index, uncertain;
   u64 thr;
@@ -127,15 +127,16 @@ template <> __device__ __forceinline__ uint32_t neg_inf_word<float>() { return 0
 template <> __device__ __forceinline__ uint32_t neg_inf_word<__half>() { return 0xfc00fc00u; }
 template <> __device__ __forceinline__ uint32_t neg_inf_word<__nv_bfloat16>() { return 0xff80ff80u; }
 
-// One cluster of CS CTAs per row, each holding a contiguous part of the row in
-// shared memory; each warp owns a contiguous part of that, so index order is
-// (CTA, warp, position).
-template <typename T, int CS>
+// One cluster of CS CTAs per row, each with a contiguous part of the row, held in
+// shared memory (STAGE) or read again from L2 by each pass; each warp owns a
+// contiguous part of that, so index order is (CTA, warp, position).
+template <typename T, int CS, bool STAGE>
 __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleArgs<T> a) {
   constexpr int NT = kSampleThreads, NW = kSampleWarps, VEC = 16 / (int)sizeof(T);
   extern __shared__ __align__(16) unsigned char dyn[];
   __shared__ SampleShared sh;
   T* seg = reinterpret_cast<T*>(dyn);
+  bool inf_row = false;  // the largest logit is +inf
   const cg::cluster_group cl = cg::this_cluster();
   const int rank = CS == 1 ? 0 : (int)cl.block_rank();
   const int row = blockIdx.x / CS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
@@ -166,55 +167,80 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   const int wbeg = min(nch, warp * per_warp), wend = min(nch, wbeg + per_warp);
   const int base = c0 * VEC - mis;  // token of the part's first element (negative: before the row)
   float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
+  // 16 bytes of the row from its memory: outside the row and for NaN -inf
+  auto fetch = [&](int ch) -> uint4 {
+    const int t0 = base + ch * VEC;
+    uint4 raw;
+    if (t0 >= 0 && t0 + VEC <= V) {
+      raw = STAGE ? __ldcs(reinterpret_cast<const uint4*>(lg + t0)) : __ldg(reinterpret_cast<const uint4*>(lg + t0));
+    } else {
+      T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) e[j] = t0 + j >= 0 && t0 + j < V ? lg[t0 + j] : round_f<T>(-CUDART_INF_F);
+    }
+    return raw;
+  };
+  auto clean = [&](uint4 raw) -> uint4 {
+    T* e = reinterpret_cast<T*>(&raw);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) e[j] = fmaxf(e[j], -CUDART_INF_F);
+    } else {
+      using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      T2* p = reinterpret_cast<T2*>(&raw);
+      const uint32_t w = neg_inf_word<T>();
+      T2 low;
+      memcpy(&low, &w, 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[j] = __hmax2(p[j], low);
+    }
+    return raw;
+  };
   {
     constexpr int U = 4;
     for (int ch0 = wbeg + lane; ch0 < wend; ch0 += 32 * U) {
       uint4 raw[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) {
-        const int ch = ch0 + 32 * i, t0 = base + ch * VEC;
-        if (ch >= wend) continue;
-        if (t0 >= 0 && t0 + VEC <= V) {
-          raw[i] = __ldcs(reinterpret_cast<const uint4*>(lg + t0));
-        } else {
-          T* e = reinterpret_cast<T*>(&raw[i]);
-#pragma unroll
-          for (int j = 0; j < VEC; ++j) e[j] = t0 + j >= 0 && t0 + j < V ? lg[t0 + j] : round_f<T>(-CUDART_INF_F);
-        }
-      }
+      for (int i = 0; i < U; ++i)
+        if (ch0 + 32 * i < wend) raw[i] = fetch(ch0 + 32 * i);
 #pragma unroll
       for (int i = 0; i < U; ++i) {
         const int ch = ch0 + 32 * i;
         if (ch >= wend) continue;
-        T* e = reinterpret_cast<T*>(&raw[i]);
-        bool nan = false;
+        raw[i] = clean(raw[i]);
+        const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float v = to_f(e[j]);
-          nan |= v != v;
           if (j < VEC / 2) mx0 = fmaxf(mx0, v);
           else mx1 = fmaxf(mx1, v);
         }
-        if (nan) {
-#pragma unroll
-          for (int j = 0; j < VEC; ++j)
-            if (to_f(e[j]) != to_f(e[j])) e[j] = round_f<T>(-CUDART_INF_F);
-        }
-        *reinterpret_cast<uint4*>(seg + (int64_t)ch * VEC) = raw[i];
+        if constexpr (STAGE) *reinterpret_cast<uint4*>(seg + (int64_t)ch * VEC) = raw[i];
       }
     }
   }
   // 16 bytes of the part; past a warp's chunks (and around the row) -inf
   auto chunk = [&](int ch, int end) -> uint4 {
-    if (ch < end) return *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
     const uint32_t w = neg_inf_word<T>();
-    return make_uint4(w, w, w, w);
+    uint4 raw = make_uint4(w, w, w, w);
+    if (ch < end) {
+      if constexpr (STAGE) raw = *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
+      else raw = clean(fetch(ch));
+    }
+    if (inf_row) {  // the +inf logits share the weight, nothing else has any
+      T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) e[j] = to_f(e[j]) == CUDART_INF_F ? round_f<T>(0.f) : round_f<T>(-CUDART_INF_F);
+    }
+    return raw;
   };
   // f(value, token, is one) for the elements of the warp's chunks; every lane makes the same number of calls
   auto each = [&](auto f) {
+    uint4 next = chunk(wbeg + lane, wend);  // a step ahead
     for (int ch0 = wbeg; ch0 < wend; ch0 += 32) {
       const int ch = ch0 + lane;
-      const uint4 raw = chunk(ch, wend);
+      const uint4 raw = next;
+      next = chunk(ch + 32, wend);
       const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
@@ -284,7 +310,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       if (lane == 0) sh.k.warp_max[warp] = wm;
     }
     if (lane == 0) sh.scratch[warp] = wm;
-    if (tid == 0) sh.n = 0, sh.uncertain = 0;
+    if (tid == 0) sh.n = 0, sh.uncertain = 0, sh.key_lo = ~0u, sh.key_hi = 0u;
     if (tid < 8) sh.add[tid] = 0;
     __syncthreads();
     const uint32_t cm = __reduce_max_sync(0xffffffffu, (uint32_t)sh.scratch[lane % NW]);
@@ -327,16 +353,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     z_high = fminf(z_high, fmaxf(z_low, 1.f) * 1.001f * (float)((per_warp + 31) / 32 * (VEC / 2)));
     z_low = fmaxf(z_low * 0.999f, 1.f);
   }
-  if (m == CUDART_INF_F && !greedy) {  // the +inf logits share the weight, nothing else has any
-    all_sync();
-    for (int i = tid; i < nch * VEC; i += NT)
-      seg[i] = to_f(seg[i]) == CUDART_INF_F ? round_f<T>(0.f) : round_f<T>(-CUDART_INF_F);
+  if (m == CUDART_INF_F && !greedy) {
+    inf_row = true;
     m = 0.f;
     kmax = float_key(0.f);
     z_low = 1.f;
     z_high = (float)V;
     general |= top_k < V;  // (the list's maxima are of the logits as they were)
-    __syncthreads();
   }
   const double u = (double)a.u[row];
   auto finish = [&](int id, double w, double z) {
@@ -654,10 +677,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     draw(keep_of, [&](float v, int t) { return composite(v, t) >= thr; }, exact_of, 0);
   };
 
-  // A weight in float32 (ex2.approx, at most 2 ulp) errs relatively by at most
-  // err_1 + x err_x: x = (m - l) c carries 3 roundings, each moving the weight by
-  // x 2^-24 ln 2, the exponential 2^-22, and sums of VEC weights VEC roundings.
-  const float err_x = 3.f * 0.7f * 5.9604645e-8f, err_1 = (4.f + VEC) * 5.9604645e-8f;
+  // A weight 2^-x in float32 (ex2.approx, at most 2 ulp) errs relatively by at
+  // most err_1 + x err_x: x = (m - l) c carries up to 4 roundings, each moving the
+  // weight by x 2^-24 ln 2, the exponential 2^-22, and sums of VEC weights VEC
+  // roundings.  Of a sum S of weights the error is then at most S (err_1 + 32
+  // err_x) and that of the weights beyond x = 32, V 32 2^-32 err_x.
+  const double err_x = 4 * 0.7 * 0x1p-24, err_1 = (4 + VEC) * 0x1p-24;
+  auto sum_error = [&](double s) { return s * (err_1 + 32 * err_x) + V * 0x1p-27 * err_x; };
   if (!general && !by_mass) {
     // ---------------------------------------------------------------------
     // no top-k, no top-p: draw from the float32 masses when the drawn mass is
@@ -669,52 +695,43 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       return;
     }
     const float x_min = min_p > 0.0 ? (float)(-log2(min_p)) : CUDART_INF_F;
-    double sum = 0.0, err = 0.0;
+    double sum = 0.0;
     bool border = false;
+    uint4 next = chunk(wbeg + lane, wend);
     for (int ch = wbeg + lane; ch < wend; ch += 32) {
-      const uint4 raw = chunk(ch, wend);
+      const uint4 raw = next;
+      next = chunk(ch + 32, wend);
       const T* e = reinterpret_cast<const T*>(&raw);
-      float s = 0.f, se = 0.f;
+      float s = 0.f;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
         const float x = (m - to_f(e[j])) * cf;
-        const float w = x <= x_min ? ex2_f32(-x) : 0.f;
         border |= x_min < CUDART_INF_F && fabsf(x - x_min) <= 1e-6f * (x_min + 1.f);
-        s += w;
-        se = fmaf(w, fmaf(fminf(x, 200.f), err_x, err_1), se);
+        s += x <= x_min ? ex2_f32(-x) : 0.f;
       }
       sum += (double)s;
-      err += (double)se;
     }
     if (border) atomicOr(&sh.uncertain, 1);
     sum = warp_sumd(sum);
-    err = warp_sumd(err);
-    if (lane == 0) {
-      sh.w_keep[warp] = fixed(sum);
-      sh.w_err[warp] = err;
-    }
+    if (lane == 0) sh.w_keep[warp] = fixed(sum);
     __syncthreads();
     if (tid == 0) {
       u64 s = 0;
-      double e = 0.0;
-      for (int w = 0; w < NW; ++w) s += sh.w_keep[w], e += sh.w_err[w];
+      for (int w = 0; w < NW; ++w) s += sh.w_keep[w];
       sh.cta_keep = s;
-      sh.cta_err = e;
       sh.cta_ties = sh.uncertain;
     }
     all_sync();
-    u64 keep_of[CS];
-    double e = 0.0;
+    u64 keep_of[CS], z = 0;
     bool sure = true;
 #pragma unroll
     for (int r = 0; r < CS; ++r) {
-      keep_of[r] = peer(r)->cta_keep;
-      e += peer(r)->cta_err;
+      z += keep_of[r] = peer(r)->cta_keep;
       sure &= peer(r)->cta_ties == 0;
     }
     // both the running mass and u Z~ move with the error, and each token's and
     // warp's mass is rounded to the fixed point
-    const u64 slack = (u64)(2.0 * e * kWeightOne) + (u64)V + 64;
+    const u64 slack = (u64)(2.0 * sum_error((double)z / kWeightOne) * kWeightOne) + (u64)V + 64;
     if (sure)
       sure = draw(keep_of, [&](float v, int) { return (m - v) * cf <= x_min; },
                   [&](float v) { return fixed((double)ex2_f32((v - m) * cf)); }, slack);
@@ -725,6 +742,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   }
 
   u64 thr = 0;  // kept: composite >= thr
+  bool many = false;  // top-p with many tokens at the border: their keys, the mass above them and the reach
+  uint32_t m_lo = 0, m_hi = 0;
+  u64 m_above = 0;
+  double m_reach = 0.0;
   if (!general) {
     // ---------------------------------------------------------------------
     // top-p.  With z_low <= Z a token below (1 - p) z_low / V cannot stay (all
@@ -737,21 +758,34 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     // exactly as well.
     // ---------------------------------------------------------------------
     const float rest = fmaxf((float)(1.0 - top_p), 1e-17f);
-    const float x_end = fmaxf(log2f((float)V / z_low) - log2f(rest), 0.f) + 0.02f;
-    const float bin_scale = (float)kBins / x_end, unit = 2147483648.0f / z_high * (1.f - 1e-3f);
-    auto bin_at = [&](float v) { return (m - v) * cf * bin_scale; };  // falls with v; its floor is the bin
+    const float x_end = fmaxf(log2f((float)V / z_low) - log2f(rest), 0.f) * (1.f + 0x1p-9f) + 0.02f;
+    // bin of a logit, as the float 2^23 + bin: adding 2^23 rounds to an integer in
+    // the low mantissa bits (no conversion instruction), and falls with v
+    const float bin_scale = fminf(cf * ((float)kBins / x_end), 3e38f);
+    auto bin_at = [&](float v) { return fmaf(m - v, bin_scale, 8388608.f); };
+    const float bins_end = 8388608.f + (float)kBins;
+    // masses in units of at most 2^-22, so that they come out the same way and all of them stay below 2^31
+    const float unit = fminf(4194304.f, 2147483648.0f / z_high * (1.f - 1e-3f));
     for (int i = tid; i < kBins; i += NT) sh.p.hist[i] = 0;
     __syncthreads();
+    const uint32_t hist_s = smem_addr(sh.p.hist);
     double sum = 0.0;
+    uint4 next = chunk(wbeg + lane, wend);
     for (int ch = wbeg + lane; ch < wend; ch += 32) {
-      const uint4 raw = chunk(ch, wend);
+      const uint4 raw = next;
+      next = chunk(ch + 32, wend);
       const T* e = reinterpret_cast<const T*>(&raw);
       float s = 0.f;
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float x = (m - to_f(e[j])) * cf, w = ex2_f32(-x), b = x * bin_scale;
+        const float v = to_f(e[j]), b = bin_at(v), w = ex2_f32((v - m) * cf);
         s += w;
-        if (b < (float)kBins) atomicAdd(&sh.p.hist[(int)b], __float2uint_rn(w * unit));
+        const uint32_t at = hist_s + 4u * (__float_as_uint(b) - 0x4b000000u);
+        const uint32_t mass = __float_as_uint(fmaf(w, unit, 8388608.f)) - 0x4b000000u;
+        asm volatile(
+            "{\n .reg .pred p;\n setp.lt.f32 p, %0, %1;\n @p red.shared.add.u32 [%2], %3;\n}\n" ::"f"(b), "f"(bins_end),
+            "r"(at), "r"(mass)
+            : "memory");
       }
       sum += (double)s;
     }
@@ -795,109 +829,138 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       blo = min((int)(both & 0xffffu), kBins - 1);
       bhi = min((int)(both >> 16), kBins - 1);
     }
-    const float edge_lo = (float)blo, edge_hi = (float)(bhi + 1);
+    const float edge_lo = 8388608.f + (float)blo, edge_hi = 8388608.f + (float)(bhi + 1);
     u64 keep_of[CS];
-    u64 acc_keep, acc_all, acc_tail;
-    double tail, tail_err;
-    // the pass over the part: masses above the bins (exact), the bins' tokens, the tail
-    auto tally = [&](auto exact_tag) {
-      constexpr bool EXACT = decltype(exact_tag)::value;
-      acc_keep = acc_all = acc_tail = 0;
-      tail = tail_err = 0.0;
+    u64 acc_keep, acc_all;
+    double tail;
+    // the pass over the part: masses above the bins (exact), the bins' tokens, and the tail in float32
+    auto tally = [&]() {
+      acc_keep = acc_all = 0;
+      tail = 0.0;
       int fill = 0;
       float* q = sh.p.queue[warp];
       auto take_one = [&](float v) {
         const double w = weight(v, m, c);
         const u64 f = fixed(w);
-        if (!EXACT || bin_at(v) < edge_lo) {
-          acc_all += f;
-          if (w >= min_p) acc_keep += f;
-        } else {
-          acc_tail += f;
-        }
+        acc_all += f;
+        if (w >= min_p) acc_keep += f;
       };
+      uint4 next = chunk(wbeg + lane, wend);
       for (int ch0 = wbeg; ch0 < wend; ch0 += 32) {
         const int ch = ch0 + lane;
-        const uint4 raw = chunk(ch, wend);
+        const uint4 raw = next;
+        next = chunk(ch + 32, wend);
         const T* e = reinterpret_cast<const T*>(&raw);
-        float s = 0.f, se = 0.f;
+        float s = 0.f;
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float v = to_f(e[j]), x = (m - v) * cf, b = x * bin_scale;
-          const bool in_tail = !(b < edge_hi);
-          if (!EXACT) {
-            const float w = in_tail ? ex2_f32(-x) : 0.f;
-            s += w;
-            se = fmaf(w, fmaf(fminf(x, 200.f), err_x, err_1), se);
-          }
-          const bool take = b < edge_lo || (EXACT && in_tail);
-          if (b >= edge_lo && !in_tail) {
-            const unsigned at = atomicAdd(&sh.n, 1u);
-            if (at < kCands) sh.p.cand[at] = composite(v, base + ch * VEC + j);
+          const float v = to_f(e[j]), b = bin_at(v), w = ex2_f32((v - m) * cf);
+          const bool in_tail = b >= edge_hi, take = b < edge_lo;
+          s += in_tail ? w : 0.f;
+          const bool border = !in_tail && !take;
+          const unsigned bb = __ballot_sync(0xffffffffu, border);
+          if (bb) {
+            const uint32_t key = float_key(v + 0.f);
+            const uint32_t lo = __reduce_min_sync(0xffffffffu, border ? key : ~0u);
+            const uint32_t hi = __reduce_max_sync(0xffffffffu, border ? key : 0u);
+            unsigned at = 0;
+            if (lane == 0) {
+              at = atomicAdd(&sh.n, __popc(bb));
+              atomicMin(&sh.key_lo, lo);
+              atomicMax(&sh.key_hi, hi);
+            }
+            at = __shfl_sync(0xffffffffu, at, 0) + __popc(bb & ((1u << lane) - 1));
+            if (border && at < kCands) sh.p.cand[at] = composite(v, base + ch * VEC + j);
           }
           const unsigned bal = __ballot_sync(0xffffffffu, take);
-          if (bal) {
-            if (take) q[fill + __popc(bal & ((1u << lane) - 1))] = v;
-            fill += __popc(bal);
-            if (fill >= 32) {
-              __syncwarp();
-              const float y0 = q[lane], y1 = q[32 + lane];
-              __syncwarp();
-              q[lane] = y1;
-              fill -= 32;
-              take_one(y0);
-            }
+          if (take) q[fill + __popc(bal & ((1u << lane) - 1))] = v;
+          fill += __popc(bal);
+          if (fill >= 32) {
+            __syncwarp();
+            const float y0 = q[lane], y1 = q[32 + lane];
+            __syncwarp();
+            q[lane] = y1;
+            fill -= 32;
+            take_one(y0);
           }
         }
-        if (!EXACT) {
-          tail += (double)s;
-          tail_err += (double)se;
-        }
+        tail += (double)s;
       }
       __syncwarp();
       if (lane < fill) take_one(q[lane]);
       __syncwarp();
     };
-    bool resolved = false;
-    for (int pass = 0; pass < 2; ++pass) {
-      const bool exact_tail = pass == 1;
-      if (exact_tail) tally(std::true_type{});
-      else tally(std::false_type{});
-      acc_keep = warp_sum64(acc_keep);
-      acc_all = warp_sum64(acc_all);
-      tail = exact_tail ? (double)warp_sum64(acc_tail) / kWeightOne : warp_sumd(tail);
-      tail_err = warp_sumd(tail_err);
-      if (lane == 0) {
-        sh.w_keep[warp] = acc_keep;
-        sh.w_all[warp] = acc_all;
-        sh.w_sum[warp] = tail;
-        sh.w_err[warp] = tail_err;
-      }
-      __syncthreads();
-      if (tid == 0) {
-        u64 k = 0, al = 0;
-        double s = 0.0, e = 0.0;
-        for (int w = 0; w < NW; ++w) k += sh.w_keep[w], al += sh.w_all[w], s += sh.w_sum[w], e += sh.w_err[w];
-        sh.cta_keep = k, sh.cta_all = al, sh.cta_sum = s, sh.cta_err = e;
-      }
-      all_sync();
-      u64 above = 0;
-      double tl = 0.0, te = 0.0;
-      unsigned n = 0;
-      int src = -1;
-      u64 own = 0;
+    // the tail once more, exactly: four independent exponentials at a time
+    auto exact_tail_sum = [&]() -> u64 {
+      u64 acc = 0;
+      uint4 next = chunk(wbeg + lane, wend);
+      for (int ch = wbeg + lane; ch < wend; ch += 32) {
+        const uint4 raw = next;
+        next = chunk(ch + 32, wend);
+        const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-      for (int r = 0; r < CS; ++r) {
-        const SampleShared* q = peer(r);
-        keep_of[r] = q->cta_keep;
-        above += q->cta_all;
-        tl += q->cta_sum;
-        te += q->cta_err;
-        const unsigned k = q->n;
-        if (tid >= n && tid < n + k && k <= kCands) own = q->p.cand[tid - n], src = r;
-        n += k;
+        for (int j = 0; j < VEC; ++j) {
+          const float v = to_f(e[j]);
+          // (a tail token is below the largest; beyond x = 60 its mass is 0)
+          const double x = fmin(((double)m - (double)v) * c, 60.0);
+          const u64 f = __double2ull_rn(exp2_neg(x) * kWeightOne);
+          acc += bin_at(v) >= edge_hi && x < 60.0 ? f : 0;
+        }
       }
-      if (n == 0 || n > kCands) break;  // too many tokens at the border: the general way
+      return acc;
+    };
+    tally();
+    acc_keep = warp_sum64(acc_keep);
+    acc_all = warp_sum64(acc_all);
+    tail = warp_sumd(tail);
+    if (lane == 0) {
+      sh.w_keep[warp] = acc_keep;
+      sh.w_all[warp] = acc_all;
+      sh.w_sum[warp] = tail;
+    }
+    __syncthreads();
+    if (tid == 0) {
+      u64 k = 0, al = 0;
+      double s = 0.0;
+      for (int w = 0; w < NW; ++w) k += sh.w_keep[w], al += sh.w_all[w], s += sh.w_sum[w];
+      sh.cta_keep = k, sh.cta_all = al, sh.cta_sum = s;
+    }
+    all_sync();
+    u64 above = 0, own = 0;
+    double tl = 0.0;
+    unsigned n = 0;
+    uint32_t key_lo = ~0u, key_hi = 0u;
+    int src = -1;
+#pragma unroll
+    for (int r = 0; r < CS; ++r) {
+      const SampleShared* q = peer(r);
+      key_lo = min(key_lo, q->key_lo);
+      key_hi = max(key_hi, q->key_hi);
+      keep_of[r] = q->cta_keep;
+      above += q->cta_all;
+      tl += q->cta_sum;
+      const unsigned k = q->n;
+      if (tid >= n && tid < n + k && k <= kCands) own = q->p.cand[tid - n], src = r;
+      n += k;
+    }
+    double te = sum_error(tl);
+    // the tail exactly, on demand: the same answer in every CTA
+    auto refine_tail = [&]() {
+      const u64 t = block_sum(exact_tail_sum());
+      if (tid == 0) sh.cta_ties = t;
+      all_sync();
+      u64 all = 0;
+#pragma unroll
+      for (int r = 0; r < CS; ++r) all += peer(r)->cta_ties;
+      tl = (double)all / kWeightOne;
+      te = 0.0;
+    };
+    // bounds of the mass that has to come before a token for it to be dropped, `in` being the bins' own mass
+    auto reach_of = [&](u64 in, double sign) {
+      return top_p * ((double)(above + in) + (tl + sign * te) * kWeightOne * (1.0 + sign * 1e-9) + sign * V);
+    };
+    bool resolved = false;
+    if (n > 0 && n <= kCands) {
       // thread i < n holds token i of the border: its weight for the others
       const double own_w = src >= 0 ? weight(key_float((uint32_t)(own >> 32)), m, c) : 0.0;
       if (src >= 0) {
@@ -925,42 +988,48 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       }
       const bool first = above == 0 && rk == 0;  // the most likely token stays
       before += above;
-      const double zx = (double)(above + cands);
-      const double reach = top_p * (zx + tl * kWeightOne);
+      if (__syncthreads_or(have && ((double)before < reach_of(cands, -1.0)) != ((double)before < reach_of(cands, 1.0))))
+        refine_tail();
+      const double reach = top_p * ((double)(above + cands) + tl * kWeightOne);
       const bool keep = have && (first || (double)before < reach);
-      if (!exact_tail) {
-        const double reach_lo = top_p * (zx + (tl - te) * kWeightOne * (1.0 - 1e-9) - V);
-        const double reach_hi = top_p * (zx + (tl + te) * kWeightOne * (1.0 + 1e-9) + V);
-        const bool unsure = have && ((double)before < reach_lo) != ((double)before < reach_hi);
-        if (__syncthreads_or(unsure)) {
-          all_sync();  // the lists and sums have been read by every CTA
-          if (tid == 0) sh.n = 0;
-          __syncthreads();
-          continue;
-        }
-      }
       // the border does lie in these bins (their histogram is approximate)
-      if (!((above == 0 || (double)above < reach) && zx >= reach)) break;
-      // threshold: the last kept token, or just above the first of them
-      const unsigned kept = block_sum32(keep && part == 0);
-      if (part == 0 && have && (kept ? rk == kept - 1 : rk == 0)) sh.thr = kept ? mine : mine + 1;
-      // the kept join the masses of their CTAs and of this CTA's warps
-      __syncthreads();
-      thr = sh.thr;
-      if (src >= 0 && own >= thr && own_w >= min_p) {
-        const u64 f = fixed(own_w);
-        atomicAdd(&sh.add[src], f);
-        if (src == rank) atomicAdd(&sh.w_keep[(((int)(0xffffffffu - (uint32_t)own) - base) / VEC) / per_warp], f);
-      }
-      __syncthreads();
+      if ((above == 0 || (double)above < reach) && (double)(above + cands) >= reach) {
+        // threshold: the last kept token, or just above the first of them
+        const unsigned kept = block_sum32(keep && part == 0);
+        if (part == 0 && have && (kept ? rk == kept - 1 : rk == 0)) sh.thr = kept ? mine : mine + 1;
+        // the kept join the masses of their CTAs and of this CTA's warps
+        __syncthreads();
+        thr = sh.thr;
+        if (src >= 0 && own >= thr && own_w >= min_p) {
+          const u64 f = fixed(own_w);
+          atomicAdd(&sh.add[src], f);
+          if (src == rank) atomicAdd(&sh.w_keep[(((int)(0xffffffffu - (uint32_t)own) - base) / VEC) / per_warp], f);
+        }
+        __syncthreads();
 #pragma unroll
-      for (int r = 0; r < CS; ++r) keep_of[r] += sh.add[r];
-      resolved = true;
-      break;
+        for (int r = 0; r < CS; ++r) keep_of[r] += sh.add[r];
+        resolved = true;
+      }
     }
     if (resolved) {
       draw(keep_of, [&](float v, int t) { return composite(v, t) >= thr; }, exact_of, 0);
       return;
+    }
+    if (n > kCands) {  // too many to rank: the border key is sought among theirs, with exact sums
+      many = true;
+      refine_tail();
+      u64 in = 0;
+      packed([&](float v, int) { const uint32_t k = float_key(v + 0.f); return k >= key_lo && k <= key_hi; },
+             [&](float v) { in += fixed(weight(v, m, c)); });
+      in = block_sum(in);
+      if (tid == 0) sh.cta_all = in;
+      all_sync();
+      in = 0;
+#pragma unroll
+      for (int r = 0; r < CS; ++r) in += peer(r)->cta_all;
+      m_lo = key_lo, m_hi = key_hi, m_above = above;
+      m_reach = top_p * ((double)(above + in) + tl * kWeightOne);
+      many = (above == 0 || (double)above < m_reach) && (double)(above + in) >= m_reach;  // (or the bins were wrong)
     }
     all_sync();
   }
@@ -970,16 +1039,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   // (top-k) and masses (top-p); then the place of the last kept token among
   // those of the border key
   // -----------------------------------------------------------------------
-  // largest K with the sum over keys >= K reaching `target`; *above = the sum over keys > K
-  auto select = [&](bool by_weight, double target, u64* above) -> uint32_t {
-    uint32_t prefix = 0;
-    u64 run = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+  // largest K in [lo, hi] with `run` (the sum over keys > hi) plus the sum over
+  // keys K .. hi reaching `target`; *above = the sum over keys > K
+  auto select = [&](bool by_weight, double target, uint32_t lo, uint32_t hi, u64 run, u64* above) -> uint32_t {
+    const int first = lo == hi ? -8 : (31 - __clz(lo ^ hi)) / 8 * 8;
+    uint32_t prefix = lo == hi ? hi : first == 24 ? 0u : hi & (~0u << (first + 8));
+    for (int shift = first; shift >= 0; shift -= 8) {
+      const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
       for (int i = tid; i < 256; i += NT) sh.p.mass[i] = 0;
       __syncthreads();
       each([&](float v, int, bool in) {
         const uint32_t k = float_key(v + 0.f);
-        const bool take = in && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)));
+        const bool take = in && k >= lo && k <= hi && (k & mask) == prefix;
         const unsigned act = __ballot_sync(0xffffffffu, take);
         if (!act) return;
         u64 w = 0;
@@ -1013,33 +1084,39 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   };
   all_sync();  // (a list that was too long has been counted by every CTA)
   uint32_t K = 0;
-  u64 ties = ~0ull, above = 0, zk;
-  if (top_k < V) {
-    K = select(false, (double)top_k, &above);
-    ties = (u64)top_k - above;
-  }
-  {  // mass of the top-k set
-    u64 acc = 0;
+  u64 ties = ~0ull, above = 0;
+  double reach = m_reach;
+  bool by_reach = many;  // of the tokens of key K those stay that have less than `reach` before them
+  if (many) {
+    K = select(true, reach, m_lo, m_hi, m_above, &above);
+  } else {
+    if (top_k < V) {
+      K = select(false, (double)top_k, 0, kmax, 0, &above);
+      ties = (u64)top_k - above;
+    }
+    // mass of the top-k set
+    u64 acc = 0, zk = 0;
     packed([&](float v, int) { return float_key(v + 0.f) > K; }, [&](float v) { acc += fixed(weight(v, m, c)); });
     acc = block_sum(acc);
     if (tid == 0) sh.cta_all = acc;
     all_sync();
-    zk = 0;
 #pragma unroll
     for (int r = 0; r < CS; ++r) zk += peer(r)->cta_all;
     if (top_k < V) zk += ties * fixed(weight(key_float(K), m, c));
-  }
-  if (top_p < 1.0) {
-    const double reach = top_p * (double)zk;
-    uint32_t kp = select(true, reach, &above);
-    if (kp > kmax || reach <= 0.0) kp = kmax, above = 0;
-    if (kp > K) {
-      K = kp;
-      ties = ~0ull;
-    } else if (top_k < V) {  // the border lies among the ties of the top-k border
-      above = zk - ties * fixed(weight(key_float(K), m, c));
+    if (top_p < 1.0) {
+      by_reach = true;
+      reach = top_p * (double)zk;
+      uint32_t kp = select(true, reach, 0, kmax, 0, &above);
+      if (reach <= 0.0) kp = kmax, above = 0;
+      if (kp > K) {
+        K = kp;
+        ties = ~0ull;
+      } else if (top_k < V) {  // the border lies among the ties of the top-k border
+        above = zk - ties * fixed(weight(key_float(K), m, c));
+      }
     }
-    // of the ties those stay that have less than the reach before them
+  }
+  if (by_reach) {
     const u64 w = fixed(weight(key_float(K), m, c));
     u64 n = w ? (u64)fmin(fmax(0.0, (reach - (double)above) / (double)w), 262144.0) : 0;
     while (n > 0 && (double)(above + (n - 1) * w) >= reach) --n;
@@ -1104,13 +1181,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   draw_exact(thr);
 }
 
-template <typename T, int CS>
-static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
-  constexpr int VEC = 16 / (int)sizeof(T);
-  const int per_cta = ((VEC - 1 + a.vocab + VEC - 1) / VEC + CS - 1) / CS;
-  const int smem = max(per_cta * 16, kList * 16);  // a list takes the part's place, with its weights
-  auto* kern = sample_kernel<T, CS>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+// Parts up to this size are staged: two CTAs then share an SM.
+constexpr int kStageBytes = 99 * 1024;
+
+template <typename T, int CS, bool STAGE>
+static int launch_sample_as(const SampleArgs<T>& a, int part, cudaStream_t s) {
+  const int smem = max(STAGE ? part : 0, kList * 16);  // a list takes the part's place, with its weights
+  auto* kern = sample_kernel<T, CS, STAGE>;
+  if (STAGE && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * CS);
@@ -1127,13 +1205,20 @@ static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
   return launch_status();
 }
 
-// CTAs per row: as few as keep a part within 100 KB (two CTAs per SM: the
-// barriers and scalar steps of a row are paid per CTA), then more while the
-// rows alone do not fill the GPU and a thread still has four tokens.
-template <typename T>
+template <typename T, int CS>
+static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  const int part = ((VEC - 1 + a.vocab + VEC - 1) / VEC + CS - 1) / CS * 16;
+  return part <= kStageBytes ? launch_sample_as<T, CS, true>(a, part, s) : launch_sample_as<T, CS, false>(a, part, s);
+}
+
+// CTAs per row: one when the rows alone occupy every SM (the barriers and scalar
+// steps of a row are paid per CTA), else more while a thread still has eight
+// tokens.  50257 tokens in float32: 64 rows with top-p 28.8 us on 4 CTAs each,
+// 53.5 on 8; 256 rows 83.3 us on one (read again from L2), 76.6 on two; with
+// top-k 50 33.8 and 42.8 us; 128 rows with top-k 500 45.1 on 2, 73.3 on 4.
 static int sample_cluster(int64_t rows, int vocab) {
   int cs = 1;
-  while (cs < 8 && (int64_t)vocab * (int)sizeof(T) > cs * 101000ll) cs *= 2;
   while (cs < 8 && rows * cs < 148 && vocab / cs > kSampleThreads * 8) cs *= 2;
   return cs;
 }
@@ -1162,7 +1247,7 @@ extern "C" walsh_status walsh_sample_tokens(const void* logits, int dtype, int64
     a.temperature_r = temperature_rows, a.top_p_r = top_p_rows, a.min_p_r = min_p_rows, a.top_k_r = top_k_rows;
     a.ids = ids, a.logp = logp;
     cudaStream_t s = (cudaStream_t)stream;
-    switch (sample_cluster<ET>(rows, vocab)) {
+    switch (sample_cluster(rows, vocab)) {
       case 1: return launch_sample<ET, 1>(a, s);
       case 2: return launch_sample<ET, 2>(a, s);
       case 4: return launch_sample<ET, 4>(a, s);
