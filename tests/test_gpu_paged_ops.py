@@ -99,6 +99,32 @@ def test_append_out_of_range_is_reported_and_skipped():
     assert torch.equal(vp.transpose(1, 2).flatten(0, 1).any(-1).any(-1).cpu(), stored)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("norm", [False, True])
+def test_append_rows_on_16_byte_boundaries_only(dtype, norm):
+    """Rows, tables and pages that start 16 but not 32 bytes into their memory; an odd start is copied first."""
+    g = gen(17)
+    n, h, hd, page, e = 21, 3, 32, 4, 16 // torch.tensor([], dtype=dtype).element_size()
+    for shift in (e, 1):
+        flat = torch.randn(n * (3 * h * hd + e) + shift, generator=g).to(dtype).to(DEV)
+        x = flat[shift:].view(n, 3 * h * hd + e)[:, :3 * h * hd].unflatten(1, (3, h, hd))
+        q, k, v = x[:, 0], x[:, 1], x[:, 2]
+        pool = torch.zeros(2, 8 * h * page * (hd + e) + e, dtype=dtype, device=DEV)
+        kp, vp = (t[e:].view(8, h, page, hd + e)[..., :hd] for t in pool)
+        slots = torch.randperm(8 * page, generator=g)[:n].to(DEV)
+        pos = torch.arange(n, device=DEV)
+        tab = torch.randn(2 * n * hd // 2 + 2, generator=g).to(DEV)
+        cos, sin = tab[1:1 + n * hd // 2].view(n, hd // 2), tab[1 + n * hd // 2:1 + n * hd].view(n, hd // 2)
+        w = (1 + torch.rand(hd, generator=g)).to(DEV) if norm else None
+        out = ops.paged_append(q, k, v, kp, vp, slots, positions=pos, rope=(cos, sin), q_norm=w, k_norm=w)
+        wq, bq = R.rotate(q, w, cos, sin)
+        wk, bk = R.rotate(k, w, cos, sin)
+        close(out, wq, bq)
+        close(kp[slots // page, :, slots % page], wk, bk)
+        assert torch.equal(vp[slots // page, :, slots % page], v)
+        assert int((pool != 0).sum()) == int((kp != 0).sum()) + int((vp != 0).sum())
+
+
 def test_append_of_nothing():
     kp = torch.zeros(1, 2, 4, 16, device=DEV)
     x = torch.zeros(0, 2, 16, device=DEV)
@@ -302,6 +328,20 @@ def test_prefill_long(dtype, hq, hk, hd):
 def test_prefill_max_q_only_sizes_the_grid():
     run_prefill(torch.float16, 4, 2, 32, [300, 1, 77], [5, 0, 0], 16, 0, 0, max_q=10)
     run_prefill(torch.float32, 4, 2, 32, [300, 1, 77], [5, 0, 0], 16, 50, 2, max_q=10)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_prefill_tiles_without_keys_among_others(dtype):
+    """More queries than keys over several tiles: the first see nothing, the later ones their keys."""
+    g = gen(18)
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [70], 1, 8, 16, dtype))
+    q = torch.randn(500, 1, 16, generator=g).to(dtype).to(DEV)
+    off = torch.tensor([0, 500], dtype=torch.int32, device=DEV)
+    for max_q in (500, 40):
+        o = ops.paged_prefill_attention(q, off, kp, vp, table, kl, max_q=max_q)
+        assert not o[:430].any()
+        want, bound = R.attend(q[430:], R.gather_keys(kp, table[0], 70), R.gather_keys(vp, table[0], 70), 0)
+        close(o[430:], want, bound)
 
 
 def test_prefill_of_one_token_each_equals_decode():

@@ -111,6 +111,27 @@ def test_wide_spread_and_the_largest_vocabulary():
     check(*rand(2, 9000, 12, spread=1e30), top_k=4000)
 
 
+@pytest.mark.parametrize("kw", [dict(top_p=0.95), dict(top_p=0.5, min_p=0.01), dict(top_p=0.9, temperature=30.0)], ids=str)
+def test_many_tokens_at_a_top_p_border(kw):
+    """Far more equal or nearly equal logits at the border than are ranked one by one."""
+    check(*rand(3, 100001, 15, torch.bfloat16), **kw)
+    logits, u = rand(3, 20000, 16)
+    check((logits * 4).round() / 4, u, **kw)
+    check(logits * 1e-4, u, **kw)
+
+
+@pytest.mark.parametrize("rows,vocab", [(150, 3000), (150, 40000), (40, 20000)])
+def test_parts_held_or_read_again(rows, vocab):
+    """One CTA per row or several, with and without room to hold the row."""
+    check(*rand(rows, vocab, 17), top_p=0.9, min_p=0.01)
+    check(*rand(rows, vocab, 18, torch.float16), top_k=40, top_p=0.9)
+    logits, u = rand(rows, vocab, 19)
+    logits[::7, 5] = float("inf")
+    logits[1::7, ::2] = float("nan")
+    check(logits, u, temperature=0.7)
+    check(logits, u, top_p=0.8)
+
+
 def test_rows_of_a_wider_matrix():
     big, u = rand(9, 1100, 13)
     check(big[::2, 3:1003], u[:5].contiguous(), top_p=0.8)

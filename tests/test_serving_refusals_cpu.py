@@ -172,3 +172,27 @@ def test_wrappers_refuse_what_does_not_fit(no_device_check):
         with pytest.raises(ValueError):
             c()
             pytest.fail(f"case {i} was accepted")
+
+
+def test_calls_run_on_the_tensors_device(monkeypatch):
+    """Tensors on another device than the current one: the call is made under
+    their device, with its stream; on the current device nothing is switched."""
+    log = []
+
+    class Guard:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            log.append(("enter", self.dev))
+
+        def __exit__(self, *a):
+            log.append(("exit", self.dev))
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 0, raising=False)
+    monkeypatch.setattr(torch.cuda, "device", Guard)
+    monkeypatch.setattr(ops, "stream", lambda: 77)
+    monkeypatch.setattr(ops, "call", lambda name, *a: log.append((name,) + a))
+    ops._call_on(0, "x", 1)
+    ops._call_on(3, "y", 2)
+    assert log == [("x", 1, 77), ("enter", 3), ("y", 2, 77), ("exit", 3)]

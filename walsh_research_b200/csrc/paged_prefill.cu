@@ -553,6 +553,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
         else step(std::false_type{}, x0, st, false);
       }
     }
+    cp_async_wait<0>();  // (a tile whose rows see nothing has started its first stage all the same)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll

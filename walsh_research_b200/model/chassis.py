@@ -11,6 +11,7 @@ import torch.nn as nn
 
 from .. import ops
 from . import _prep
+from .paged import PagedLayer
 from .fht_cuda import HadamardHeadMixerFused, HadamardTernaryLinearTuple
 
 
@@ -179,6 +180,21 @@ class CausalSelfAttention(nn.Module):
         return (self.algebra == "hadamard" and x.dtype == torch.float16 and self.n_embd in (512, 2048)
                 and self.head_dim % 16 == 0)
 
+    def _attend(self, x, project, k_cache, v_cache, start_pos: int):
+        """q/k/v, the cache write and attention: [B, T, H, hd].  ``project(x,
+        start_pos, q, k, v)`` writes rotated q and k and v [B, H, T, hd].  With
+        a PagedLayer as k_cache the B T tokens are projected as one row of
+        tokens (the rope rows are each token's own) and stored page by page."""
+        B, T, C = x.shape
+        H, hd = self.n_head, self.head_dim
+        if isinstance(k_cache, PagedLayer):
+            qkv = torch.empty((3, 1, H, B * T, hd), dtype=k_cache.dtype, device=x.device)
+            project(x.reshape(1, B * T, C), 0, *qkv)
+            return k_cache.attend(*(t[0].transpose(0, 1) for t in qkv)).view(B, T, H, hd)
+        q = torch.empty((B, H, T, hd), dtype=k_cache.dtype, device=x.device)
+        project(x, start_pos, q, k_cache, v_cache)
+        return ops.attention(q, k_cache, v_cache, start_pos)
+
     def forward_site(self, x, rope_cos, rope_sin, k_cache, v_cache, start_pos: int, xs, hmix):
         """Attention plus the mHC site epilogue: xs [B, T, n, C] <- H_res xs + H_post attn(x)."""
         if self.algebra != "hadamard":
@@ -188,11 +204,10 @@ class CausalSelfAttention(nn.Module):
             return ops.mhc_post(xs, f, hmix, out=xs)
         B, T, C = x.shape
         H, hd = self.n_head, self.head_dim
-        q = torch.empty((B, H, T, hd), dtype=x.dtype, device=x.device)
         # one tcgen05 GEMM over the dense q | k | v matrix, RoPE and the cache write in its epilogue
         w, sc = self._qkv_dense(x.dtype)
-        ops.octo_qkv(x, H, w, sc, rope_cos, rope_sin, start_pos, q, k_cache, v_cache)
-        o = ops.attention(q, k_cache, v_cache, start_pos)
+        o = self._attend(x, lambda u, start, q, k, v: ops.octo_qkv(u, H, w, sc, rope_cos, rope_sin, start, q, k, v),
+                         k_cache, v_cache, start_pos)
         if B * T >= ops.ATTN_OUT_DENSE_FROM:
             # mixer and wo folded into one tcgen05 GEMM, the site update in its
             # epilogue (or, for few tokens, mhc_post after it)
@@ -215,14 +230,14 @@ class CausalSelfAttention(nn.Module):
         at cache rows start_pos.. (q/k/v in the caches' dtype); returns the wo
         output [B, T, C] in out_dtype (default x's)."""
         B, T, C = x.shape
-        H, hd = self.n_head, self.head_dim
-        q = torch.empty((B, H, T, hd), dtype=k_cache.dtype, device=x.device)
-        if self.algebra == "hadamard":
-            ops.attn_qkv(x, H, self._triple(self.wq), self._triple(self.wk), self._triple(self.wv),
-                         rope_cos, rope_sin, start_pos, q, k_cache, v_cache)
-        else:
-            self._octonion_qkv(x, rope_cos, rope_sin, start_pos, q, k_cache, v_cache)
-        o = ops.attention(q, k_cache, v_cache, start_pos)           # [B, T, H, hd]
+
+        def project(u, start, q, k, v):
+            if self.algebra == "hadamard":
+                ops.attn_qkv(u, self.n_head, self._triple(self.wq), self._triple(self.wk), self._triple(self.wv),
+                             rope_cos, rope_sin, start, q, k, v)
+            else:
+                self._octonion_qkv(u, rope_cos, rope_sin, start, q, k, v)
+        o = self._attend(x, project, k_cache, v_cache, start_pos)   # [B, T, H, hd]
         y = o.view(B, T, C)
         if self.algebra == "hadamard":
             if self.head_mixer is not None:
@@ -244,9 +259,8 @@ class CausalSelfAttention(nn.Module):
         mixer and wo with the mHC site epilogue."""
         from .cayley_dickson_cuda import folded_output
         B, T, C = x.shape
-        q = torch.empty((B, self.n_head, T, self.head_dim), dtype=k_cache.dtype, device=x.device)
-        self._octonion_qkv(x, rope_cos, rope_sin, start_pos, q, k_cache, v_cache)
-        o = ops.attention(q, k_cache, v_cache, start_pos)
+        o = self._attend(x, lambda u, start, q, k, v: self._octonion_qkv(u, rope_cos, rope_sin, start, q, k, v),
+                         k_cache, v_cache, start_pos)
         w, s = folded_output(self, o.dtype)
         return ops.octo_post(o.view(B, T, C), w, s, xs, hmix, out=xs)
 

@@ -25,6 +25,7 @@ import torch.nn.functional as F
 from .. import _lib, ops
 from . import _prep
 from .chassis import CausalSelfAttention, KVCache, RMSNorm, WalshConfig, precompute_freqs_cis, rope_tables
+from .paged import PagedBatch, PagedKVCache
 
 MAP_EPS = float(torch.finfo(torch.float32).eps)
 
@@ -430,9 +431,16 @@ class mHCWalsh(nn.Module):
         err = torch.zeros(1, dtype=torch.int32, device=idx.device)
         x = ops.embed_gather(idx, self.stream_table(dt), err).view(B, T, n, C)
         cos_all, sin_all = rope_tables(self, self.freqs_cis)
-        cos, sin = cos_all[start_pos:start_pos + T], sin_all[start_pos:start_pos + T]
         idt = _lib.inner_dtype(dt)
-        if kv_cache is None:
+        step = None
+        if isinstance(kv_cache, PagedBatch):
+            step = self._begin_paged(kv_cache, B, T, start_pos, idt, cos_all.shape[0])
+            cos, sin = cos_all[step.positions], sin_all[step.positions]
+        else:
+            cos, sin = cos_all[start_pos:start_pos + T], sin_all[start_pos:start_pos + T]
+        if step is not None:
+            pass
+        elif kv_cache is None:
             H, hd = self.config.n_head, C // self.config.n_head
             kc = torch.empty((B, H, T, hd), dtype=idt, device=idx.device)
             vc = torch.empty_like(kc)
@@ -446,7 +454,9 @@ class mHCWalsh(nn.Module):
             self._layers_in_parts(x, cos, sin, kv_cache, parts)
         else:
             for l, layer in enumerate(self.layers):
-                if kv_cache is not None:
+                if step is not None:
+                    kc, vc, cpos = step.layer(l), None, 0
+                elif kv_cache is not None:
                     kc, vc = kv_cache.k_cache[l], kv_cache.v_cache[l]
                     cpos = kv_cache.cached_len
                 else:
@@ -470,6 +480,19 @@ class mHCWalsh(nn.Module):
             return logits, loss, h_out
         return logits, loss
 
+    @staticmethod
+    def _begin_paged(batch, B, T, start_pos, idt, n_pos):
+        """Where this forward's B x T tokens go in a paged cache (positions are the sequences' own lengths)."""
+        if batch.dtype != idt or batch.batch_size != B:
+            raise ValueError(f"the paged batch is of {batch.batch_size} sequences in {batch.dtype}; this forward needs "
+                             f"{B} in {idt}")
+        if start_pos != 0:
+            raise ValueError("start_pos does not apply to a paged cache: every sequence continues at its own length")
+        step = batch.begin(T)
+        if step.max_len > n_pos:
+            raise ValueError(f"position {step.max_len - 1} is beyond the {n_pos} of the rotation table")
+        return step
+
     # Batched decode can run the batch in `decode_streams` parts, each on its
     # own CUDA stream: sequences share nothing inside the layer stack, so one
     # part's latency-bound small kernels (mapping, projections, router, MoE,
@@ -483,7 +506,8 @@ class mHCWalsh(nn.Module):
     DECODE_PARTS_FROM = 128  # batch size from which a T <= 4 step is split
 
     def _decode_parts(self, B, T, kv_cache):
-        if kv_cache is None or T > 4 or B < self.DECODE_PARTS_FROM or self.decode_streams < 2:
+        if (kv_cache is None or isinstance(kv_cache, PagedBatch) or T > 4 or B < self.DECODE_PARTS_FROM
+                or self.decode_streams < 2):
             return 1
         if torch.is_grad_enabled() or any(l.__dict__.get("_ep") is not None for l in self.layers):
             return 1
@@ -582,8 +606,77 @@ class mHCWalsh(nn.Module):
             z = z.masked_fill(z < kth, float("-inf"))
         return torch.multinomial(F.softmax(z, dim=-1), num_samples=1, generator=generator)
 
+    @classmethod
+    def _draw(cls, logits, temperature, top_k, generator=None, top_p=None, min_p=None):
+        """One token per row [B, 1]: the reference's rule, or with top_p or min_p
+        ops.sample_tokens from uniform numbers of the generator."""
+        if top_p is None and min_p is None:
+            return cls._sample(logits, temperature, top_k, generator)
+        u = torch.rand(logits.shape[0], device=logits.device, generator=generator)
+        return ops.sample_tokens(logits, u, temperature=temperature, top_k=top_k or 0,
+                                 top_p=1.0 if top_p is None else top_p, min_p=min_p or 0.0)[:, None]
+
     @torch.no_grad()
-    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, use_cache=True, generator=None):
+    def generate_batch(self, prompts, max_new_tokens, temperature=1.0, top_k=None, top_p=None, min_p=None, window=0,
+                       sinks=0, stop_token=None, page_size=64, max_seq_len=None, generator=None):
+        """Continuations of prompts of different lengths (a list of 1-D id
+        tensors on the model's device), decoded together over a paged cache:
+        one forward per prompt length, then one per step for all sequences
+        still running, tokens drawn by ops.sample_tokens.  Returns a list of 1-D
+        tensors, prompt and continuation.  A sequence ends after
+        ``max_new_tokens``, at ``stop_token`` (kept; checked on the host every
+        step when given) or when ``max_seq_len`` (default block_size, at most
+        the rotation table's 2 block_size) tokens are cached.  ``window`` and
+        ``sinks`` as in PagedKVCache."""
+        limit = self.config.block_size if max_seq_len is None else int(max_seq_len)
+        if not 0 < limit <= self.freqs_cis.shape[0]:
+            raise ValueError(f"max_seq_len must be in 1 .. {self.freqs_cis.shape[0]}, got {limit}")
+        prompts = [p[-limit:] for p in prompts]
+        if any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+            raise ValueError("prompts must be non-empty 1-D tensors of token ids")
+        if max_new_tokens <= 0 or not prompts:
+            return list(prompts)
+        C, H, dev = self.config.n_embd, self.config.n_head, prompts[0].device
+        grown = [min(limit, p.numel() + max_new_tokens - 1) for p in prompts]
+        cache = PagedKVCache(self.config.n_layer, sum(-(-n // page_size) for n in grown), page_size, H, C // H, dev,
+                             dtype=_lib.inner_dtype(self._act_dtype()), max_seqs=len(prompts), max_seq_len=limit,
+                             window=window, sinks=sinks)
+        seqs = cache.add(len(prompts))
+        draw = lambda z: self._draw(z, temperature, top_k, generator, 1.0 if top_p is None else top_p, min_p)  # noqa: E731
+        logits = [None] * len(prompts)
+        for n in sorted({p.numel() for p in prompts}):
+            members = [i for i, p in enumerate(prompts) if p.numel() == n]
+            batch = cache.select([seqs[i] for i in members])
+            out, _ = self(torch.stack([prompts[i] for i in members]), kv_cache=batch)
+            batch.increment(n)
+            for i, row in zip(members, out[:, -1]):
+                logits[i] = row
+        nxt = draw(torch.stack(logits))
+        tokens = [[t] for t in nxt[:, 0].unbind()]
+        live = list(range(len(prompts)))
+        for _ in range(max_new_tokens - 1):
+            if stop_token is not None:
+                going = (nxt[:, 0] != stop_token).tolist()
+            else:
+                going = [True] * len(live)
+            full = [n >= limit for n in cache.lengths([seqs[i] for i in live])]
+            stay = [j for j, (g, f) in enumerate(zip(going, full)) if g and not f]
+            if len(stay) < len(live):
+                cache.remove([seqs[live[j]] for j in range(len(live)) if j not in set(stay)])
+                nxt, live = nxt[stay], [live[j] for j in stay]
+            if not live:
+                break
+            batch = cache.select([seqs[i] for i in live])
+            out, _ = self(nxt, kv_cache=batch)
+            batch.increment(1)
+            nxt = draw(out[:, -1])
+            for i, t in zip(live, nxt[:, 0].unbind()):
+                tokens[i].append(t)
+        return [torch.cat((p, torch.stack(t).to(p.dtype))) for p, t in zip(prompts, tokens)]
+
+    @torch.no_grad()
+    def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, use_cache=True, generator=None, top_p=None,
+                 min_p=None):
         """Autoregressive sampling, [B, T] -> [B, T + new] token ids, with the
         reference's per-step rule (temperature, optional top-k, multinomial;
         src/model/mhc.py:753-789).
@@ -595,7 +688,8 @@ class mHCWalsh(nn.Module):
         generation stops early once the cache is full.  use_cache=False
         re-forwards the cropped context for every token, as mHCWalsh.generate
         does in the reference.  ``generator`` seeds the draws (a
-        torch.Generator on the model's device)."""
+        torch.Generator on the model's device).  ``top_p`` or ``min_p`` draws by
+        ops.sample_tokens instead (top_k, then top_p, then min_p)."""
         if max_new_tokens <= 0:
             return idx
         bs = self.config.block_size
@@ -603,7 +697,7 @@ class mHCWalsh(nn.Module):
             seq = idx
             for _ in range(max_new_tokens):
                 logits, _ = self(seq[:, -bs:])
-                seq = torch.cat((seq, self._sample(logits[:, -1, :], temperature, top_k, generator)), dim=1)
+                seq = torch.cat((seq, self._draw(logits[:, -1, :], temperature, top_k, generator, top_p, min_p)), dim=1)
             return seq
         ctx = idx[:, -bs:]
         B, T = ctx.shape
@@ -612,13 +706,13 @@ class mHCWalsh(nn.Module):
                         batch_size=B)
         logits, _ = self(ctx, kv_cache=cache, start_pos=0)
         cache.increment(T)
-        nxt = self._sample(logits[:, -1, :], temperature, top_k, generator)
+        nxt = self._draw(logits[:, -1, :], temperature, top_k, generator, top_p, min_p)
         out = [idx, nxt]
         for _ in range(max_new_tokens - 1):
             if cache.cached_len >= bs:
                 break
             logits, _ = self(nxt, kv_cache=cache, start_pos=cache.cached_len)
             cache.increment(1)
-            nxt = self._sample(logits[:, -1, :], temperature, top_k, generator)
+            nxt = self._draw(logits[:, -1, :], temperature, top_k, generator, top_p, min_p)
             out.append(nxt)
         return torch.cat(out, dim=1)

@@ -730,7 +730,7 @@ def paged_append(q, k, v, k_pages, v_pages, slots, positions=None, rope=None, q_
     if n == 0:
         return q_out
     _call_on(dev, "walsh_paged_append", kv, qp, q_ts, q_hs, kp, k_ts, k_hs, vp, v_ts, v_hs, n, hq, slots.data_ptr(),
-             ptr(positions), slots.dtype == torch.int64, ptr(cos), ptr(sin), n_pos, ptr(q_norm), ptr(k_norm), eps,
+             ptr(positions), slots.dtype == torch.int64, ptr(cos), ptr(sin), n_pos, ptr(q_norm), ptr(k_norm), float(eps),
              ptr(q_out))
     return q_out
 
@@ -767,6 +767,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, wind
         return out
     if max_len is None:
         max_len = page_table.shape[1] * ps
+    max_len = int(max_len)
     nbytes = _attn_scratch_bytes(dcode(q.dtype), hk, hd, window, sinks, B, hq, max_len)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
     _call_on(dev, "walsh_paged_attn_fwd", kv, qp, q_bs, q_hs, B, hq, max_len, ptr(scratch), out.data_ptr())
@@ -791,7 +792,7 @@ def paged_prefill_attention(q, q_offsets, k_pages, v_pages, page_table, kv_lens,
     if n == 0 or B == 0:
         return out
     _call_on(dev, "walsh_paged_prefill_fwd", kv, qp, q_ts, q_hs, n, q_offsets.data_ptr(), B, hq,
-             n if max_q is None else min(max_q, n), out.data_ptr())
+             n if max_q is None else min(int(max_q), n), out.data_ptr())
     return out
 
 
@@ -833,6 +834,7 @@ def sample_tokens(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0
     ids = torch.empty(rows, dtype=torch.int64, device=logits.device)
     logp = torch.empty_like(uniforms) if want_logprob else None
     _call_on(dev, "walsh_sample_tokens", logits.data_ptr(), dcode(logits.dtype), logits.stride(0) if rows > 1 else 0,
-             rows, vocab, uniforms.data_ptr(), tv, max(0, min(kv, vocab)), pv, mv, ptr(tr), ptr(kr), ptr(pr), ptr(mr),
+             rows, vocab, uniforms.data_ptr(), float(tv), max(0, min(int(kv), vocab)), float(pv), float(mv), ptr(tr),
+             ptr(kr), ptr(pr), ptr(mr),
              ids.data_ptr(), ptr(logp))
     return (ids, logp) if want_logprob else ids
