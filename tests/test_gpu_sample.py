@@ -120,6 +120,13 @@ def test_many_tokens_at_a_top_p_border(kw):
     check(logits * 1e-4, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [700, 1023, 1025, 1500, 2049, 3333, 4097, 9000])
+@pytest.mark.parametrize("top_k", [33, 300, 512, 513])
+def test_top_k_of_rows_of_all_sizes(dtype, vocab, top_k):
+    check(*rand(3, vocab, vocab + top_k, dtype), top_k=top_k, top_p=0.97)
+
+
 @pytest.mark.parametrize("rows,vocab", [(150, 3000), (150, 40000), (40, 20000)])
 def test_parts_held_or_read_again(rows, vocab):
     """One CTA per row or several, with and without room to hold the row."""

@@ -8,11 +8,19 @@
 //   min-p:  w_i >= min_p
 //   draw:   the first token in index order whose running mass exceeds u Z
 //
-// A token at a border is kept or dropped whole, so the weights and their sums
-// are held to about 2^-45 of the largest weight: exp in double, rounded to a
-// 64-bit integer multiple of 2^-44.  Integer sums do not depend on the order
-// they are taken in, so neither do the draws.  The vocabulary is limited to
-// 2^18 tokens, which keeps every sum below 2^63.
+// A token at a border is kept or dropped whole, so what decides is held to about
+// 2^-45 of the largest weight: exp in double, rounded to a 64-bit integer
+// multiple of 2^-44 (sums of integers do not depend on the order they are taken
+// in, so neither do the draws).  Float32 sums are used only together with a bound
+// of their error, and replaced by exact ones where that bound could change the
+// answer.  The vocabulary is limited to 2^18 tokens, which keeps every sum below
+// 2^63.
+//
+// Bytes are the floor (256 rows of 50257 float32 logits: 7.9 us), instructions
+// the bound: about 140 thousand warp instructions per row with top-p (one pass
+// for the largest logit, one for the total and a histogram, one for the masses
+// above the border) run at 60 % of the issue slots, 73 us; 1 row with top-k 50
+// takes 12.5 us, the barriers and dependent steps of a row.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -100,6 +108,7 @@ struct SampleShared {
     } k;
     struct {
       float queue[kSampleWarps][64];
+      uint16_t queue_tok[kSampleWarps][64];  // from the warp's first element
       u64 cand[kCands];  // this CTA's tokens at the border
       union {
         uint32_t hist[kBins];
@@ -137,6 +146,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   __shared__ SampleShared sh;
   T* seg = reinterpret_cast<T*>(dyn);
   bool inf_row = false;  // the largest logit is +inf
+  bool nans = true;      // the part may hold NaN (in memory)
   const cg::cluster_group cl = cg::this_cluster();
   const int rank = CS == 1 ? 0 : (int)cl.block_rank();
   const int row = blockIdx.x / CS, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, V = a.vocab;
@@ -167,11 +177,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   const int wbeg = min(nch, warp * per_warp), wend = min(nch, wbeg + per_warp);
   const int base = c0 * VEC - mis;  // token of the part's first element (negative: before the row)
   float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
-  // 16 bytes of the row from its memory: outside the row and for NaN -inf
+  bool any_nan = false;
+  // 16 bytes of the row from its memory, -inf outside the row
+  const int in0 = base < 0 ? 1 : 0, in1 = base + nch * VEC > V ? nch - 1 : nch;  // chunks wholly inside
   auto fetch = [&](int ch) -> uint4 {
     const int t0 = base + ch * VEC;
     uint4 raw;
-    if (t0 >= 0 && t0 + VEC <= V) {
+    if (ch >= in0 && ch < in1) {
       raw = STAGE ? __ldcs(reinterpret_cast<const uint4*>(lg + t0)) : __ldg(reinterpret_cast<const uint4*>(lg + t0));
     } else {
       T* e = reinterpret_cast<T*>(&raw);
@@ -180,7 +192,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
     return raw;
   };
-  auto clean = [&](uint4 raw) -> uint4 {
+  auto clean = [&](uint4 raw) -> uint4 {  // NaN count as -inf
     T* e = reinterpret_cast<T*>(&raw);
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
@@ -207,11 +219,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       for (int i = 0; i < U; ++i) {
         const int ch = ch0 + 32 * i;
         if (ch >= wend) continue;
-        raw[i] = clean(raw[i]);
+        if constexpr (STAGE) raw[i] = clean(raw[i]);
         const T* e = reinterpret_cast<const T*>(&raw[i]);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
           const float v = to_f(e[j]);
+          if constexpr (!STAGE) any_nan |= v != v;
           if (j < VEC / 2) mx0 = fmaxf(mx0, v);
           else mx1 = fmaxf(mx1, v);
         }
@@ -219,13 +232,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       }
     }
   }
-  // 16 bytes of the part; past a warp's chunks (and around the row) -inf
+  // 16 bytes of the part (past a warp's chunks and around the row -inf)
   auto chunk = [&](int ch, int end) -> uint4 {
     const uint32_t w = neg_inf_word<T>();
     uint4 raw = make_uint4(w, w, w, w);
     if (ch < end) {
       if constexpr (STAGE) raw = *reinterpret_cast<const uint4*>(seg + (int64_t)ch * VEC);
-      else raw = clean(fetch(ch));
+      else raw = nans ? clean(fetch(ch)) : fetch(ch);
     }
     if (inf_row) {  // the +inf logits share the weight, nothing else has any
       T* e = reinterpret_cast<T*>(&raw);
@@ -312,7 +325,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     if (lane == 0) sh.scratch[warp] = wm;
     if (tid == 0) sh.n = 0, sh.uncertain = 0, sh.key_lo = ~0u, sh.key_hi = 0u;
     if (tid < 8) sh.add[tid] = 0;
-    __syncthreads();
+    if constexpr (STAGE) __syncthreads();
+    else nans = __syncthreads_or(any_nan);
     const uint32_t cm = __reduce_max_sync(0xffffffffu, (uint32_t)sh.scratch[lane % NW]);
     if (tid == 0) sh.cta_max = cm;
     if (by_mass) {  // the sum of the threads' largest weights, relative to this part's largest
@@ -429,11 +443,17 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         }
         uint32_t lo = 0, hi = kmax;  // count(>= lo) >= k; wanted: not many more
         const unsigned enough = (unsigned)top_k + max(16, top_k / 4);
+        // a small row has too few half chunks: its logits themselves are counted
+        const bool few = CS == 1 && V < top_k * VEC;
         while (lo < hi) {
           const uint32_t mid = lo + (hi - lo + 1) / 2;
           unsigned n = 0;
+          if (few) {
+            each([&](float v, int, bool in) { n += in && float_key(v + 0.f) >= mid; });
+          } else {
 #pragma unroll
-          for (int i = 0; i < 2 * CS; ++i) n += keys[i] >= mid;
+            for (int i = 0; i < 2 * CS; ++i) n += keys[i] >= mid;
+          }
           n = block_sum32(n);
           if (n >= (unsigned)top_k) {
             lo = mid;
@@ -661,7 +681,25 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   };
   auto draw_exact = [&](u64 thr) {
     u64 acc = 0;
-    packed([&](float v, int t) { return composite(v, t) >= thr; }, [&](float v) { acc += exact_of(v); });
+    if (thr == 0 && min_p <= 0.0) {  // every token: no packing, independent exponentials
+      uint4 next = chunk(wbeg + lane, wend);
+      for (int ch = wbeg + lane; ch < wend; ch += 32) {
+        const uint4 raw = next;
+        next = chunk(ch + 32, wend);
+        const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll 1
+        for (int h = 0; h < VEC; h += 4)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = VEC == 4 || h == 0 ? to_f(e[j]) : to_f(e[VEC - 4 + j]);
+            const double x = fmin(((double)m - (double)v) * c, 60.0);
+            const u64 f = fixed(exp2_neg(x));
+            acc += v == m ? (u64)kWeightOne : x < 60.0 ? f : 0;
+          }
+      }
+    } else {
+      packed([&](float v, int t) { return composite(v, t) >= thr; }, [&](float v) { acc += exact_of(v); });
+    }
     acc = warp_sum64(acc);
     if (lane == 0) sh.w_keep[warp] = acc;
     __syncthreads();
@@ -677,13 +715,16 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     draw(keep_of, [&](float v, int t) { return composite(v, t) >= thr; }, exact_of, 0);
   };
 
-  // A weight 2^-x in float32 (ex2.approx, at most 2 ulp) errs relatively by at
-  // most err_1 + x err_x: x = (m - l) c carries up to 4 roundings, each moving the
-  // weight by x 2^-24 ln 2, the exponential 2^-22, and sums of VEC weights VEC
-  // roundings.  Of a sum S of weights the error is then at most S (err_1 + 32
-  // err_x) and that of the weights beyond x = 32, V 32 2^-32 err_x.
-  const double err_x = 4 * 0.7 * 0x1p-24, err_1 = (4 + VEC) * 0x1p-24;
-  auto sum_error = [&](double s) { return s * (err_1 + 32 * err_x) + V * 0x1p-27 * err_x; };
+  // A weight 2^-x in float32 (ex2.approx, at most 2^-22 off) errs relatively by at
+  // most err_1 + x err_x: the difference m - l and the product with c are rounded
+  // once each and c itself is off by a known factor, each moving the weight by x
+  // ln 2 times its relative error; sums of VEC weights add VEC roundings.  Of a
+  // sum S of weights the error is then at most S (err_1 + x0 err_x) and, as t 2^-t
+  // is below 0.54, that of the weights beyond x0 V 2^-x0 0.54 err_x more.
+  const double err_x = 0.6932 * (0x1p-23 + fabs((double)cf / c - 1.0)), err_1 = (4 + VEC) * 0x1p-24;
+  auto sum_error = [&](double s, float x0) {
+    return s * (err_1 + x0 * err_x) + 0.54 * V * (double)ex2_f32(-x0) * err_x;
+  };
   if (!general && !by_mass) {
     // ---------------------------------------------------------------------
     // no top-k, no top-p: draw from the float32 masses when the drawn mass is
@@ -731,7 +772,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
     // both the running mass and u Z~ move with the error, and each token's and
     // warp's mass is rounded to the fixed point
-    const u64 slack = (u64)(2.0 * sum_error((double)z / kWeightOne) * kWeightOne) + (u64)V + 64;
+    const u64 slack = (u64)(2.0 * sum_error((double)z / kWeightOne, 32.f) * kWeightOne) + (u64)V + 64;
     if (sure)
       sure = draw(keep_of, [&](float v, int) { return (m - v) * cf <= x_min; },
                   [&](float v) { return fixed((double)ex2_f32((v - m) * cf)); }, slack);
@@ -833,17 +874,36 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     u64 keep_of[CS];
     u64 acc_keep, acc_all;
     double tail;
-    // the pass over the part: masses above the bins (exact), the bins' tokens, and the tail in float32
+    // the pass over the part: the tail in float32; what is above it goes through the
+    // warp's queue, 32 at a time, to the exact masses or the bins' tokens
     auto tally = [&]() {
       acc_keep = acc_all = 0;
       tail = 0.0;
       int fill = 0;
       float* q = sh.p.queue[warp];
-      auto take_one = [&](float v) {
-        const double w = weight(v, m, c);
-        const u64 f = fixed(w);
-        acc_all += f;
-        if (w >= min_p) acc_keep += f;
+      uint16_t* qt = sh.p.queue_tok[warp];
+      auto take = [&](float v, int t, bool is) {
+        const bool border = is && bin_at(v) >= edge_lo;
+        if (is && !border) {
+          const double w = weight(v, m, c);
+          const u64 f = fixed(w);
+          acc_all += f;
+          if (w >= min_p) acc_keep += f;
+        }
+        const unsigned bb = __ballot_sync(0xffffffffu, border);
+        if (bb) {
+          const uint32_t key = float_key(v + 0.f);
+          const uint32_t lo = __reduce_min_sync(0xffffffffu, border ? key : ~0u);
+          const uint32_t hi = __reduce_max_sync(0xffffffffu, border ? key : 0u);
+          unsigned at = 0;
+          if (lane == 0) {
+            at = atomicAdd(&sh.n, __popc(bb));
+            atomicMin(&sh.key_lo, lo);
+            atomicMax(&sh.key_hi, hi);
+          }
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(bb & ((1u << lane) - 1));
+          if (border && at < kCands) sh.p.cand[at] = composite(v, base + wbeg * VEC + t);
+        }
       };
       uint4 next = chunk(wbeg + lane, wend);
       for (int ch0 = wbeg; ch0 < wend; ch0 += 32) {
@@ -852,62 +912,82 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         next = chunk(ch + 32, wend);
         const T* e = reinterpret_cast<const T*>(&raw);
         float s = 0.f;
+        unsigned up = 0;  // elements above the tail
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float v = to_f(e[j]), b = bin_at(v), w = ex2_f32((v - m) * cf);
-          const bool in_tail = b >= edge_hi, take = b < edge_lo;
+          const float v = to_f(e[j]), w = ex2_f32((v - m) * cf);
+          const bool in_tail = bin_at(v) >= edge_hi;
           s += in_tail ? w : 0.f;
-          const bool border = !in_tail && !take;
-          const unsigned bb = __ballot_sync(0xffffffffu, border);
-          if (bb) {
-            const uint32_t key = float_key(v + 0.f);
-            const uint32_t lo = __reduce_min_sync(0xffffffffu, border ? key : ~0u);
-            const uint32_t hi = __reduce_max_sync(0xffffffffu, border ? key : 0u);
-            unsigned at = 0;
-            if (lane == 0) {
-              at = atomicAdd(&sh.n, __popc(bb));
-              atomicMin(&sh.key_lo, lo);
-              atomicMax(&sh.key_hi, hi);
-            }
-            at = __shfl_sync(0xffffffffu, at, 0) + __popc(bb & ((1u << lane) - 1));
-            if (border && at < kCands) sh.p.cand[at] = composite(v, base + ch * VEC + j);
+          up |= in_tail ? 0u : 1u << j;
+        }
+        tail += (double)s;
+        // one element per lane and turn
+        for (unsigned bal = __ballot_sync(0xffffffffu, up != 0); bal; bal = __ballot_sync(0xffffffffu, up != 0)) {
+          if (up) {
+            const int j = __ffs(up) - 1;
+            float v = to_f(e[0]);
+#pragma unroll
+            for (int i = 1; i < VEC; ++i)
+              if (i == j) v = to_f(e[i]);
+            const int at = fill + __popc(bal & ((1u << lane) - 1));
+            q[at] = v;
+            qt[at] = (uint16_t)((ch - wbeg) * VEC + j);
+            up &= up - 1;
           }
-          const unsigned bal = __ballot_sync(0xffffffffu, take);
-          if (take) q[fill + __popc(bal & ((1u << lane) - 1))] = v;
           fill += __popc(bal);
           if (fill >= 32) {
             __syncwarp();
-            const float y0 = q[lane], y1 = q[32 + lane];
+            const float v0 = q[lane], v1 = q[32 + lane];
+            const uint16_t t0 = qt[lane], t1 = qt[32 + lane];
             __syncwarp();
-            q[lane] = y1;
+            q[lane] = v1;
+            qt[lane] = t1;
             fill -= 32;
-            take_one(y0);
+            take(v0, t0, true);
           }
         }
-        tail += (double)s;
       }
       __syncwarp();
-      if (lane < fill) take_one(q[lane]);
+      take(q[lane], qt[lane], lane < fill);
       __syncwarp();
     };
-    // the tail once more, exactly: four independent exponentials at a time
-    auto exact_tail_sum = [&]() -> u64 {
-      u64 acc = 0;
+    // the tail once more with an error below 2^-31 of it: independent Taylor series
+    // of degree 8 in double (the first dropped term is (ln 2 / 2)^9 / 9! = 2e-10)
+    auto exact_tail_sum = [&]() -> double {
+      const double mc = (double)m * c;
+      double acc = 0.0;
       uint4 next = chunk(wbeg + lane, wend);
       for (int ch = wbeg + lane; ch < wend; ch += 32) {
         const uint4 raw = next;
         next = chunk(ch + 32, wend);
         const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll 1
+        for (int h = 0; h < VEC; h += 4) {
+        double s[4];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          const float v = to_f(e[j]);
-          // (a tail token is below the largest; beyond x = 60 its mass is 0)
-          const double x = fmin(((double)m - (double)v) * c, 60.0);
-          const u64 f = __double2ull_rn(exp2_neg(x) * kWeightOne);
-          acc += bin_at(v) >= edge_hi && x < 60.0 ? f : 0;
+        for (int j = 0; j < 4; ++j) {
+          const float v = VEC == 4 || h == 0 ? to_f(e[j]) : to_f(e[VEC - 4 + j]);
+          const double x = fma((double)v, -c, mc);
+          const bool is = bin_at(v) >= edge_hi && x < 60.0;  // beyond it a mass is nothing
+          const double t = (is ? x : 0.0) + 6755399441055744.0;  // 1.5 * 2^52: x to the nearest integer
+          const int n = __double2loint(t);
+          const double g = (t - 6755399441055744.0) - (is ? x : 0.0);
+          // 2^g, |g| <= 1/2, coefficients (ln 2)^k / k!
+          double p = 1.3215486790144307e-06;
+          p = fma(p, g, 1.5252733804059841e-05);
+          p = fma(p, g, 1.5403530393381608e-04);
+          p = fma(p, g, 1.3333558146428443e-03);
+          p = fma(p, g, 9.6181291076284772e-03);
+          p = fma(p, g, 5.5504108664821580e-02);
+          p = fma(p, g, 2.4022650695910072e-01);
+          p = fma(p, g, 6.9314718055994531e-01);
+          p = fma(p, g, 1.0);
+          s[j] = is ? __hiloint2double(__double2hiint(p) - (n << 20), __double2loint(p)) : 0.0;
+        }
+        acc += (s[0] + s[1]) + (s[2] + s[3]);
         }
       }
-      return acc;
+      return warp_sumd(acc);
     };
     tally();
     acc_keep = warp_sum64(acc_keep);
@@ -943,16 +1023,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       if (tid >= n && tid < n + k && k <= kCands) own = q->p.cand[tid - n], src = r;
       n += k;
     }
-    double te = sum_error(tl);
+    double te = sum_error(tl, x_end);
     // the tail exactly, on demand: the same answer in every CTA
     auto refine_tail = [&]() {
-      const u64 t = block_sum(exact_tail_sum());
-      if (tid == 0) sh.cta_ties = t;
+      const double mine = exact_tail_sum();
+      all_sync();  // (every CTA has read the sums)
+      if (lane == 0) sh.w_sum[warp] = mine;
+      __syncthreads();
+      if (tid == 0) {
+        double s = 0.0;
+        for (int w = 0; w < NW; ++w) s += sh.w_sum[w];
+        sh.cta_sum = s;
+      }
       all_sync();
-      u64 all = 0;
+      tl = 0.0;
 #pragma unroll
-      for (int r = 0; r < CS; ++r) all += peer(r)->cta_ties;
-      tl = (double)all / kWeightOne;
+      for (int r = 0; r < CS; ++r) tl += peer(r)->cta_sum;
       te = 0.0;
     };
     // bounds of the mass that has to come before a token for it to be dropped, `in` being the bins' own mass
@@ -1214,9 +1300,9 @@ static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
 
 // CTAs per row: one when the rows alone occupy every SM (the barriers and scalar
 // steps of a row are paid per CTA), else more while a thread still has eight
-// tokens.  50257 tokens in float32: 64 rows with top-p 28.8 us on 4 CTAs each,
-// 53.5 on 8; 256 rows 83.3 us on one (read again from L2), 76.6 on two; with
-// top-k 50 33.8 and 42.8 us; 128 rows with top-k 500 45.1 on 2, 73.3 on 4.
+// tokens.  Rows of 50257 tokens: 64 in float32 with top-p 26.5 us on 4 CTAs each
+// (53 on 8); 256 in float32 72.8 us on one, read again from L2, 70.7 on two,
+// held; with top-k 50 31.9 and 43.2 us; 256 in bf16 56.4 us on one, held.
 static int sample_cluster(int64_t rows, int vocab) {
   int cs = 1;
   while (cs < 8 && rows * cs < 148 && vocab / cs > kSampleThreads * 8) cs *= 2;
