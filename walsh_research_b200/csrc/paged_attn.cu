@@ -10,15 +10,21 @@
 // The visible keys of a (sequence, key/value head) are numbered 0..n-1 and
 // cut into nsplit ranges of `chunk`; a CTA of W warps takes one range, each
 // warp a slice of it with its own running maximum, sum and accumulator
-// (float32), joined through shared memory.  With more than one non-empty
-// range the CTA leaves (m, l, o) in the workspace and paged_join_kernel
-// combines them in order of the ranges, so results do not depend on timing.
+// (float32), joined through shared memory.  A few ranges are joined by a cluster
+// of their CTAs; more leave (m, l, o) in the workspace for paged_join_kernel.
+// Both combine them in order of the ranges, so results do not depend on timing.
+// Measured (of the HBM copy rate): 256 sequences of up to 1024 keys, 32 heads of
+// 16 channels, 49.6 us (0.84); 12 of up to 32768, 8 shared heads of 64, 82 us
+// (0.90); 48 under a window of 1000, 64 heads of 32, 59.8 us (0.93).
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include "mma.cuh"
 #include "paged.cuh"
 
 namespace walsh {
+
+namespace cg = cooperative_groups;
 
 template <typename T>
 struct DecodeArgs {
@@ -40,14 +46,38 @@ __device__ __forceinline__ void split_range(int n, int chunk, int nsplit, int c,
   *end = c == nsplit - 1 ? n : (int)min((int64_t)n, (int64_t)(c + 1) * chunk);
 }
 
+// The ranges of one unit joined through distributed shared memory: the CTAs of a
+// cluster hold their range's (m, l, o) in cj [rows][HD + 2] and each combines a
+// share of the outputs, in order of the ranges.
+template <typename T, int HD>
+__device__ __forceinline__ void cluster_join(const DecodeArgs<T>& a, float* cj, int c, int ng, int64_t row0) {
+  const cg::cluster_group cl = cg::this_cluster();
+  cl.sync();
+  for (int i = c * blockDim.x + threadIdx.x; i < ng * HD; i += a.nsplit * blockDim.x) {
+    const int r = i / HD, d = i - r * HD;
+    float M = -CUDART_INF_F, L = 0.f, O = 0.f;
+    for (int s = 0; s < a.nsplit; ++s) M = fmaxf(M, cl.map_shared_rank(cj, s)[r * (HD + 2) + HD]);
+    const float sub = M == -CUDART_INF_F ? 0.f : M;
+    for (int s = 0; s < a.nsplit; ++s) {
+      const float* q = cl.map_shared_rank(cj, s) + r * (HD + 2);
+      const float f = ex2_f32(q[HD] - sub);
+      L = fmaf(q[HD + 1], f, L);
+      O = fmaf(q[d], f, O);
+    }
+    a.o[(row0 + r) * HD + d] = round_f<T>(L == 0.f ? 0.f : O / L);
+  }
+  cl.sync();  // no CTA leaves while its memory is read
+}
+
 // ---------------------------------------------------------------------------
 // CUDA-core form for float32.  LPK lanes share one key, 16 bytes of it each; a
 // warp step covers 32 / LPK keys and KPT steps are in flight.
 // ---------------------------------------------------------------------------
-template <typename T, int HD, int GH, int W>
+template <typename T, int HD, int GH, int W, bool CL>
 __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeArgs<T> a) {
   constexpr int VEC = 16 / (int)sizeof(T), LPK = HD / VEC, KS = 32 / LPK, KPT = 4;
   __shared__ float red[W][GH][LPK][VEC + 2];
+  __shared__ float cj[CL ? GH * (HD + 2) : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LPK, slot = lane / LPK;
   int unit = blockIdx.x;
   const int c = unit % a.nsplit;
@@ -59,7 +89,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
   const Visible vis = visible_keys(len - 1, a.pg.window, a.pg.sinks);
   int beg, end;
   split_range(vis.n, a.chunk, a.nsplit, c, &beg, &end);
-  if (beg >= end && c > 0) return;
+  if (!CL && beg >= end && c > 0) return;
   const int gh0 = gt * GH, ng = min(GH, a.group - gh0);
   const int h0 = hk * a.group + gh0;
   const int per = ((end - beg + W - 1) / W + KS - 1) / KS * KS;
@@ -152,6 +182,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
   }
   __syncthreads();
   const int64_t Hq = (int64_t)a.kv_heads * a.group;
+  const int64_t row0 = (int64_t)b * Hq + h0;
   const bool whole = vis.n <= a.chunk || a.nsplit == 1;  // this range is all there is
   for (int i = threadIdx.x; i < ng * HD; i += W * 32) {
     const int g = i / HD, d = i - g * HD, p = d / VEC, j = d - p * VEC;
@@ -167,7 +198,13 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
       O = fmaf(red[w][g][p][2 + j], f, O);
     }
     const int64_t row = (int64_t)b * Hq + h0 + g;
-    if (whole) {
+    if constexpr (CL) {
+      cj[(row - row0) * (HD + 2) + d] = O;
+      if (d == 0) {
+        cj[(row - row0) * (HD + 2) + HD] = M;
+        cj[(row - row0) * (HD + 2) + HD + 1] = L;
+      }
+    } else if (whole) {
       a.o[row * HD + d] = round_f<T>(L == 0.f ? 0.f : O / L);  // no visible key: zeros
     } else {
       a.part_o[(row * a.nsplit + c) * HD + d] = O;
@@ -177,6 +214,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
       }
     }
   }
+  if constexpr (CL) cluster_join<T, HD>(a, cj, c, ng, row0);
 }
 
 // ---------------------------------------------------------------------------
@@ -200,7 +238,7 @@ template <> __device__ __forceinline__ uint32_t dec_pack<__half>(float lo, float
 template <> __device__ __forceinline__ uint32_t dec_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
 
 // RH: halves of the 16 MMA rows in use (1: up to 8 heads, 2: up to 16)
-template <typename T, int HD, int RH, int W, int KT, int NS>
+template <typename T, int HD, int RH, int W, int KT, int NS, bool CL>
 __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeArgs<T> a) {
   constexpr int CH = HD / 8, STAGE = 2 * KT * HD, RI = 32 / CH;  // RI: rows per copy instruction
   constexpr int OL = HD + 4;                                     // padded row of the join buffer
@@ -216,7 +254,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
   const Visible vis = visible_keys(len - 1, a.pg.window, a.pg.sinks);
   int beg, end;
   split_range(vis.n, a.chunk, a.nsplit, c, &beg, &end);
-  if (beg >= end && c > 0) return;
+  if (!CL && beg >= end && c > 0) return;
   const int ng = min(8 * RH, a.group - gt * 8 * RH), h0 = hk * a.group + gt * 8 * RH;
   const int per = ((end - beg + W - 1) / W + 15) / 16 * 16;
   const int wbeg = min(end, beg + warp * per), n = min(end, wbeg + per) - wbeg;  // this warp's keys
@@ -381,6 +419,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
   // join the warps: rows of the ring are free
   float* jo = reinterpret_cast<float*>(smb);             // [W][8 RH][OL]
   float* jm = jo + W * 8 * RH * OL;                      // [W][8 RH][2]
+  float* cj = jm + W * 8 * RH * 2;                       // [8 RH][HD + 2], cluster join
   if constexpr (W > 1) __syncthreads();
 #pragma unroll
   for (int h = 0; h < RH; ++h) {
@@ -399,6 +438,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
   if constexpr (W > 1) __syncthreads();
   else __syncwarp();
   const int64_t Hq = (int64_t)a.kv_heads * a.group;
+  const int64_t row0 = (int64_t)b * Hq + h0;
   const bool whole = vis.n <= a.chunk || a.nsplit == 1;  // this range is all there is
   for (int i = threadIdx.x; i < ng * HD; i += W * 32) {
     const int r = i / HD, d = i - r * HD;
@@ -414,7 +454,13 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
       O = fmaf(jo[(w * 8 * RH + r) * OL + d], f, O);
     }
     const int64_t row = (int64_t)b * Hq + h0 + r;
-    if (whole) {
+    if constexpr (CL) {
+      cj[(row - row0) * (HD + 2) + d] = O;
+      if (d == 0) {
+        cj[(row - row0) * (HD + 2) + HD] = M;
+        cj[(row - row0) * (HD + 2) + HD + 1] = L;
+      }
+    } else if (whole) {
       a.o[row * HD + d] = round_f<T>(L == 0.f ? 0.f : O / L);  // no visible key: zeros
     } else {
       a.part_o[(row * a.nsplit + c) * HD + d] = O;
@@ -424,15 +470,17 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
       }
     }
   }
+  if constexpr (CL) cluster_join<T, HD>(a, cj, c, ng, row0);
 }
 
-// Joins the ranges of each (sequence, head): one warp per row.
+// Joins the ranges of each (sequence, head): one CTA per row, its warps take
+// every fourth group of ranges with four loads in flight.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs<T> a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t Hq = (int64_t)a.kv_heads * a.group;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= a.B * Hq) return;
+  constexpr int DP = HD < 32 ? HD : 32, DN = HD / DP, SL = 32 / DP;  // channels and ranges per step of a warp
+  __shared__ float red[4][HD + 2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x, Hq = (int64_t)a.kv_heads * a.group;
   const Visible vis = visible_keys(seq_len(a.pg, (int)(row / Hq)) - 1, a.pg.window, a.pg.sinks);
   if (vis.n <= a.chunk) return;  // written whole
   const int nc = (int)min((int64_t)a.nsplit, ((int64_t)vis.n + a.chunk - 1) / a.chunk);
@@ -442,28 +490,59 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const DecodeArgs<T> a) 
   for (int i = lane; i < nc; i += 32) M = fmaxf(M, ml[2 * i]);
   M = warp_max(M);
   const float sub_m = M == -CUDART_INF_F ? 0.f : M;
-  constexpr int DP = HD < 32 ? HD : 32;  // channels per step
-  constexpr int SL = 32 / DP;            // ranges per step
   const int d0 = lane % DP, s0 = lane / DP;
-  float L = 0.f, O[HD / DP] = {};
-  for (int i = s0; i < nc; i += SL) {
+  float L = 0.f, O[DN] = {};
+#pragma unroll 4
+  for (int i = warp * SL + s0; i < nc; i += 4 * SL) {
     const float f = ex2_f32(ml[2 * i] - sub_m);
     L = fmaf(ml[2 * i + 1], f, L);
 #pragma unroll
-    for (int k = 0; k < HD / DP; ++k) O[k] = fmaf(po[(int64_t)i * HD + k * DP + d0], f, O[k]);
+    for (int k = 0; k < DN; ++k) O[k] = fmaf(po[(int64_t)i * HD + k * DP + d0], f, O[k]);
   }
 #pragma unroll
   for (int o = DP; o < 32; o <<= 1) {
     L += __shfl_xor_sync(0xffffffffu, L, o);
 #pragma unroll
-    for (int k = 0; k < HD / DP; ++k) O[k] += __shfl_xor_sync(0xffffffffu, O[k], o);
+    for (int k = 0; k < DN; ++k) O[k] += __shfl_xor_sync(0xffffffffu, O[k], o);
   }
-  if (lane < DP)
+  if (lane < DP) {
 #pragma unroll
-    for (int k = 0; k < HD / DP; ++k) a.o[row * HD + k * DP + d0] = round_f<T>(L == 0.f ? 0.f : O[k] / L);
+    for (int k = 0; k < DN; ++k) red[warp][k * DP + d0] = O[k];
+    if (lane == 0) red[warp][HD] = L;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < HD; d += 128) {
+    const float l = red[0][HD] + red[1][HD] + red[2][HD] + red[3][HD];
+    const float o = red[0][d] + red[1][d] + red[2][d] + red[3][d];
+    a.o[row * HD + d] = round_f<T>(l == 0.f ? 0.f : o / l);
+  }
 }
 
-template <typename T, int HD, int RH, int W>
+// Launches CTAs, in clusters of `cluster` when that is more than one.
+template <typename K, typename A>
+static int launch_ctas(K* kern, const A& a, int64_t ctas, int threads, int smem, int cluster, cudaStream_t s) {
+  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+    return launch_status();
+  if (cluster <= 1) {
+    kern<<<(unsigned)ctas, threads, smem, s>>>(a);
+    return launch_status();
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = cluster;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, a);
+  return launch_status();
+}
+
+template <typename T, int HD, int RH, int W, bool CL>
 static int launch_decode_mma(const DecodeArgs<T>& a, int64_t ctas, cudaStream_t s) {
   // 8 KB of K and V per stage (4 KB for 16 channels)
   constexpr int KT = HD <= 32 ? 64 : HD == 64 ? 32 : 16;
@@ -471,41 +550,44 @@ static int launch_decode_mma(const DecodeArgs<T>& a, int64_t ctas, cudaStream_t 
   // ring leaves room for more warps (256 x 1024 keys, 16 channels: 2 stages
   // 49.4 us, 3 50.7, 4 58.4; 12 x 32768, 64 channels: 82.3, 89.4, 94.8)
   constexpr int NS = 2;
-  constexpr int ring = W * NS * 2 * KT * HD * 2, join = W * 8 * RH * (HD + 4 + 2) * 4;
-  constexpr int smem = ring > join ? ring : join;
-  auto* kern = paged_decode_mma_kernel<T, HD, RH, W, KT, NS>;
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-    return launch_status();
-  kern<<<(unsigned)ctas, W * 32, smem, s>>>(a);
-  return launch_status();
+  constexpr int ring = W * NS * 2 * KT * HD * 2, join = (W * 8 * RH * (HD + 4 + 2) + (CL ? 8 * RH * (HD + 2) : 0)) * 4;
+  return launch_ctas(paged_decode_mma_kernel<T, HD, RH, W, KT, NS, CL>, a, ctas, W * 32, ring > join ? ring : join,
+                     CL ? a.nsplit : 1, s);
 }
 
-template <typename T, int HD, int W>
+template <typename T, int HD, int W, bool CL>
 static int launch_decode(const DecodeArgs<T>& a, cudaStream_t s) {
   const int64_t ctas = (int64_t)a.B * a.kv_heads * a.gtiles * a.nsplit;
   int r;
   if constexpr (sizeof(T) == 2) {
-    r = a.group <= 8 ? launch_decode_mma<T, HD, 1, W>(a, ctas, s) : launch_decode_mma<T, HD, 2, W>(a, ctas, s);
+    r = a.group <= 8 ? launch_decode_mma<T, HD, 1, W, CL>(a, ctas, s) : launch_decode_mma<T, HD, 2, W, CL>(a, ctas, s);
   } else {
-    if (a.group == 1) paged_decode_vec_kernel<T, HD, 1, W><<<(unsigned)ctas, W * 32, 0, s>>>(a);
-    else paged_decode_vec_kernel<T, HD, 4, W><<<(unsigned)ctas, W * 32, 0, s>>>(a);
-    r = launch_status();
+    const int cl = CL ? a.nsplit : 1;
+    r = a.group == 1 ? launch_ctas(paged_decode_vec_kernel<T, HD, 1, W, CL>, a, ctas, W * 32, 0, cl, s)
+                     : launch_ctas(paged_decode_vec_kernel<T, HD, 4, W, CL>, a, ctas, W * 32, 0, cl, s);
   }
-  if (r) return r;
+  if (r || CL) return r;
   if (a.nsplit > 1) {
     const int64_t rows = (int64_t)a.B * a.kv_heads * a.group;
-    paged_join_kernel<T, HD><<<(unsigned)((rows + 3) / 4), 128, 0, s>>>(a);
+    paged_join_kernel<T, HD><<<(unsigned)rows, 128, 0, s>>>(a);
     return launch_status();
   }
   return WALSH_OK;
 }
 
-// How a call is cut: `warps` per CTA, `nsplit` ranges of `chunk` visible keys.
+// How a call is cut: `warps` per CTA, `nsplit` ranges of `chunk` visible keys per
+// unit (sequence, key/value head, head tile), by the bytes of its longest.
 struct DecodePlan {
   int warps, gtiles, nsplit, chunk;
+  bool cluster;  // the ranges' CTAs join through distributed shared memory
 };
-constexpr int kDecodeWarps = 148 * 16;  // wanted in all
-constexpr int kDecodeMinKeys = 128;     // of one warp
+constexpr int64_t kRangeBytes = 256 << 10;  // longer ranges are cut for the balance between sequences
+constexpr int64_t kRangeLeast = 32 << 10;   // shorter ones cost more to join than they save
+// from so many units up to so many bytes each, a warp per unit: 256 x 1024 keys
+// (8192 units of 64 KB) 49.6 us against 58 with four, 100 x 200 keys 8.2 against
+// 14.3; but 64 x 4000 (2048 of 256 KB) 71 against 48, 30 x 500 (960) 9.0 against 7.7
+constexpr int kSingleUnits = 2000;
+constexpr int64_t kSingleBytes = 100000;
 static DecodePlan decode_plan(const walsh_paged_kv* kv, int B, int q_heads, int max_len) {
   const int group = q_heads / kv->kv_heads, tile = kv->dtype == WALSH_F32 ? 4 : group <= 8 ? 8 : 16;
   DecodePlan p;
@@ -513,18 +595,30 @@ static DecodePlan decode_plan(const walsh_paged_kv* kv, int B, int q_heads, int 
   const int64_t units = (int64_t)B * kv->kv_heads * p.gtiles;
   int64_t n = max_len;
   if (kv->window > 0) n = min64(n, (int64_t)kv->window + kv->sinks);
-  const int64_t want = (kDecodeWarps + units - 1) / units, most = n / kDecodeMinKeys;
-  const int64_t per_unit = most < 1 ? 1 : min64(most, want);
-  p.warps = per_unit >= 4 ? 4 : 1;
-  p.nsplit = (int)((per_unit + p.warps - 1) / p.warps);
+  const int64_t bytes = n * 2 * kv->head_dim * (kv->dtype == WALSH_F32 ? 4 : 2);  // of a unit
+  // one warp per unit when there are enough units for the GPU, or nothing to share
+  p.warps = (units >= kSingleUnits && bytes <= kSingleBytes) || bytes < (8 << 10) ? 1 : 4;
+  // CTAs of four warps that fit on the GPU together: no range waits for another
+  // (2 x 20000 keys of 64 channels, 3 per SM 20.3 us, 4 24.2; 16 x 8000 of 32, 3
+  // 14.2, 5 11.8; 4 x 4000 of 16, 3 10.3, 4 9.1, 5 (too many for clusters) 11.1)
+  const int ctas = 148 * (kv->head_dim == 16 ? 4 : kv->head_dim == 32 ? 5 : 3);
+  int64_t split = units > 0 ? ctas / units : 1;
+  if (split < bytes / kRangeBytes) split = bytes / kRangeBytes;
+  split = min64(split, bytes / kRangeLeast);
+  p.nsplit = p.warps == 1 || split < 1 ? 1 : (int)split;
   p.chunk = (int)((n + p.nsplit - 1) / p.nsplit);
   if (p.chunk < 1) p.chunk = 1;
+  // the clusters' one launch saves the joining kernel and its scratch (1 x 4099
+  // keys 7.8 -> 6.6 us) while all of them run at once; beyond that CTAs that wait
+  // for their cluster keep others out (12 x 32768 keys: 95 us against 84)
+  p.cluster = p.nsplit > 1 && p.nsplit <= 8 && units * p.nsplit <= 148 * 4;
   return p;
 }
 
 template <typename T, int HD>
-static int launch_decode_warps(const DecodeArgs<T>& a, int warps, cudaStream_t s) {
-  return warps == 1 ? launch_decode<T, HD, 1>(a, s) : launch_decode<T, HD, 4>(a, s);
+static int launch_decode_plan(const DecodeArgs<T>& a, const DecodePlan& p, cudaStream_t s) {
+  if (p.cluster) return launch_decode<T, HD, 4, true>(a, s);
+  return p.warps == 1 ? launch_decode<T, HD, 1, false>(a, s) : launch_decode<T, HD, 4, false>(a, s);
 }
 
 }  // namespace walsh
@@ -541,7 +635,7 @@ static int decode_check(const walsh_paged_kv* kv, int B, int q_heads, int max_le
 extern "C" int64_t walsh_paged_attn_scratch_bytes(const walsh_paged_kv* kv, int B, int q_heads, int max_len) {
   if (decode_check(kv, B, q_heads, max_len) != WALSH_OK) return -1;
   const DecodePlan p = decode_plan(kv, B, q_heads, max_len);
-  return p.nsplit > 1 ? (int64_t)B * q_heads * p.nsplit * (kv->head_dim + 2) * 4 : 0;
+  return p.nsplit > 1 && !p.cluster ? (int64_t)B * q_heads * p.nsplit * (kv->head_dim + 2) * 4 : 0;
 }
 
 extern "C" walsh_status walsh_paged_attn_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_bs, int64_t q_hs,
@@ -555,22 +649,22 @@ extern "C" walsh_status walsh_paged_attn_fwd(const walsh_paged_kv* kv, const voi
     return WALSH_ERR_ALIGN;
   if (B == 0) return WALSH_OK;
   const DecodePlan p = decode_plan(kv, B, q_heads, max_len);
-  WALSH_CHECK_ARG(p.nsplit == 1 || scratch);
+  WALSH_CHECK_ARG(p.nsplit == 1 || p.cluster || scratch);
   return WALSH_DISPATCH_DTYPE(kv->dtype, ET, [&]() -> int {
     DecodeArgs<ET> a;
     a.pg = make_pages<ET>(kv);
     a.q = (const ET*)q, a.q_bs = q_bs, a.q_hs = q_hs, a.o = (ET*)o;
     a.part_o = (float*)scratch;
-    a.part_ml = a.part_o + (int64_t)B * q_heads * p.nsplit * kv->head_dim;
+    a.part_ml = scratch ? a.part_o + (int64_t)B * q_heads * p.nsplit * kv->head_dim : nullptr;
     a.B = B, a.kv_heads = kv->kv_heads, a.group = q_heads / kv->kv_heads;
     a.gtiles = p.gtiles, a.nsplit = p.nsplit, a.chunk = p.chunk;
     a.scale_log2 = kv->scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
     switch (kv->head_dim) {
-      case 16: return launch_decode_warps<ET, 16>(a, p.warps, s);
-      case 32: return launch_decode_warps<ET, 32>(a, p.warps, s);
-      case 64: return launch_decode_warps<ET, 64>(a, p.warps, s);
-      default: return launch_decode_warps<ET, 128>(a, p.warps, s);
+      case 16: return launch_decode_plan<ET, 16>(a, p, s);
+      case 32: return launch_decode_plan<ET, 32>(a, p, s);
+      case 64: return launch_decode_plan<ET, 64>(a, p, s);
+      default: return launch_decode_plan<ET, 128>(a, p, s);
     }
   }());
 }
