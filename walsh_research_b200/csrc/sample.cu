@@ -963,28 +963,28 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll 1
         for (int h = 0; h < VEC; h += 4) {
-        double s[4];
+          double s[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float v = VEC == 4 || h == 0 ? to_f(e[j]) : to_f(e[VEC - 4 + j]);
-          const double x = fma((double)v, -c, mc);
-          const bool is = bin_at(v) >= edge_hi && x < 60.0;  // beyond it a mass is nothing
-          const double t = (is ? x : 0.0) + 6755399441055744.0;  // 1.5 * 2^52: x to the nearest integer
-          const int n = __double2loint(t);
-          const double g = (t - 6755399441055744.0) - (is ? x : 0.0);
-          // 2^g, |g| <= 1/2, coefficients (ln 2)^k / k!
-          double p = 1.3215486790144307e-06;
-          p = fma(p, g, 1.5252733804059841e-05);
-          p = fma(p, g, 1.5403530393381608e-04);
-          p = fma(p, g, 1.3333558146428443e-03);
-          p = fma(p, g, 9.6181291076284772e-03);
-          p = fma(p, g, 5.5504108664821580e-02);
-          p = fma(p, g, 2.4022650695910072e-01);
-          p = fma(p, g, 6.9314718055994531e-01);
-          p = fma(p, g, 1.0);
-          s[j] = is ? __hiloint2double(__double2hiint(p) - (n << 20), __double2loint(p)) : 0.0;
-        }
-        acc += (s[0] + s[1]) + (s[2] + s[3]);
+          for (int j = 0; j < 4; ++j) {
+            const float v = VEC == 4 || h == 0 ? to_f(e[j]) : to_f(e[VEC - 4 + j]);
+            const double x = fma((double)v, -c, mc);
+            const bool is = bin_at(v) >= edge_hi && x < 60.0;  // beyond it a mass is nothing
+            const double t = (is ? x : 0.0) + 6755399441055744.0;  // 1.5 * 2^52: x to the nearest integer
+            const int n = __double2loint(t);
+            const double g = (t - 6755399441055744.0) - (is ? x : 0.0);
+            // 2^g, |g| <= 1/2, coefficients (ln 2)^k / k!
+            double p = 1.3215486790144307e-06;
+            p = fma(p, g, 1.5252733804059841e-05);
+            p = fma(p, g, 1.5403530393381608e-04);
+            p = fma(p, g, 1.3333558146428443e-03);
+            p = fma(p, g, 9.6181291076284772e-03);
+            p = fma(p, g, 5.5504108664821580e-02);
+            p = fma(p, g, 2.4022650695910072e-01);
+            p = fma(p, g, 6.9314718055994531e-01);
+            p = fma(p, g, 1.0);
+            s[j] = is ? __hiloint2double(__double2hiint(p) - (n << 20), __double2loint(p)) : 0.0;
+          }
+          acc += (s[0] + s[1]) + (s[2] + s[3]);
         }
       }
       return warp_sumd(acc);
