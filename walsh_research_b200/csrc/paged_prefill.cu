@@ -247,16 +247,19 @@ __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArg
 }
 
 // Tensor-core form for 16-bit types (mma.sync m16n8k16, float32 accumulation):
-// W warps of 16 rows, K/V tiles of KT keys double-buffered in shared memory by
+// W warps of MT x 16 rows; stages of KS keys double-buffered in shared memory by
 // 16-byte asynchronous copies, one page lookup per key row and thread, made a
-// tile ahead.  Per tile and warp: S = Q K^T, the running maximum, P = 2^(c s -
-// c m) in float32, row sums of the float32 P, and O += P V with P rounded to
-// the type as the MMA operand: that rounding is relative to each probability
-// and independent between keys, so an output moves by about as much as its own
-// rounding does.  O and the row sums are only rescaled when a row's maximum has
-// grown by more than 8 powers of two since it was last moved (P <= 2^8).
-// With 16 channels the exponentials bound it (16 per clock and SM), with 32
-// they and the MMAs take the same time.
+// stage ahead; steps of KT keys within a stage without barriers, and only those
+// that some row of the warp sees.  Per step and warp: S - m = Q K^T - m (m is the
+// MMAs' addend), P = 2^(c (S - m)) in float32, row sums of the float32 P, and O
+// += P V with P rounded to the type as the MMA operand: that rounding is relative
+// to each probability and independent between keys, so an output moves by about
+// as much as its own rounding does.  m, O and the row sums move only when a row's
+// maximum has grown by more than 8 powers of two (P <= 2^8).
+// With 16 channels the exponentials are the floor (16 per clock and SM), with 32
+// they and the MMAs take the same time; instructions bound it: of about 300 per
+// 16 x 64 scores 130 are the mathematics, 60 a stage's copies, lookups and
+// barriers (8 x 2048 tokens, 32 heads of 16, window 512: 148 us; the floor 55).
 template <typename T> __device__ __forceinline__ uint32_t pack_p(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack_p<__half>(float lo, float hi) { return pack_f16(lo, hi); }
 template <> __device__ __forceinline__ uint32_t pack_p<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
@@ -269,11 +272,16 @@ __device__ __forceinline__ int row_swz(int r, int c) {  // 16-byte piece c of ro
 }
 
 // d = a b + (c_lo, c_lo, c_hi, c_hi)
-template <typename T> __device__ __forceinline__ void mma_rowc(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo, float c_hi);
-template <> __device__ __forceinline__ void mma_rowc<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo, float c_hi) {
+template <typename T>
+__device__ __forceinline__ void mma_rowc(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo, float c_hi);
+template <>
+__device__ __forceinline__ void mma_rowc<__half>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo,
+                                                 float c_hi) {
   mma_f16_rowc(d, a, b0, b1, c_lo, c_hi);
 }
-template <> __device__ __forceinline__ void mma_rowc<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo, float c_hi) {
+template <>
+__device__ __forceinline__ void mma_rowc<__nv_bfloat16>(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, float c_lo,
+                                                        float c_hi) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%11,%11};\n"
@@ -284,13 +292,6 @@ template <> __device__ __forceinline__ void mma_rowc<__nv_bfloat16>(float* d, co
 template <typename T, int HD, int W, int MT, int KT, int KS, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const PrefillArgs<T> a) {
   constexpr int QT = W * MT * 16, NT = W * 32, CH = HD / 8, STAGE = KS * HD;
-  // c q as two 16-bit terms (22 bits together), so that the MMAs give c s - m
-  #ifndef NOFOLD
-  constexpr bool FOLD = HD == 16;
-#else
-  constexpr bool FOLD = false;
-#endif
-  constexpr int QF = FOLD ? 2 : 1;
   extern __shared__ __align__(16) unsigned char smb[];
   T* Ks = reinterpret_cast<T*>(smb);  // [2][KS][HD]
   T* Vs = Ks + 2 * STAGE;             // [2][KS][HD]
@@ -603,12 +604,14 @@ static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, cudaSt
 // (4, 1, 64, 128, 5) 149 us, (8, 1, 32, 256, 3) 148, (4, 2, 32, 128, 5) 148,
 // (8, 1, 64, 128, 2) 177, and 4.4 against 5.1 - 5.5 us for a few short
 // prompts; 32 channels (3 later parts of 3500, 64 heads, window 1024): (4, 2,
-// 32, 256, 3) 199 us, (4, 2, 32, 128, 4) 208, (4, 1, 64, 128, 4) 213.
+// 32, 256, 3) 199 us, (4, 2, 32, 128, 4) 208, (4, 1, 64, 128, 4) 213; 64 channels
+// (8 x 1000, 32 on 8 heads): (4, 1, 64, 128, 3) 84 us, (4, 1, 64, 64, 3) 86, (8, 1,
+// 64, 64, 1) 114; 128 (8 x 800, 16 on 2): (4, 1, 64, 64, 2) 52, (8, 1, 64, 64, 1) 57.
 template <typename T, int HD>
 static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
   if constexpr (HD == 16) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 5>(a, B, max_q, s);
   else if constexpr (HD == 32) return launch_prefill_tile<T, HD, 4, 2, 32, 256, 3>(a, B, max_q, s);
-  else if constexpr (HD == 64) return launch_prefill_tile<T, HD, 4, 1, 64, 64, 3>(a, B, max_q, s);
+  else if constexpr (HD == 64) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 3>(a, B, max_q, s);
   else return launch_prefill_tile<T, HD, 4, 1, 64, 64, 2>(a, B, max_q, s);
 }
 

@@ -363,8 +363,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       const float f = key_float(peer(r)->cta_max);
       if (f > -CUDART_INF_F) z_low += (float)peer(r)->cta_sum * ex2_f32((f - m) * cf);
     }
-    // Z is at most that sum times the elements behind one of the maxima
-    z_high = fminf(z_high, fmaxf(z_low, 1.f) * 1.001f * (float)((per_warp + 31) / 32 * (VEC / 2)));
+    // Z is at most that sum times the elements behind one of the maxima (of the
+    // longest part: every CTA needs the same bound)
+    const int steps = ((per_cta + NW - 1) / NW + 31) / 32;
+    z_high = fminf(z_high, fmaxf(z_low, 1.f) * 1.001f * (float)(steps * (VEC / 2)));
     z_low = fmaxf(z_low * 0.999f, 1.f);
   }
   if (m == CUDART_INF_F && !greedy) {
@@ -804,7 +806,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     // the low mantissa bits (no conversion instruction), and falls with v
     const float bin_scale = fminf(cf * ((float)kBins / x_end), 3e38f);
     auto bin_at = [&](float v) { return fmaf(m - v, bin_scale, 8388608.f); };
-    const float bins_end = 8388608.f + (float)kBins;
     // masses in units of at most 2^-22, so that they come out the same way and all of them stay below 2^31
     const float unit = fminf(4194304.f, 2147483648.0f / z_high * (1.f - 1e-3f));
     for (int i = tid; i < kBins; i += NT) sh.p.hist[i] = 0;
@@ -821,11 +822,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       for (int j = 0; j < VEC; ++j) {
         const float v = to_f(e[j]), b = bin_at(v), w = ex2_f32((v - m) * cf);
         s += w;
-        const uint32_t at = hist_s + 4u * (__float_as_uint(b) - 0x4b000000u);
+        const uint32_t bin = __float_as_uint(b) - 0x4b000000u;
         const uint32_t mass = __float_as_uint(fmaf(w, unit, 8388608.f)) - 0x4b000000u;
         asm volatile(
-            "{\n .reg .pred p;\n setp.lt.f32 p, %0, %1;\n @p red.shared.add.u32 [%2], %3;\n}\n" ::"f"(b), "f"(bins_end),
-            "r"(at), "r"(mass)
+            "{\n .reg .pred p;\n setp.lt.u32 p, %0, %1;\n @p red.shared.add.u32 [%2], %3;\n}\n" ::"r"(bin), "n"(kBins),
+            "r"(hist_s + 4u * bin), "r"(mass)
             : "memory");
       }
       sum += (double)s;
