@@ -162,11 +162,9 @@ def status_str(code: int) -> str:
 
 def call(name: str, *args) -> int:
     global launch_count
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     launch_count += KERNELS_PER_CALL.get(name, 1)
-    if name in _PLAIN_INT or name in _RESTYPE:
-        return rc
-    if rc != 0:
+    if rc != 0 and name not in _PLAIN_INT and name not in _RESTYPE:
         raise WalshError(name, rc, status_str(rc))
     return rc
 

@@ -600,27 +600,27 @@ def _call_on(dev, name, *args):
 
 
 def _head_rows(x, heads, hd, dtype, what):
-    """x [N, heads, hd] with its address, token and head strides, copied when a
-    row is not contiguous or not on 16-byte boundaries."""
+    """x [N, heads, hd] with its address, sizes, token and head strides, copied
+    when a row is not contiguous or not on 16-byte boundaries."""
     shape = x.shape
     if len(shape) != 3 or shape[2] != hd or (heads is not None and shape[1] != heads):
         raise ValueError(f"{what} has shape {tuple(shape)}; expected [N, {heads or 'heads'}, {hd}]")
-    if x.dtype != dtype:
+    if x.dtype is not dtype:
         raise ValueError(f"{what} is {x.dtype}; the pages are {dtype}")
-    mask = 3 if dtype == torch.float32 else 7
+    n, h, _ = shape
     st, sh, sd = x.stride()
-    if shape[0] <= 1:
+    if n <= 1:
         st = 0
-    if shape[1] <= 1:
+    if h <= 1:
         sh = 0
-    if sd != 1 or (st | sh) & mask:
+    if sd != 1 or (st | sh) & (3 if dtype is torch.float32 else 7):
         x = x.contiguous()
-        st, sh = (shape[1] * hd if shape[0] > 1 else 0), (hd if shape[1] > 1 else 0)
+        st, sh = (h * hd if n > 1 else 0), (hd if h > 1 else 0)
     p = x.data_ptr()
     if p & 15:
         x = x.clone(memory_format=torch.contiguous_format)
-        st, sh, p = (shape[1] * hd if shape[0] > 1 else 0), (hd if shape[1] > 1 else 0), x.data_ptr()
-    return x, p, st, sh
+        st, sh, p = (h * hd if n > 1 else 0), (hd if h > 1 else 0), x.data_ptr()
+    return x, p, n, h, st, sh
 
 
 _INT32 = (torch.int32,)
@@ -636,7 +636,7 @@ def _index_vector(x, n, what, dtypes=_INT32):
 def _out_rows(out, like, shape):
     if out is None:  # (of a view, empty_like would keep the strides)
         return torch.empty_like(like) if like.is_contiguous() else torch.empty(shape, dtype=like.dtype, device=like.device)
-    if out.shape != shape or out.dtype != like.dtype or not out.is_contiguous():
+    if out.shape != shape or out.dtype is not like.dtype or not out.is_contiguous():
         raise ValueError(f"out must be contiguous {like.dtype} {tuple(shape)}, got {out.dtype} {tuple(out.shape)}")
     return out
 
@@ -691,48 +691,51 @@ def paged_append(q, k, v, k_pages, v_pages, slots, positions=None, rope=None, q_
     q|k|v, or head-major).  Slots must be distinct.  ``err`` (int32 [1])
     becomes nonzero when a slot or position is out of range; such a token is
     not stored and its q_out row is zero (for a position).  One launch."""
-    dev = _device_of(k_pages, v_pages, q, k, v, slots, positions, q_norm, k_norm, q_out, err)
+    if (positions is None) != (rope is None):
+        raise ValueError("positions and rope go together")
+    cos, sin = (None, None) if rope is None else rope
+    dev = _device_of(k_pages, v_pages, q, k, v, slots, positions, cos, sin, q_norm, k_norm, q_out, err)
     kv = _paged_kv(k_pages, v_pages, err=err)
     _, hk, _, hd = k_pages.shape
     dt = k_pages.dtype
-    k, kp, k_ts, k_hs = _head_rows(k, hk, hd, dt, "k")
-    v, vp, v_ts, v_hs = _head_rows(v, hk, hd, dt, "v")
-    n = k.shape[0]
-    hq = q_ts = q_hs = 0
-    qp = None
+    k, kp, n, _, k_ts, k_hs = _head_rows(k, hk, hd, dt, "k")
+    v, vp, nv, _, v_ts, v_hs = _head_rows(v, hk, hd, dt, "v")
+    hq = q_ts = q_hs = n_pos = 0
+    qp = op = pp = cp = sp = None
+    nq = n
     if q is not None:
-        q, qp, q_ts, q_hs = _head_rows(q, None, hd, dt, "q")
-        hq = q.shape[1]
-        q_out = _out_rows(q_out, q, (q.shape[0], hq, hd))
+        q, qp, nq, hq, q_ts, q_hs = _head_rows(q, None, hd, dt, "q")
+        q_out = _out_rows(q_out, q, (nq, hq, hd))
+        op = q_out.data_ptr()
     elif q_out is not None or q_norm is not None:
         raise ValueError("q_out and q_norm need q")
-    if v.shape[0] != n or (q is not None and q.shape[0] != n):
+    if nv != n or nq != n:
         raise ValueError("q, k and v must have the same number of tokens")
     slots = _index_vector(slots, n, "slots", _INTS)
-    cos = sin = None
-    n_pos = 0
-    if (positions is None) != (rope is None):
-        raise ValueError("positions and rope go together")
     if positions is not None:
         positions = _index_vector(positions, n, "positions", _INTS)
-        if positions.dtype != slots.dtype:
+        if positions.dtype is not slots.dtype:
             positions = positions.to(slots.dtype)
-        cos, sin = rope
-        _device_of(k_pages, cos, sin)
-        if (cos.dim() != 2 or cos.shape[1] != hd // 2 or cos.shape != sin.shape or cos.dtype != torch.float32
-                or sin.dtype != torch.float32):
+        size = cos.shape
+        if (len(size) != 2 or size[1] * 2 != hd or sin.shape != size or cos.dtype is not torch.float32
+                or sin.dtype is not torch.float32):
             raise ValueError(f"rope must be two float32 [n_pos, {hd // 2}] tables")
         cos, sin = _c(cos), _c(sin)
-        n_pos = cos.shape[0]
-    for w, what in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None and (w.dtype != torch.float32 or w.shape != (hd,) or not w.is_contiguous()):
-            raise ValueError(f"{what} must be contiguous float32 [{hd}]")
+        n_pos, pp, cp, sp = size[0], positions.data_ptr(), cos.data_ptr(), sin.data_ptr()
+    if q_norm is not None:
+        _check_norm(q_norm, hd, "q_norm")
+    if k_norm is not None:
+        _check_norm(k_norm, hd, "k_norm")
     if n == 0:
         return q_out
-    _call_on(dev, "walsh_paged_append", kv, qp, q_ts, q_hs, kp, k_ts, k_hs, vp, v_ts, v_hs, n, hq, slots.data_ptr(),
-             ptr(positions), slots.dtype == torch.int64, ptr(cos), ptr(sin), n_pos, ptr(q_norm), ptr(k_norm), float(eps),
-             ptr(q_out))
+    _call_on(dev, "walsh_paged_append", kv, qp, q_ts, q_hs, kp, k_ts, k_hs, vp, v_ts, v_hs, n, hq, slots.data_ptr(), pp,
+             slots.dtype is torch.int64, cp, sp, n_pos, ptr(q_norm), ptr(k_norm), float(eps), op)
     return q_out
+
+
+def _check_norm(w, hd, what):
+    if w.dtype is not torch.float32 or w.shape != (hd,) or not w.is_contiguous():
+        raise ValueError(f"{what} must be contiguous float32 [{hd}]")
 
 
 @functools.lru_cache(maxsize=4096)
@@ -758,11 +761,10 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, wind
     dev = _device_of(k_pages, v_pages, q, page_table, kv_lens, out, err)
     kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
     _, hk, ps, hd = k_pages.shape
-    q, qp, q_bs, q_hs = _head_rows(q, None, hd, k_pages.dtype, "q")
-    B, hq, _ = shape = q.shape
+    q, qp, B, hq, q_bs, q_hs = _head_rows(q, None, hd, k_pages.dtype, "q")
     if page_table.shape[0] != B:
         raise ValueError(f"{B} queries and a page table of {page_table.shape[0]} rows")
-    out = _out_rows(out, q, shape)
+    out = _out_rows(out, q, (B, hq, hd))
     if B == 0:
         return out
     if max_len is None:
@@ -784,11 +786,11 @@ def paged_prefill_attention(q, q_offsets, k_pages, v_pages, page_table, kv_lens,
     of ``out`` outside every span are left as they are."""
     dev = _device_of(k_pages, v_pages, q, q_offsets, page_table, kv_lens, out, err)
     kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
-    q, qp, q_ts, q_hs = _head_rows(q, None, k_pages.shape[3], k_pages.dtype, "q")
-    n, hq, _ = shape = q.shape
+    hd = k_pages.shape[3]
+    q, qp, n, hq, q_ts, q_hs = _head_rows(q, None, hd, k_pages.dtype, "q")
     B = page_table.shape[0]
     q_offsets = _index_vector(q_offsets, B + 1, "q_offsets")
-    out = _out_rows(out, q, shape)
+    out = _out_rows(out, q, (n, hq, hd))
     if n == 0 or B == 0:
         return out
     _call_on(dev, "walsh_paged_prefill_fwd", kv, qp, q_ts, q_hs, n, q_offsets.data_ptr(), B, hq,
