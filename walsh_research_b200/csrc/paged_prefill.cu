@@ -88,17 +88,22 @@ __device__ __noinline__ void prefill_row_again(const PrefillArgs<T>& a, int b, i
     if (i * 32 + lane < HD) op[i * 32 + lane] = round_f<T>(l == 0.f ? 0.f : acc[i] / l);
 }
 
-// CUDA-core form for float32: 64 rows x 32 keys a step, 256 threads; a half warp owns four
+// CUDA-core form for float32: 64 rows x KT keys a step, 256 threads; a half warp owns four
 // rows (scores, softmax and accumulator), so only K and V tiles need barriers.
-template <typename T, int HD>
+// Shared-memory loads bound it: a thread's KT / 16 x 4 scores and its four rows of P V
+// read operands as float4 (KT = 64; 32 for 128 channels, whose tiles fill the memory).
+template <typename T, int HD, int KT>
 __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArgs<T> a) {
-  constexpr int QT = 64, KT = 32, LD = HD + 4, VEC = 16 / (int)sizeof(T), CH = HD / VEC;
+  constexpr int QT = 64, KJ = KT / 16, LD = HD + 4, LP = KT + 4, VEC = 16 / (int)sizeof(T), CH = HD / VEC;
+  static_assert(sizeof(T) == 4, "16-bit types take the tensor-core form");
   extern __shared__ __align__(16) float sm[];
   float* Qs = sm;             // [QT][LD]
   float* Ks = Qs + QT * LD;   // [KT][LD]
   float* Vs = Ks + KT * LD;   // [KT][LD]
-  float* Ps = Vs + KT * LD;   // [QT][KT + 1]
-  __shared__ int okk[KT];
+  float* Ps = Vs + KT * LD;   // [QT][LP]
+  // key of each row of a tile (-1: none, or in a bad page) and its offset, looked up a tile ahead
+  __shared__ int okk[2][KT];
+  __shared__ int64_t offs[2][KT];
   const int b = blockIdx.z, hk = blockIdx.y, tid = threadIdx.x, ty = tid >> 4, tx = tid & 15;
   int64_t first;
   const int T_ = query_span(a, b, &first);
@@ -107,142 +112,149 @@ __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArg
   const int len = seq_len(a.pg, b), pos0 = len - T_;
   const int* trow = a.pg.table + (int64_t)b * a.pg.table_stride;
   const int64_t hoff = (int64_t)hk * a.pg.head_stride;
-  // the grid covers max_q tokens; tiles of a longer span follow in further turns
-  for (int64_t r0 = (int64_t)blockIdx.x * QT; r0 < nrows; r0 += (int64_t)gridDim.x * QT) {
-  const int nr = (int)min64(QT, nrows - r0);
-  __syncthreads();
-  for (int i = tid; i < QT * CH; i += 256) {
-    const int r = i / CH, c = i - r * CH;
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (r < nr) {
-      const uint32_t t = fdiv((uint32_t)(r0 + r), a.group), g = (uint32_t)(r0 + r) - t * G;
-      raw = *reinterpret_cast<const uint4*>(a.q + (first + t) * a.q_ts + (int64_t)(hk * G + g) * a.q_hs + c * VEC);
-    }
-    const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) Qs[r * LD + c * VEC + j] = to_f(e[j]) * a.scale_log2;
-  }
-  int pos[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = min(ty * 4 + i, nr - 1);
-    pos[i] = pos0 + (int)fdiv((uint32_t)(r0 + r), a.group);
-  }
-  // keys some row of this tile sees: sinks, then lo .. hi
-  const int pos_first = pos0 + (int)fdiv((uint32_t)r0, a.group);
-  const int pos_last = pos0 + (int)fdiv((uint32_t)(r0 + nr - 1), a.group);
-  const int lo = a.pg.window > 0 ? max(0, pos_first + 1 - a.pg.window) : 0;
-  const int nsink = min(a.pg.sinks, lo), n = nsink + max(0, pos_last + 1 - lo);
-  float m[4], l[4], acc[4][HD / 16];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    m[i] = -CUDART_INF_F;
-    l[i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < HD / 16; ++d) acc[i][d] = 0.f;
-  }
-  for (int k0 = 0; k0 < n; k0 += KT) {
+  const int64_t tiles = (nrows + QT - 1) / QT;
+  // the grid covers max_q tokens, latest (longest) tiles first; tiles of a longer span follow in further turns
+  for (int64_t turn = blockIdx.x; turn < tiles; turn += gridDim.x) {
+    const int64_t r0 = (tiles - 1 - turn) * QT;
+    const int nr = (int)min64(QT, nrows - r0);
     __syncthreads();
-    for (int i = tid; i < KT * CH; i += 256) {
-      const int r = i / CH, c = i - r * CH, x = k0 + r;
-      const int key = x < nsink ? x : lo + (x - nsink);
-      int64_t off = -1;
-      if (x < n) off = key_offset(a.pg, trow, key);
-      uint4 kr = make_uint4(0u, 0u, 0u, 0u), vr = kr;
-      if (off >= 0) {
-        kr = __ldg(reinterpret_cast<const uint4*>(a.pg.k + hoff + off + c * VEC));
-        vr = __ldg(reinterpret_cast<const uint4*>(a.pg.v + hoff + off + c * VEC));
+    for (int i = tid; i < QT * CH; i += 256) {
+      const int r = i / CH, c = i - r * CH;
+      uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+      if (r < nr) {
+        const uint32_t t = fdiv((uint32_t)(r0 + r), a.group), g = (uint32_t)(r0 + r) - t * G;
+        raw = *reinterpret_cast<const uint4*>(a.q + (first + t) * a.q_ts + (int64_t)(hk * G + g) * a.q_hs + c * VEC);
       }
-      if (c == 0) okk[r] = off >= 0 ? key : -1;
-      const T *ke = reinterpret_cast<const T*>(&kr), *ve = reinterpret_cast<const T*>(&vr);
+      const T* e = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-      for (int j = 0; j < VEC; ++j) {
-        Ks[r * LD + c * VEC + j] = to_f(ke[j]);
-        Vs[r * LD + c * VEC + j] = to_f(ve[j]);
-      }
+      for (int j = 0; j < VEC; ++j) Qs[r * LD + c * VEC + j] = to_f(e[j]) * a.scale_log2;
     }
-    __syncthreads();
-    float s[4][2] = {};
-    for (int d = 0; d < HD; d += 4) {
-      float4 q4[4], k4[2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q4[i] = *reinterpret_cast<const float4*>(&Qs[(ty * 4 + i) * LD + d]);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) k4[j] = *reinterpret_cast<const float4*>(&Ks[(tx + 16 * j) * LD + d]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-          s[i][j] = fmaf(q4[i].x, k4[j].x, fmaf(q4[i].y, k4[j].y, fmaf(q4[i].z, k4[j].z, fmaf(q4[i].w, k4[j].w, s[i][j]))));
-    }
+    int pos[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      bool see[2];
-      float mt = -CUDART_INF_F;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int key = okk[tx + 16 * j];
-        see[j] = key >= 0 && key <= pos[i] &&
-                 (a.pg.window == 0 || key > pos[i] - a.pg.window || key < a.pg.sinks);
-        if (!see[j]) s[i][j] = -CUDART_INF_F;
-        mt = fmaxf(mt, s[i][j]);
-      }
-#pragma unroll
-      for (int o = 1; o < 16; o <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
-      const float mn = fmaxf(m[i], mt), sub_m = mn == -CUDART_INF_F ? 0.f : mn;
-      const float corr = ex2_f32(m[i] - sub_m);
-      m[i] = mn;
-      l[i] *= corr;
-#pragma unroll
-      for (int d = 0; d < HD / 16; ++d) acc[i][d] *= corr;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float p = see[j] ? ex2_f32(s[i][j] - sub_m) : 0.f;
-        l[i] += p;
-        Ps[(ty * 4 + i) * (KT + 1) + tx + 16 * j] = p;
-      }
+      const int r = min(ty * 4 + i, nr - 1);
+      pos[i] = pos0 + (int)fdiv((uint32_t)(r0 + r), a.group);
     }
-    __syncwarp();
-    for (int j = 0; j < KT; ++j) {
-      float v[HD / 16];
+    // keys some row of this tile sees: sinks, then lo .. hi
+    const int pos_first = pos0 + (int)fdiv((uint32_t)r0, a.group);
+    const int pos_last = pos0 + (int)fdiv((uint32_t)(r0 + nr - 1), a.group);
+    const int lo = a.pg.window > 0 ? max(0, pos_first + 1 - a.pg.window) : 0;
+    const int nsink = min(a.pg.sinks, lo), n = nsink + max(0, pos_last + 1 - lo);
+    float m[4], l[4], acc[4][HD / 16];
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) v[d] = Vs[j * LD + tx + 16 * d];
+    for (int i = 0; i < 4; ++i) {
+      m[i] = -CUDART_INF_F;
+      l[i] = 0.f;
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) acc[i][d] = 0.f;
+    }
+    auto lookup = [&](int k0, int buf) {
+      if (tid < KT) {
+        const int x = k0 + tid, key = x < nsink ? x : lo + (x - nsink);
+        const int64_t off = x < n ? key_offset(a.pg, trow, key) : -1;
+        offs[buf][tid] = off;
+        okk[buf][tid] = off >= 0 ? key : -1;
+      }
+    };
+    lookup(0, 0);
+    for (int k0 = 0, buf = 0; k0 < n; k0 += KT, buf ^= 1) {
+      __syncthreads();
+      for (int i = tid; i < KT * CH; i += 256) {
+        const int r = i / CH, c = i - r * CH;
+        const int64_t off = offs[buf][r];
+        uint4 kr = make_uint4(0u, 0u, 0u, 0u), vr = kr;
+        if (off >= 0) {
+          kr = __ldg(reinterpret_cast<const uint4*>(a.pg.k + hoff + off + c * VEC));
+          vr = __ldg(reinterpret_cast<const uint4*>(a.pg.v + hoff + off + c * VEC));
+        }
+        *reinterpret_cast<uint4*>(&Ks[r * LD + c * VEC]) = kr;
+        *reinterpret_cast<uint4*>(&Vs[r * LD + c * VEC]) = vr;
+      }
+      lookup(k0 + KT, buf ^ 1);
+      __syncthreads();
+      float s[4][KJ] = {};
+      for (int d = 0; d < HD; d += 4) {
+        float4 q4[4], k4[KJ];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q4[i] = *reinterpret_cast<const float4*>(&Qs[(ty * 4 + i) * LD + d]);
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) k4[j] = *reinterpret_cast<const float4*>(&Ks[(tx + 16 * j) * LD + d]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < KJ; ++j)
+            s[i][j] = fmaf(q4[i].x, k4[j].x, fmaf(q4[i].y, k4[j].y, fmaf(q4[i].z, k4[j].z, fmaf(q4[i].w, k4[j].w, s[i][j]))));
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float p = Ps[(ty * 4 + i) * (KT + 1) + j];
+        bool see[KJ];
+        float mt = -CUDART_INF_F;
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) acc[i][d] = fmaf(p, v[d], acc[i][d]);
+        for (int j = 0; j < KJ; ++j) {
+          const int key = okk[buf][tx + 16 * j];
+          see[j] = key >= 0 && key <= pos[i] &&
+                   (a.pg.window == 0 || key > pos[i] - a.pg.window || key < a.pg.sinks);
+          if (!see[j]) s[i][j] = -CUDART_INF_F;
+          mt = fmaxf(mt, s[i][j]);
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, o));
+        const float mn = fmaxf(m[i], mt), sub_m = mn == -CUDART_INF_F ? 0.f : mn;
+        const float corr = ex2_f32(m[i] - sub_m);
+        m[i] = mn;
+        l[i] *= corr;
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) acc[i][d] *= corr;
+#pragma unroll
+        for (int j = 0; j < KJ; ++j) {
+          const float p = see[j] ? ex2_f32(s[i][j] - sub_m) : 0.f;
+          l[i] += p;
+          Ps[(ty * 4 + i) * LP + tx + 16 * j] = p;
+        }
       }
+      __syncwarp();
+      for (int j = 0; j < KT; j += 4) {
+        float4 p4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p4[i] = *reinterpret_cast<const float4*>(&Ps[(ty * 4 + i) * LP + j]);
+#pragma unroll
+        for (int d = 0; d < HD / 16; ++d) {
+          const float* vp = &Vs[j * LD + tx + 16 * d];
+          const float v0 = vp[0], v1 = vp[LD], v2 = vp[2 * LD], v3 = vp[3 * LD];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            acc[i][d] = fmaf(p4[i].w, v3, fmaf(p4[i].z, v2, fmaf(p4[i].y, v1, fmaf(p4[i].x, v0, acc[i][d]))));
+        }
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  }
-  const int64_t Hq = (int64_t)a.kv_heads * G;
+    const int64_t Hq = (int64_t)a.kv_heads * G;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float L = l[i];
+    for (int i = 0; i < 4; ++i) {
+      float L = l[i];
 #pragma unroll
-    for (int o = 1; o < 16; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    const int r = ty * 4 + i;
-    bool nan = false;
-    if (r < nr) {
-      const uint32_t t = fdiv((uint32_t)(r0 + r), a.group), g = (uint32_t)(r0 + r) - t * G;
-      T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + g) * HD;
+      for (int o = 1; o < 16; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+      const int r = ty * 4 + i;
+      bool nan = false;
+      if (r < nr) {
+        const uint32_t t = fdiv((uint32_t)(r0 + r), a.group), g = (uint32_t)(r0 + r) - t * G;
+        T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + g) * HD;
 #pragma unroll
-      for (int d = 0; d < HD / 16; ++d) {
-        const float x = L == 0.f ? 0.f : acc[i][d] / L;
-        nan |= x != x;
-        op[tx + 16 * d] = round_f<T>(x);
+        for (int d = 0; d < HD / 16; ++d) {
+          const float x = L == 0.f ? 0.f : acc[i][d] / L;
+          nan |= x != x;
+          op[tx + 16 * d] = round_f<T>(x);
+        }
       }
+      const unsigned again = __ballot_sync(0xffffffffu, nan);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        if (again & (0xffffu << (16 * h))) {
+          const uint32_t x = (uint32_t)(r0 + (ty & ~1) * 4 + h * 4 + i), t = fdiv(x, a.group), g = x - t * G;
+          prefill_row_again<T, HD>(a, b, hk, a.q + (first + t) * a.q_ts + (int64_t)(hk * G + g) * a.q_hs, pos0 + (int)t,
+                                   a.o + ((first + t) * Hq + (int64_t)hk * G + g) * HD);
+        }
     }
-    const unsigned again = __ballot_sync(0xffffffffu, nan);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      if (again & (0xffffu << (16 * h))) {
-        const uint32_t x = (uint32_t)(r0 + (ty & ~1) * 4 + h * 4 + i), t = fdiv(x, a.group), g = x - t * G;
-        prefill_row_again<T, HD>(a, b, hk, a.q + (first + t) * a.q_ts + (int64_t)(hk * G + g) * a.q_hs, pos0 + (int)t,
-                                 a.o + ((first + t) * Hq + (int64_t)hk * G + g) * HD);
-      }
-  }
   }
 }
 
@@ -617,15 +629,19 @@ static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStr
 
 template <typename T, int HD>
 static int launch_prefill(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
-  if constexpr (sizeof(T) == 2) return launch_prefill_mma<T, HD>(a, B, max_q, s);
-  constexpr int QT = 64, KT = 32, LD = HD + 4;
-  const int smem = ((QT + 2 * KT) * LD + QT * (KT + 1)) * 4;
-  auto* kern = paged_prefill_vec_kernel<T, HD>;
-  if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  if constexpr (sizeof(T) == 2) {
+    return launch_prefill_mma<T, HD>(a, B, max_q, s);
+  } else {
+    constexpr int QT = 64, KT = HD == 128 ? 32 : 64, LD = HD + 4;
+    constexpr int smem = ((QT + 2 * KT) * LD + QT * (KT + 4)) * 4;
+    auto* kern = paged_prefill_vec_kernel<T, HD, KT>;
+    if (smem > 40 * 1024 &&
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return launch_status();
+    const int64_t tiles = ((int64_t)max_q * a.group.d + QT - 1) / QT;
+    kern<<<dim3((unsigned)tiles, a.kv_heads, B), 256, smem, s>>>(a);
     return launch_status();
-  const int64_t tiles = ((int64_t)max_q * a.group.d + QT - 1) / QT;
-  kern<<<dim3((unsigned)tiles, a.kv_heads, B), 256, smem, s>>>(a);
-  return launch_status();
+  }
 }
 
 }  // namespace walsh
