@@ -62,6 +62,12 @@ __device__ __forceinline__ void store32(void* p, const uint4* r, bool wide) {
   }
 }
 
+// four values of a rotation table (whose rows need not lie on 16-byte boundaries)
+__device__ __forceinline__ float4 load_rope(const float* p, bool vec) {
+  if (vec) return __ldg(reinterpret_cast<const float4*>(p));
+  return make_float4(__ldg(p), __ldg(p + 1), __ldg(p + 2), __ldg(p + 3));
+}
+
 // 32 bytes as floats, and back with one rounding each
 template <typename T>
 __device__ __forceinline__ void piece_to_f(const uint4* raw, float* x) {
@@ -148,8 +154,7 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const AppendArgs<T> a
       const float* sp = a.sin + pos * (HD / 2) + c / 2;
 #pragma unroll
       for (int j = 0; j < VEC; j += 8) {  // rows of the tables are 32 bytes or more
-        const float4 cv = a.vec_rope ? __ldg(reinterpret_cast<const float4*>(cp + j / 2)) : make_float4(cp[j / 2], cp[j / 2 + 1], cp[j / 2 + 2], cp[j / 2 + 3]);
-        const float4 sv = a.vec_rope ? __ldg(reinterpret_cast<const float4*>(sp + j / 2)) : make_float4(sp[j / 2], sp[j / 2 + 1], sp[j / 2 + 2], sp[j / 2 + 3]);
+        const float4 cv = load_rope(cp + j / 2, a.vec_rope), sv = load_rope(sp + j / 2, a.vec_rope);
         const float cc[4] = {cv.x, cv.y, cv.z, cv.w}, sn[4] = {sv.x, sv.y, sv.z, sv.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -1296,7 +1296,10 @@ template <typename T, int CS>
 static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
   const int part = ((VEC - 1 + a.vocab + VEC - 1) / VEC + CS - 1) / CS * 16;
-  return part <= kStageBytes ? launch_sample_as<T, CS, true>(a, part, s) : launch_sample_as<T, CS, false>(a, part, s);
+  constexpr int most = (kSampleMaxVocab / VEC + 1 + CS - 1) / CS * 16;  // of any vocabulary
+  if constexpr (most > kStageBytes)
+    if (part > kStageBytes) return launch_sample_as<T, CS, false>(a, part, s);
+  return launch_sample_as<T, CS, true>(a, part, s);
 }
 
 // CTAs per row: one when the rows alone occupy every SM (the barriers and scalar
