@@ -167,6 +167,16 @@ def test_generate_batch_draws_stops_and_ends():
     assert m.generate_batch([], 3) == [] and torch.equal(m.generate_batch(prompts[:1], 0)[0], prompts[0])
 
 
+def test_generate_batch_returns_long_prompts_whole():
+    """Only the last max_seq_len ids are read, but all of them come back."""
+    cfg, n, sd, m = _model()
+    long, short = _ids(cfg, 90, seed=1), _ids(cfg, 6, seed=2)
+    a = m.generate_batch([long, short], 3, top_k=1, max_seq_len=32)
+    b = m.generate_batch([long[-32:], short], 3, top_k=1, max_seq_len=32)
+    assert torch.equal(a[0][:90], long) and torch.equal(a[0][90:], b[0][32:]) and a[0].numel() == 91
+    assert torch.equal(a[1], b[1]) and a[1].numel() == 9
+
+
 def test_generate_with_top_p_follows_sample_tokens():
     from walsh_research_b200 import _lib, ops
     from walsh_research_b200.model import KVCache

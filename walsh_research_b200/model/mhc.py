@@ -626,16 +626,18 @@ class mHCWalsh(nn.Module):
         tensors, prompt and continuation.  A sequence ends after
         ``max_new_tokens``, at ``stop_token`` (kept; checked on the host every
         step when given) or when ``max_seq_len`` (default block_size, at most
-        the rotation table's 2 block_size) tokens are cached.  ``window`` and
-        ``sinks`` as in PagedKVCache."""
+        the rotation table's 2 block_size) tokens are cached; of a longer prompt
+        the last ``max_seq_len`` ids are read.  ``window`` and ``sinks`` as in
+        PagedKVCache."""
         limit = self.config.block_size if max_seq_len is None else int(max_seq_len)
         if not 0 < limit <= self.freqs_cis.shape[0]:
             raise ValueError(f"max_seq_len must be in 1 .. {self.freqs_cis.shape[0]}, got {limit}")
-        prompts = [p[-limit:] for p in prompts]
-        if any(p.dim() != 1 or p.numel() == 0 for p in prompts):
+        given = list(prompts)
+        if any(p.dim() != 1 or p.numel() == 0 for p in given):
             raise ValueError("prompts must be non-empty 1-D tensors of token ids")
-        if max_new_tokens <= 0 or not prompts:
-            return list(prompts)
+        if max_new_tokens <= 0 or not given:
+            return given
+        prompts = [p[-limit:] for p in given]
         C, H, dev = self.config.n_embd, self.config.n_head, prompts[0].device
         grown = [min(limit, p.numel() + max_new_tokens - 1) for p in prompts]
         cache = PagedKVCache(self.config.n_layer, sum(-(-n // page_size) for n in grown), page_size, H, C // H, dev,
@@ -672,7 +674,7 @@ class mHCWalsh(nn.Module):
             nxt = draw(out[:, -1])
             for i, t in zip(live, nxt[:, 0].unbind()):
                 tokens[i].append(t)
-        return [torch.cat((p, torch.stack(t).to(p.dtype))) for p, t in zip(prompts, tokens)]
+        return [torch.cat((p, torch.stack(t).to(p.dtype))) for p, t in zip(given, tokens)]
 
     @torch.no_grad()
     def generate(self, idx, max_new_tokens, temperature=1.0, top_k=None, use_cache=True, generator=None, top_p=None,
