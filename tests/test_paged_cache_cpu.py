@@ -100,3 +100,19 @@ def test_table_rows_are_free_of_other_sequences():
             c.select(live).begin(2)
             c.select(live).increment(2)
         assert len(set(owned(c))) == len(owned(c)) == 40 - c.free_pages
+
+
+def test_batches_of_nothing_or_of_removed_sequences_are_refused():
+    c = make()
+    a, b = c.add(2)
+    batch = c.select([a, b])
+    for what in (lambda: c.select([]).begin(1), lambda: batch.begin(0), lambda: batch.increment(-1)):
+        with pytest.raises(ValueError):
+            what()
+    batch.begin(3)
+    batch.increment(3)
+    c.remove([a])
+    for what in (lambda: batch.begin(1), lambda: batch.increment(1)):
+        with pytest.raises(ValueError):
+            what()
+    assert c.free_pages == 9 and c.lengths([b]) == [3]

@@ -125,12 +125,18 @@ class PagedBatch:
 
     def increment(self, n: int = 1):
         """Counts the ``n`` tokens per sequence that the last forward stored."""
+        if n < 0:
+            raise ValueError(f"stored tokens cannot be taken back, got {n}")
+        self.cache._ids(self.ids)  # none of them removed since
         self.cache._reserve(self.ids, n)
         self.cache._advance(self.ids, n)
 
     def begin(self, n: int) -> "PagedStep":
         """Reserves pages for ``n`` tokens per sequence and lays out where they go."""
         c, ids = self.cache, self.ids
+        if n < 1 or not len(ids):
+            raise ValueError(f"a forward needs sequences and tokens, got {len(ids)} of {n} tokens")
+        c._ids(ids)  # none of them removed since the selection
         c._reserve(ids, n)
         B, ps = len(ids), c.page_size
         pos = c._len[ids][:, None] + np.arange(n)[None]
