@@ -1,0 +1,66 @@
+"""Paged attention in 16-bit types: what the float32 probabilities lose on
+their way through the tensor cores, and values that are not finite."""
+import pytest
+import torch
+
+import serving_reference as R
+from walsh_research_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+HALF = [torch.float16, torch.bfloat16]
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def attend(q, k, v, pos0, window=0, sinks=0):
+    """As serving_reference.attend with a bound in which each probability is
+    held by two terms of q's type: off by half a step of a half step relative,
+    and in float16, whose smallest step is 2^-24, by 2^-25 of the largest."""
+    dt, hd, L = q.dtype, q.shape[-1], k.shape[0]
+    half = torch.finfo(dt).eps / 2
+    q, k, v = (t.double() for t in (q, k, v))
+    g = q.shape[1] // k.shape[1]
+    k, v = k.repeat_interleave(g, 1), v.repeat_interleave(g, 1)
+    i, j = pos0 + torch.arange(q.shape[0], device=q.device)[:, None], torch.arange(L, device=q.device)[None]
+    see = j <= i
+    if window:
+        see = see & ((j > i - window) | (j < sinks))
+    scale = hd ** -0.5
+    s = torch.einsum("thd,jhd->htj", q, k) * scale
+    s_abs = torch.einsum("thd,jhd->htj", q.abs(), k.abs()).masked_fill(~see, 0.0).amax(-1) * scale
+    p = torch.exp(s - s.masked_fill(~see, float("-inf")).amax(-1, keepdim=True)).masked_fill(~see, 0.0)
+    l = p.sum(-1, keepdim=True)
+    o = torch.einsum("htj,jhd->thd", p / l, v)
+    a = torch.einsum("htj,jhd->thd", p / l, v.abs())
+    seen = torch.einsum("htj,jhd->thd", see.double().expand_as(p) / l, v.abs())
+    # scores: hd products summed in float32, good exponentials; sums over the keys in at least 16 parts
+    d = 2 * (2.0 ** -24 * (hd + 4) * s_abs + 2.0 ** -22) + 2 * (L / 16 + 64) * 2.0 ** -24
+    least = 2.0 ** -25 if dt is torch.float16 else 0.0
+    return o, half * o.abs() + (half * half + d.t()[..., None]) * a + least * seen + torch.finfo(dt).tiny * torch.finfo(dt).eps
+
+
+def close(got, want, bound):
+    got = got.double()
+    assert not torch.isnan(got).any()
+    d = (got - want).abs()
+    assert (d <= bound).all(), f"{int((d > bound).sum())} of {d.numel()} off, worst {float((d / bound).max()):.3g} bounds"
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("hq,hk,hd", [(32, 32, 16), (4, 2, 32), (8, 1, 64), (6, 2, 128), (20, 1, 16)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (64, 3)])
+def test_prefill_keeps_probabilities_in_two_terms(dtype, hq, hk, hd, window, sinks):
+    g = gen(hd + hq)
+    new, past = [200, 70], [0, 150]
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [a + b for a, b in zip(new, past)], hk, 16, hd, dtype))
+    q = (1.5 * torch.randn(sum(new), hq, hd, generator=g)).to(dtype).to(DEV)
+    off = torch.tensor([0] + new).cumsum(0).int().to(DEV)
+    out = ops.paged_prefill_attention(q, off, kp, vp, table, kl, window=window, sinks=sinks)
+    at = 0
+    for b, t in enumerate(new):
+        k, v = (R.gather_keys(p, table[b], past[b] + t) for p in (kp, vp))
+        close(out[at:at + t], *attend(q[at:at + t], k, v, past[b], window, sinks))
+        at += t

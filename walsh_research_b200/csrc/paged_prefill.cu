@@ -264,17 +264,28 @@ __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArg
 // stage ahead; steps of KT keys within a stage without barriers, and only those
 // that some row of the warp sees.  Per step and warp: S - m = Q K^T - m (m is the
 // MMAs' addend), P = 2^(c (S - m)) in float32, row sums of the float32 P, and O
-// += P V with P rounded to the type as the MMA operand: that rounding is relative
-// to each probability and independent between keys, so an output moves by about
-// as much as its own rounding does.  m, O and the row sums move only when a row's
-// maximum has grown by more than 8 powers of two (P <= 2^8).
+// += P V with P as two 16-bit terms, P rounded to the type and what that left
+// over, rounded again: 2^-18 (bf16) or 2^-22 (fp16, down to its smallest step) of
+// each probability, below the output's own rounding.  P rounded once would save
+// half of these MMAs and the splitting (150 against 179 us in the case below, 199
+// against 256 with 32 channels), but moves two outputs of five by a step.  m, O
+// and the row sums move only when a row's maximum has grown by more than 8 powers
+// of two (P <= 2^8).
 // With 16 channels the exponentials are the floor (16 per clock and SM), with 32
-// they and the MMAs take the same time; instructions bound it: of about 300 per
-// 16 x 64 scores 130 are the mathematics, 60 a stage's copies, lookups and
-// barriers (8 x 2048 tokens, 32 heads of 16, window 512: 148 us; the floor 55).
+// they and the MMAs take the same time; instructions bound it (8 x 2048 tokens,
+// 32 heads of 16, window 512: 179 us; the floor 55).
 template <typename T> __device__ __forceinline__ uint32_t pack_p(float lo, float hi);
 template <> __device__ __forceinline__ uint32_t pack_p<__half>(float lo, float hi) { return pack_f16(lo, hi); }
 template <> __device__ __forceinline__ uint32_t pack_p<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
+
+// two probabilities as the pair rounded to T and what that left over, rounded to T
+template <typename T>
+__device__ __forceinline__ void split_p(uint64_t p, uint32_t* hi, uint32_t* rest) {
+  *hi = pack_p<T>(f2_lo(p), f2_hi(p));
+  const float2 h = unpack2<T>(*hi);
+  const uint64_t r = f2_fma(f2_pack(h.x, h.y), f2_dup(-1.f), p);
+  *rest = pack_p<T>(f2_lo(r), f2_hi(r));
+}
 
 template <int HD>
 __device__ __forceinline__ int row_swz(int r, int c) {  // 16-byte piece c of row r: its place in the row
@@ -517,18 +528,20 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
             thr_min = fminf(thr_min, thr[mt][h]);
           }
       }
-      uint32_t pf[MT][KT / 16][4];
+      // P as two 16-bit terms, O += P V with both
+      uint32_t pf[MT][KT / 16][4], pl[MT][KT / 16][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint64_t rs0 = 0, rs1 = 0;
 #pragma unroll
         for (int i = 0; i < KT / 8; ++i) {
           const uint64_t x = f2_mul(f2_pack(s[mt][i][0], s[mt][i][1]), c2), y = f2_mul(f2_pack(s[mt][i][2], s[mt][i][3]), c2);
-          const float p0 = ex2_f32(f2_lo(x)), p1 = ex2_f32(f2_hi(x)), p2 = ex2_f32(f2_lo(y)), p3 = ex2_f32(f2_hi(y));
-          rs0 = f2_fma(f2_pack(p0, p1), one2, rs0);
-          rs1 = f2_fma(f2_pack(p2, p3), one2, rs1);
-          pf[mt][i >> 1][(i & 1) * 2 + 0] = pack_p<T>(p0, p1);
-          pf[mt][i >> 1][(i & 1) * 2 + 1] = pack_p<T>(p2, p3);
+          const uint64_t p0 = f2_pack(ex2_f32(f2_lo(x)), ex2_f32(f2_hi(x))), p1 = f2_pack(ex2_f32(f2_lo(y)), ex2_f32(f2_hi(y)));
+          rs0 = f2_fma(p0, one2, rs0);
+          rs1 = f2_fma(p1, one2, rs1);
+          const int kk = i >> 1, j = (i & 1) * 2;
+          split_p<T>(p0, &pf[mt][kk][j], &pl[mt][kk][j]);
+          split_p<T>(p1, &pf[mt][kk][j + 1], &pl[mt][kk][j + 1]);
         }
         l[mt][0] += f2_lo(rs0) + f2_hi(rs0);
         l[mt][1] += f2_lo(rs1) + f2_hi(rs1);
@@ -543,6 +556,8 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
           for (int mt = 0; mt < MT; ++mt) {
             mma16<T>(acc[mt][2 * dp], pf[mt][kk], vf[0], vf[1]);
             mma16<T>(acc[mt][2 * dp + 1], pf[mt][kk], vf[2], vf[3]);
+            mma16<T>(acc[mt][2 * dp], pl[mt][kk], vf[0], vf[1]);
+            mma16<T>(acc[mt][2 * dp + 1], pl[mt][kk], vf[2], vf[3]);
           }
         }
     };
@@ -612,13 +627,14 @@ static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, cudaSt
 }
 
 // Warps, 16-row tiles per warp, keys per step and per stage, CTAs per SM.
-// Measured on one GPU: 16 channels (8 x 2048 tokens, 32 heads, window 512):
-// (4, 1, 64, 128, 5) 149 us, (8, 1, 32, 256, 3) 148, (4, 2, 32, 128, 5) 148,
-// (8, 1, 64, 128, 2) 177, and 4.4 against 5.1 - 5.5 us for a few short
-// prompts; 32 channels (3 later parts of 3500, 64 heads, window 1024): (4, 2,
-// 32, 256, 3) 199 us, (4, 2, 32, 128, 4) 208, (4, 1, 64, 128, 4) 213; 64 channels
-// (8 x 1000, 32 on 8 heads): (4, 1, 64, 128, 3) 84 us, (4, 1, 64, 64, 3) 86, (8, 1,
-// 64, 64, 1) 114; 128 (8 x 800, 16 on 2): (4, 1, 64, 64, 2) 52, (8, 1, 64, 64, 1) 57.
+// Measured, replayed from a graph: 16 channels (8 x 2048 tokens, 32 heads, window
+// 512): (4, 1, 64, 128, 5) 179 us, (4, 1, 64, 128, 4) 178, (8, 1, 32, 256, 3) 184,
+// (4, 2, 32, 256, 4) 165, but 5.8 against 4.8 us for a few short prompts; 32
+// channels (3 later parts up to 3500, 64 heads, window 1024): (4, 2, 32, 256, 3)
+// 256 us, (4, 2, 32, 128, 4) 281, (4, 1, 64, 128, 4) 269; 64 channels (8 x 1000, 32
+// on 8 heads): (4, 1, 64, 128, 3) 195 us, (4, 1, 64, 64, 3) 201, (4, 1, 64, 128, 2)
+// 211; 128 (8 x 800, 16 on 2): (4, 1, 64, 64, 2) 130, (4, 1, 32, 64, 2) 131, (8, 1,
+// 64, 64, 1) 143.
 template <typename T, int HD>
 static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
   if constexpr (HD == 16) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 5>(a, B, max_q, s);
