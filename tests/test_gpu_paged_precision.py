@@ -64,3 +64,17 @@ def test_prefill_keeps_probabilities_in_two_terms(dtype, hq, hk, hd, window, sin
         k, v = (R.gather_keys(p, table[b], past[b] + t) for p in (kp, vp))
         close(out[at:at + t], *attend(q[at:at + t], k, v, past[b], window, sinks))
         at += t
+
+
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("hq,hk,hd", [(8, 8, 16), (8, 1, 64), (9, 1, 16), (16, 1, 32), (24, 2, 64), (40, 2, 128)])
+def test_decode_keeps_probabilities_in_two_terms(dtype, hq, hk, hd):
+    g = gen(hd + hq)
+    lens = [700, 33, 1, 2500]
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, lens, hk, 16, hd, dtype))
+    q = (1.5 * torch.randn(len(lens), hq, hd, generator=g)).to(dtype).to(DEV)
+    for window, sinks in ((0, 0), (300, 2)):
+        out = ops.paged_attention(q, kp, vp, table, kl, window=window, sinks=sinks)
+        for b, n in enumerate(lens):
+            k, v = (R.gather_keys(p, table[b], n) for p in (kp, vp))
+            close(out[b:b + 1], *attend(q[b:b + 1], k, v, n - 1, window, sinks))

@@ -223,9 +223,11 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
 // of NS stages of KT keys (16-byte asynchronous copies; no CTA barrier until
 // the join), page lookups made a stage ahead, one key row per lane.  The heads
 // of the group are the rows of the MMAs: S = Q K^T and O += P V (m16n8k16).
-// With up to 8 heads the rows 8 - 15 carry what rounding P to 16 bits left over
-// in rows 0 - 7, so P keeps 16 (bf16) to 22 bits at no cost; with 9 to 16 heads
-// P is rounded once, which moves an output by about as much as its own rounding.
+// P enters as two 16-bit terms, rounded and what that left over, so it keeps 16
+// (bf16) to 22 bits: with up to 8 heads the rows 8 - 15 carry the second term at
+// no cost, with 9 to 16 heads it takes MMAs of its own (64 x 4000 keys,
+// 64 heads on 4 of 64 channels 54 us both ways, 48 on 4 of 32 36 -> 38.5, 32 on 2
+// of 128 60 -> 66.5).
 // ---------------------------------------------------------------------------
 template <int HD>
 __device__ __forceinline__ int dec_swz(int r, int c) {  // 16-byte piece c of row r: its place in the row
@@ -344,7 +346,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
         for (int e = 0; e < 2; ++e)
           if (!((ok[i >> 2] >> ((i & 3) * 8 + 2 * t4 + e)) & 1u)) s[i][e] = s[i][2 + e] = -CUDART_INF_F;
     }
-    uint32_t pf[KT / 16][4];
+    uint32_t pf[KT / 16][4], pl[RH == 2 ? KT / 16 : 1][4];
 #pragma unroll
     for (int h = 0; h < RH; ++h) {
       float mt = -CUDART_INF_F;
@@ -362,10 +364,10 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
         rs += p0 + p1;
         const uint32_t hi = dec_pack<T>(p0, p1);
         pf[i >> 1][(i & 1) * 2 + h] = hi;
-        if constexpr (RH == 1) {
-          const float2 hf = unpack2<T>(hi);
-          pf[i >> 1][(i & 1) * 2 + 1] = dec_pack<T>(p0 - hf.x, p1 - hf.y);
-        }
+        const float2 hf = unpack2<T>(hi);
+        const uint32_t rest = dec_pack<T>(p0 - hf.x, p1 - hf.y);
+        if constexpr (RH == 1) pf[i >> 1][(i & 1) * 2 + 1] = rest;
+        else pl[i >> 1][(i & 1) * 2 + h] = rest;
       }
       l[h] = l[h] * corr + rs;
 #pragma unroll
@@ -383,6 +385,10 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
         ldsm_x4_t(vf, vt_s + r * HD + dec_swz<HD>(r, ch) * 8);
         mma16<T>(acc[2 * dp], pf[kk], vf[0], vf[1]);
         mma16<T>(acc[2 * dp + 1], pf[kk], vf[2], vf[3]);
+        if constexpr (RH == 2) {
+          mma16<T>(acc[2 * dp], pl[kk], vf[0], vf[1]);
+          mma16<T>(acc[2 * dp + 1], pl[kk], vf[2], vf[3]);
+        }
       }
   };
   for (int st0 = 0; st0 < nst; st0 += NS) {
