@@ -1,0 +1,71 @@
+"""Token sampling of batches of large vocabularies: every layout of a row over
+CTAs, against the definition in float64."""
+import pytest
+import torch
+
+from walsh_research_b200 import ops
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def expect(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """(ids, sure): the draws of the definition in float64, and which of them
+    do not hang on sums closer than 1e-9 of the row's mass (weights are float64
+    exponentials of relative error 1e-15; sums of 2^18 of them, 2^18 2^-53)."""
+    z = logits.double()
+    V = z.shape[1]
+    w = torch.exp((z - z.amax(1, keepdim=True)) / temperature)
+    order = torch.argsort(z, dim=1, descending=True, stable=True)
+    ws = w.gather(1, order)
+    if 0 < top_k < V:
+        ws[:, top_k:] = 0
+    sure = torch.ones(len(z), dtype=torch.bool, device=z.device)
+    if top_p < 1:
+        before, total = ws.cumsum(1) - ws, ws.sum(1, keepdim=True)
+        keep = before < top_p * total
+        keep[:, 0] = True
+        sure &= ((before - top_p * total).abs() > 1e-9 * total).all(1)
+        ws = ws * keep
+    if min_p > 0:
+        sure &= ((ws - min_p).abs() > 1e-12).all(1)
+        ws = ws * (ws >= min_p)
+    kept = torch.zeros_like(w).scatter_(1, order, ws)
+    run = kept.cumsum(1)
+    t = u.double()[:, None] * run[:, -1:]
+    ids = (run <= t).sum(1)
+    near = torch.stack((run.gather(1, ids[:, None].clamp_max(V - 1))[:, 0], run.gather(1, (ids[:, None] - 1).clamp_min(0))[:, 0]))
+    sure &= ((near - t[:, 0]).abs() > 1e-9 * run[:, -1]).all(0) | ((ids == 0) & (near[0] - t[:, 0] > 1e-9 * run[:, -1]))
+    return ids, sure, torch.log(kept.gather(1, ids[:, None].clamp_max(V - 1))[:, 0] / run[:, -1])
+
+
+def check(logits, u, **kw):
+    want, sure, lp = expect(logits, u, **kw)
+    assert sure.float().mean() > 0.9
+    for _ in range(2):
+        ids = ops.sample_tokens(logits, u, **kw)
+        assert torch.equal(ids[sure], want[sure]), (int((ids[sure] != want[sure]).sum()), int(sure.sum()))
+        ids, logp = ops.sample_tokens(logits, u, want_logprob=True, **kw)
+        assert torch.equal(ids[sure], want[sure])
+        # rounded once to float32; the weight itself good to 2^-45 of the largest
+        bound = 2.0 ** -23 * lp.abs() + 2.0 ** -44 * torch.exp((-lp).clamp_max(30.0))
+        assert ((logp.double() - lp).abs() <= bound)[sure].all()
+
+
+def rand(rows, vocab, seed, dtype=torch.float32, spread=2.0, pad=0):
+    """Rows ``vocab + pad`` apart, starting ``pad`` elements into their memory."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    z = (spread * torch.randn(rows, vocab + pad, generator=g, device=DEV)).to(dtype)[:, pad:]
+    return z, torch.rand(rows, generator=g, device=DEV)
+
+
+WAYS = [dict(), dict(min_p=0.001), dict(top_p=0.9), dict(top_p=0.97, min_p=0.0005, temperature=1.5), dict(top_k=600),
+        dict(top_k=40, top_p=0.9)]
+
+
+@pytest.mark.parametrize("kw", WAYS, ids=str)
+@pytest.mark.parametrize("rows,vocab", [(1, 70000), (18, 33000), (19, 50257), (36, 20000), (37, 40000), (73, 50257),
+                                        (74, 9000), (100, 50257), (147, 9000), (60, 8200)])
+def test_rows_on_clusters_of_every_size(rows, vocab, kw):
+    for seed in range(3):
+        check(*rand(rows, vocab, seed + rows), **kw)

@@ -121,9 +121,10 @@ struct SampleShared {
   };
   u64 w_keep[kSampleWarps], w_all[kSampleWarps], scratch[kSampleWarps], step[32], add[8];
   double w_sum[kSampleWarps];
-  // what other CTAs of the cluster read
+  // what other CTAs of the cluster read; each sum of a phase has a place of its own,
+  // since a CTA may be a phase ahead of one that still reads
   u64 cta_keep, cta_all, cta_ties;
-  double cta_sum;
+  double cta_bound, cta_z, cta_tail;
   uint32_t cta_max, n, key_lo, key_hi;  // key_lo, key_hi: of the tokens at the border
   // what the CTA that finds it writes into every CTA
   int tie_index, uncertain;
@@ -338,7 +339,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       if (tid == 0) {
         double s = 0.0;
         for (int w = 0; w < NW; ++w) s += sh.w_sum[w];
-        sh.cta_sum = s;
+        sh.cta_bound = s;
       }
     }
   }
@@ -361,7 +362,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
 #pragma unroll
     for (int r = 0; r < CS; ++r) {
       const float f = key_float(peer(r)->cta_max);
-      if (f > -CUDART_INF_F) z_low += (float)peer(r)->cta_sum * ex2_f32((f - m) * cf);
+      if (f > -CUDART_INF_F) z_low += (float)peer(r)->cta_bound * ex2_f32((f - m) * cf);
     }
     // Z is at most that sum times the elements behind one of the maxima (of the
     // longest part: every CTA needs the same bound)
@@ -837,7 +838,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     if (tid == 0) {
       double s = 0.0;
       for (int w = 0; w < NW; ++w) s += sh.w_sum[w];
-      sh.cta_sum = s;
+      sh.cta_z = s;
     }
     all_sync();
     int blo, bhi;
@@ -847,7 +848,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       uint32_t h0 = 0, h1 = 0;
 #pragma unroll
       for (int r = 0; r < CS; ++r) {
-        z += peer(r)->cta_sum;
+        z += peer(r)->cta_z;
         const uint2 h = *reinterpret_cast<const uint2*>(&peer(r)->p.hist[2 * tid]);
         h0 += h.x;
         h1 += h.y;
@@ -1004,7 +1005,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       u64 k = 0, al = 0;
       double s = 0.0;
       for (int w = 0; w < NW; ++w) k += sh.w_keep[w], al += sh.w_all[w], s += sh.w_sum[w];
-      sh.cta_keep = k, sh.cta_all = al, sh.cta_sum = s;
+      sh.cta_keep = k, sh.cta_all = al, sh.cta_tail = s;
     }
     all_sync();
     u64 above = 0, own = 0;
@@ -1019,7 +1020,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       key_hi = max(key_hi, q->key_hi);
       keep_of[r] = q->cta_keep;
       above += q->cta_all;
-      tl += q->cta_sum;
+      tl += q->cta_tail;
       const unsigned k = q->n;
       if (tid >= n && tid < n + k && k <= kCands) own = q->p.cand[tid - n], src = r;
       n += k;
@@ -1034,12 +1035,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       if (tid == 0) {
         double s = 0.0;
         for (int w = 0; w < NW; ++w) s += sh.w_sum[w];
-        sh.cta_sum = s;
+        sh.cta_tail = s;
       }
       all_sync();
       tl = 0.0;
 #pragma unroll
-      for (int r = 0; r < CS; ++r) tl += peer(r)->cta_sum;
+      for (int r = 0; r < CS; ++r) tl += peer(r)->cta_tail;
       te = 0.0;
     };
     // bounds of the mass that has to come before a token for it to be dropped, `in` being the bins' own mass
