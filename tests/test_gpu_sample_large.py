@@ -69,3 +69,14 @@ WAYS = [dict(), dict(min_p=0.001), dict(top_p=0.9), dict(top_p=0.97, min_p=0.000
 def test_rows_on_clusters_of_every_size(rows, vocab, kw):
     for seed in range(3):
         check(*rand(rows, vocab, seed + rows), **kw)
+
+
+@pytest.mark.parametrize("kw", WAYS, ids=str)
+@pytest.mark.parametrize("rows,vocab,dtype,pad", [
+    (150, 65537, torch.float32, 0), (150, 65536, torch.float32, 1), (150, 65534, torch.float32, 3),
+    (150, 128256, torch.float32, 0), (100, 151936, torch.float32, 0), (150, 151936, torch.bfloat16, 0),
+    (150, 131066, torch.float16, 7), (148, 1 << 18, torch.float32, 1), (148, 1 << 18, torch.bfloat16, 0),
+    (80, 1 << 18, torch.float16, 3), (40, 1 << 18, torch.float32, 3)])
+def test_many_rows_of_large_vocabularies(rows, vocab, dtype, pad, kw):
+    """Parts of up to 129 steps per warp, also of rows that start off a 16-byte boundary."""
+    check(*rand(rows, vocab, vocab + rows, dtype, pad=pad), **kw)

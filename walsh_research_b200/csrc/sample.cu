@@ -29,10 +29,10 @@
 #include "common.cuh"
 #include "mma.cuh"
 #include "paged.cuh"
+#include "sample_plan.h"
 
 namespace walsh {
 
-constexpr int kSampleMaxVocab = 1 << 18;
 constexpr double kWeightOne = 17592186044416.0;  // 2^44
 
 template <typename T>
@@ -92,7 +92,6 @@ __device__ __forceinline__ double weight(float l, float m, double c) {
 }
 __device__ __forceinline__ u64 fixed(double w) { return __double2ull_rn(w * kWeightOne); }
 
-constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 constexpr int kBins = 1024;      // bins of the mass histogram
 constexpr int kCands = 256;      // tokens resolved one by one at a top-p border
 constexpr int kList = 1024;      // tokens of a top-k list
@@ -119,7 +118,7 @@ struct SampleShared {
       };
     } p;
   };
-  u64 w_keep[kSampleWarps], w_all[kSampleWarps], scratch[kSampleWarps], step[32], add[8];
+  u64 w_keep[kSampleWarps], w_all[kSampleWarps], scratch[kSampleWarps], step[kSampleSteps], add[8];
   double w_sum[kSampleWarps];
   // what other CTAs of the cluster read; each sum of a phase has a place of its own,
   // since a CTA may be a phase ahead of one that still reads
@@ -172,9 +171,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   // ---- the row's part of this CTA; chunks of 16 bytes, `mis` elements before the row's first chunk boundary
   const T* lg = a.logits + (int64_t)row * a.ld;
   const int mis = (int)(((uintptr_t)lg & 15) / sizeof(T));
-  const int chunks = (mis + V + VEC - 1) / VEC, per_cta = (chunks + CS - 1) / CS;
+  const int chunks = sample_chunks(V, mis, VEC), per_cta = sample_cta_chunks(chunks, CS);
   const int c0 = rank * per_cta, nch = max(0, min(per_cta, chunks - c0));
-  const int per_warp = max(1, (nch + NW - 1) / NW);
+  const int per_warp = sample_warp_chunks(nch);
   const int wbeg = min(nch, warp * per_warp), wend = min(nch, wbeg + per_warp);
   const int base = c0 * VEC - mis;  // token of the part's first element (negative: before the row)
   float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
@@ -366,7 +365,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
     // Z is at most that sum times the elements behind one of the maxima (of the
     // longest part: every CTA needs the same bound)
-    const int steps = ((per_cta + NW - 1) / NW + 31) / 32;
+    const int steps = sample_steps(sample_warp_chunks(per_cta));
     z_high = fminf(z_high, fmaxf(z_low, 1.f) * 1.001f * (float)(steps * (VEC / 2)));
     z_low = fmaxf(z_low * 0.999f, 1.f);
   }
@@ -612,7 +611,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
     const u64 target = drawn_mass(z);
     if (target >= mine0 && target < mine0 + mine) {
-      auto find = [&](u64 v, u64* at) {  // first lane whose running sum from *at exceeds the target (32: none)
+      auto find = [&](u64 v, u64* at) {  // first lane whose running sum from *at exceeds the target (32: none, all added)
         u64 incl = v;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -620,15 +619,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
           if (lane >= o) incl += y;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, *at + incl > target);
-        if (!hit) return 32;
-        const int l = __ffs(hit) - 1;
-        *at += __shfl_sync(0xffffffffu, incl - v, l);
+        const int l = hit ? __ffs(hit) - 1 : 32;
+        *at += __shfl_sync(0xffffffffu, hit ? incl - v : incl, hit ? l : 31);
         return l;
       };
       u64 at = mine0;
       const int hw = find(lane < NW ? sh.w_keep[lane] : 0, &at);
       const int hb = min(nch, hw * per_warp), he = min(nch, hb + per_warp);
-      const int steps = (he - hb + 31) / 32;
+      const int steps = sample_steps(he - hb);
       u64 w[VEC], sum = 0;
       auto weigh = [&](int s) {
         const int ch = hb + 32 * s + lane;
@@ -652,8 +650,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         if (lane == 0) sh.step[s] = t;
       }
       __syncthreads();
-      const int hs = find(lane < steps ? sh.step[lane] : 0, &at);
-      if (hs == 32 || hw == 32) {  // the approximate sums of the two walks differ by their rounding
+      int hs = 0, in = 32;  // the step that holds it is hs + in
+      for (; hs < steps; hs += 32)
+        if ((in = find(hs + lane < steps ? sh.step[hs + lane] : 0, &at)) < 32) break;
+      hs += in;
+      if (in == 32 || hw == 32) {  // the approximate sums of the two walks differ by their rounding
         if (tid == 0)
           for (int r = 0; r < CS; ++r) peer(r)->uncertain = 1;
       } else if (hs % NW == warp) {
@@ -1296,22 +1297,11 @@ static int launch_sample_as(const SampleArgs<T>& a, int part, cudaStream_t s) {
 template <typename T, int CS>
 static int launch_sample(const SampleArgs<T>& a, cudaStream_t s) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  const int part = ((VEC - 1 + a.vocab + VEC - 1) / VEC + CS - 1) / CS * 16;
-  constexpr int most = (kSampleMaxVocab / VEC + 1 + CS - 1) / CS * 16;  // of any vocabulary
+  const int part = sample_cta_chunks(sample_chunks(a.vocab, VEC - 1, VEC), CS) * 16;
+  constexpr int most = sample_cta_chunks(sample_chunks(kSampleMaxVocab, VEC - 1, VEC), CS) * 16;  // of any vocabulary
   if constexpr (most > kStageBytes)
     if (part > kStageBytes) return launch_sample_as<T, CS, false>(a, part, s);
   return launch_sample_as<T, CS, true>(a, part, s);
-}
-
-// CTAs per row: one when the rows alone occupy every SM (the barriers and scalar
-// steps of a row are paid per CTA), else more while a thread still has eight
-// tokens.  Rows of 50257 tokens: 64 in float32 with top-p 26.5 us on 4 CTAs each
-// (53 on 8); 256 in float32 72.8 us on one, read again from L2, 70.7 on two,
-// held; with top-k 50 31.9 and 43.2 us; 256 in bf16 56.4 us on one, held.
-static int sample_cluster(int64_t rows, int vocab) {
-  int cs = 1;
-  while (cs < 8 && rows * cs < 148 && vocab / cs > kSampleThreads * 8) cs *= 2;
-  return cs;
 }
 
 }  // namespace walsh
