@@ -588,6 +588,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const float x = q[lane], y = q[32 + lane];
         __syncwarp();
         q[lane] = y;
+        __syncwarp();  // before other lanes append over it
         fill -= 32;
         f(x);
       }
@@ -945,6 +946,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
             __syncwarp();
             q[lane] = v1;
             qt[lane] = t1;
+            __syncwarp();  // before other lanes append over it
             fill -= 32;
             take(v0, t0, true);
           }
