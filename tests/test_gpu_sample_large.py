@@ -1,8 +1,12 @@
 """Token sampling of batches of large vocabularies: every layout of a row over
 CTAs, against the definition in float64."""
+from fractions import Fraction
+
+import numpy as np
 import pytest
 import torch
 
+import serving_reference as R
 from walsh_research_b200 import ops
 
 pytestmark = pytest.mark.gpu
@@ -80,3 +84,23 @@ def test_rows_on_clusters_of_every_size(rows, vocab, kw):
 def test_many_rows_of_large_vocabularies(rows, vocab, dtype, pad, kw):
     """Parts of up to 129 steps per warp, also of rows that start off a 16-byte boundary."""
     check(*rand(rows, vocab, vocab + rows, dtype, pad=pad), **kw)
+
+
+@pytest.mark.parametrize("rows", [1, 150])
+@pytest.mark.parametrize("step", [1e-3, 1e-6])
+def test_top_p_within_a_hair_of_a_token(rows, step):
+    """top_p a relative 1.5e-11 to either side of the mass before a token, which
+    60000 equal tokens behind the border decide.  Weights are multiples of 2^-44
+    of the largest, so the reach is good to 60300 * 2^-45 of a mass of over 340:
+    5e-12.  u draws the last token that stays (its share is over 2^-9, u is 1 -
+    2^-24)."""
+    z = torch.cat((-step * torch.arange(300), torch.full((60000,), -9.49 * 0.6931472)))
+    w = [int(x) for x in np.rint(np.exp(z.double().numpy()) * 2.0 ** 60)]
+    logits = z.to(DEV).expand(rows, -1)
+    u = torch.full((rows,), 1 - 2.0 ** -24, device=DEV)
+    for r in (2, 40, 111, 250, 299):
+        p = float(Fraction(sum(w[:r]), sum(w)))
+        for side, last in ((1 - 1.5e-11, r - 1), (1 + 1.5e-11, r)):
+            assert R.sample_row(z.double().numpy(), 1 - 2.0 ** -24, top_p=p * side)[0] == last
+            ids = ops.sample_tokens(logits, u, top_p=p * side)
+            assert (ids == last).all(), (r, side > 1, ids[0].item())

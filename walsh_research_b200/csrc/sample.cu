@@ -684,24 +684,30 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const double w = weight(v, m, c);
     return w >= min_p ? fixed(w) : 0;
   };
+  // exact mass of this thread's tokens for which want(value) holds: no packing, independent exponentials
+  auto mass_of = [&](auto want) -> u64 {
+    u64 acc = 0;
+    uint4 next = chunk(wbeg + lane, wend);
+    for (int ch = wbeg + lane; ch < wend; ch += 32) {
+      const uint4 raw = next;
+      next = chunk(ch + 32, wend);
+      const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll 1
+      for (int h = 0; h < VEC; h += 4)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float v = VEC == 4 || h == 0 ? to_f(e[j]) : to_f(e[VEC - 4 + j]);
+          const double x = fmin(((double)m - (double)v) * c, 60.0);
+          const u64 f = fixed(exp2_neg(x));
+          acc += !want(v) ? 0 : v == m ? (u64)kWeightOne : x < 60.0 ? f : 0;
+        }
+    }
+    return acc;
+  };
   auto draw_exact = [&](u64 thr) {
     u64 acc = 0;
-    if (thr == 0 && min_p <= 0.0) {  // every token: no packing, independent exponentials
-      uint4 next = chunk(wbeg + lane, wend);
-      for (int ch = wbeg + lane; ch < wend; ch += 32) {
-        const uint4 raw = next;
-        next = chunk(ch + 32, wend);
-        const T* e = reinterpret_cast<const T*>(&raw);
-#pragma unroll 1
-        for (int h = 0; h < VEC; h += 4)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float v = VEC == 4 || h == 0 ? to_f(e[j]) : to_f(e[VEC - 4 + j]);
-            const double x = fmin(((double)m - (double)v) * c, 60.0);
-            const u64 f = fixed(exp2_neg(x));
-            acc += v == m ? (u64)kWeightOne : x < 60.0 ? f : 0;
-          }
-      }
+    if (thr == 0 && min_p <= 0.0) {
+      acc = mass_of([](float) { return true; });
     } else {
       packed([&](float v, int t) { return composite(v, t) >= thr; }, [&](float v) { acc += exact_of(v); });
     }
@@ -956,9 +962,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       take(q[lane], qt[lane], lane < fill);
       __syncwarp();
     };
-    // the tail once more with an error below 2^-31 of it: independent Taylor series
+    // the tail once more with an error below 1e-9 of it: independent Taylor series
     // of degree 8 in double (the first dropped term is (ln 2 / 2)^9 / 9! = 2e-10)
-    auto exact_tail_sum = [&]() -> double {
+    auto fine_tail_sum = [&]() -> double {
       const double mc = (double)m * c;
       double acc = 0.0;
       uint4 next = chunk(wbeg + lane, wend);
@@ -1029,9 +1035,9 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       n += k;
     }
     double te = sum_error(tl, x_end);
-    // the tail exactly, on demand: the same answer in every CTA
+    // the tail to 1e-9 of it, on demand: the same answer in every CTA
     auto refine_tail = [&]() {
-      const double mine = exact_tail_sum();
+      const double mine = fine_tail_sum();
       all_sync();  // (every CTA has read the sums)
       if (lane == 0) sh.w_sum[warp] = mine;
       __syncthreads();
@@ -1046,8 +1052,22 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       for (int r = 0; r < CS; ++r) tl += peer(r)->cta_tail;
       te = 0.0;
     };
-    // bounds of the mass that has to come before a token for it to be dropped, `in` being the bins' own mass
+    // and exactly
+    bool exact_tail = false;
+    u64 tail_mass = 0;
+    auto take_tail = [&]() {
+      const u64 mine = block_sum(mass_of([&](float v) { return bin_at(v) >= edge_hi; }));
+      all_sync();  // (every CTA has read what cta_all held)
+      if (tid == 0) sh.cta_all = mine;
+      all_sync();
+#pragma unroll
+      for (int r = 0; r < CS; ++r) tail_mass += peer(r)->cta_all;
+      exact_tail = true;
+    };
+    // the mass that has to come before a token for it to be dropped, `in` being the
+    // bins' own mass; sign -1, 1: bounds of it
     auto reach_of = [&](u64 in, double sign) {
+      if (exact_tail) return top_p * (double)(above + in + tail_mass);
       return top_p * ((double)(above + in) + (tl + sign * te) * kWeightOne * (1.0 + sign * 1e-9) + sign * V);
     };
     bool resolved = false;
@@ -1079,12 +1099,20 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       }
       const bool first = above == 0 && rk == 0;  // the most likely token stays
       before += above;
-      if (__syncthreads_or(have && ((double)before < reach_of(cands, -1.0)) != ((double)before < reach_of(cands, 1.0))))
+      // does the error of the tail matter to this token, or to the bins?
+      const double all_in = (double)(above + cands);
+      auto unsure = [&]() {
+        const double lo = reach_of(cands, -1.0), hi = reach_of(cands, 1.0);
+        return __syncthreads_or((have && ((double)before < lo) != ((double)before < hi)) || (all_in >= lo) != (all_in >= hi));
+      };
+      if (unsure()) {
         refine_tail();
-      const double reach = top_p * ((double)(above + cands) + tl * kWeightOne);
+        if (unsure()) take_tail();
+      }
+      const double reach = reach_of(cands, 0.0);
       const bool keep = have && (first || (double)before < reach);
       // the border does lie in these bins (their histogram is approximate)
-      if ((above == 0 || (double)above < reach) && (double)(above + cands) >= reach) {
+      if ((above == 0 || (double)above < reach) && all_in >= reach) {
         // threshold: the last kept token, or just above the first of them
         const unsigned kept = block_sum32(keep && part == 0);
         if (part == 0 && have && (kept ? rk == kept - 1 : rk == 0)) sh.thr = kept ? mine : mine + 1;
@@ -1107,19 +1135,19 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       return;
     }
     if (n > kCands) {  // too many to rank: the border key is sought among theirs, with exact sums
-      many = true;
-      refine_tail();
+      take_tail();
       u64 in = 0;
       packed([&](float v, int) { const uint32_t k = float_key(v + 0.f); return k >= key_lo && k <= key_hi; },
              [&](float v) { in += fixed(weight(v, m, c)); });
       in = block_sum(in);
+      all_sync();  // (and the tail)
       if (tid == 0) sh.cta_all = in;
       all_sync();
       in = 0;
 #pragma unroll
       for (int r = 0; r < CS; ++r) in += peer(r)->cta_all;
       m_lo = key_lo, m_hi = key_hi, m_above = above;
-      m_reach = top_p * ((double)(above + in) + tl * kWeightOne);
+      m_reach = reach_of(in, 0.0);
       many = (above == 0 || (double)above < m_reach) && (double)(above + in) >= m_reach;  // (or the bins were wrong)
     }
     all_sync();
