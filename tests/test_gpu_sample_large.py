@@ -104,3 +104,20 @@ def test_top_p_within_a_hair_of_a_token(rows, step):
             assert R.sample_row(z.double().numpy(), 1 - 2.0 ** -24, top_p=p * side)[0] == last
             ids = ops.sample_tokens(logits, u, top_p=p * side)
             assert (ids == last).all(), (r, side > 1, ids[0].item())
+
+
+@pytest.mark.parametrize("t", [float("inf"), 3e38, 1.2e38, 2e37, 1e-45])
+@pytest.mark.parametrize("kw", [dict(), dict(top_p=0.8), dict(min_p=0.2), dict(top_k=600, top_p=0.9)], ids=str)
+def test_temperatures_and_differences_at_the_ends_of_float32(t, kw):
+    """Differences of logits past float32's range, or of its smallest steps, and
+    temperatures that still weigh them: +-3e38 at 1.2e38 is a weight of e^-5."""
+    g = torch.Generator().manual_seed(21)
+    if t > 1:
+        z = 3e38 * (2 * torch.rand(24, 700, generator=g) - 1)
+    else:
+        z = torch.randint(0, 6, (24, 700), generator=g).float() * 2.0 ** -149
+    u = torch.rand(24, generator=g)
+    ids = ops.sample_tokens(z.to(DEV), u.to(DEV), temperature=t, **kw).tolist()
+    want = [R.sample_row(z[r].double().numpy(), float(u[r]), t, kw.get("top_k", 0), kw.get("top_p", 1.0),
+                         kw.get("min_p", 0.0))[0] for r in range(24)]
+    assert ids == want

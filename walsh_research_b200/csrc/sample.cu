@@ -164,9 +164,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   int top_k = a.top_k_r ? a.top_k_r[row] : a.top_k;
   if (top_k <= 0 || top_k > V) top_k = V;
   const bool greedy = !(temp > 0.0) || top_k == 1;
-  const bool by_list = top_k < V && top_k <= kListTopK, by_mass = top_k == V && top_p < 1.0;
   const double c = temp > 0.0 ? 1.4426950408889634074 / temp : 1.0;
-  const float cf = fminf(fmaxf((float)c, 1.2e-38f), 3e38f);
+  const float cf = (float)c;
+  // float32 weights only where neither c nor a difference of logits that still weighs (60 / c) may leave float32
+  const bool approx = c >= 1e-36 && c <= 3e38;
+  const bool by_list = top_k < V && top_k <= kListTopK, by_mass = top_k == V && top_p < 1.0 && approx;
 
   // ---- the row's part of this CTA; chunks of 16 bytes, `mis` elements before the row's first chunk boundary
   const T* lg = a.logits + (int64_t)row * a.ld;
@@ -355,7 +357,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     all_sync();
     return;
   }
-  bool general = top_k < V && !by_list;
+  bool general = top_k < V ? !by_list : top_p < 1.0 && !by_mass;
   float z_low = 0.f, z_high = (float)V;
   if (by_mass) {
 #pragma unroll
@@ -742,7 +744,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     // farther from the token's borders than their error, else from exact ones;
     // a log probability needs the exact sum anyway
     // ---------------------------------------------------------------------
-    if (a.logp) {
+    if (a.logp || !approx) {
       draw_exact(0);
       return;
     }
