@@ -116,3 +116,20 @@ def test_batches_of_nothing_or_of_removed_sequences_are_refused():
         with pytest.raises(ValueError):
             what()
     assert c.free_pages == 9 and c.lengths([b]) == [3]
+
+
+def test_a_batch_of_a_removed_sequence_is_refused_although_its_row_is_in_use_again():
+    c = make()
+    a = c.add()
+    old = c.select(a)
+    c.remove(a)
+    b = c.add()
+    assert a == b                                          # the row is handed out again
+    for call in (lambda: old.begin(2), lambda: old.increment(2)):
+        with pytest.raises(ValueError, match="removed"):
+            call()
+    assert c.lengths(b) == [0] and c.free_pages == 10
+    new = c.select(b)
+    new.begin(2)
+    new.increment(2)
+    assert c.lengths(b) == [2]

@@ -46,6 +46,7 @@ class PagedKVCache:
         self._table = np.full((max_seqs, -(-max_seq_len // page_size)), -1, dtype=np.int32)
         self._len = np.zeros(max_seqs, dtype=np.int64)
         self._used = np.zeros(max_seqs, dtype=bool)
+        self._removed = np.zeros(max_seqs, dtype=np.int64)  # sequences removed from each row, which add() hands out again
 
     def add(self, n: int = 1) -> List[int]:
         """``n`` new empty sequences."""
@@ -63,6 +64,7 @@ class PagedKVCache:
             self._free.extend(int(p) for p in row[row >= 0])
             row[:] = -1
             self._used[s] = False
+            self._removed[s] += 1
             self._rows.append(int(s))
 
     def lengths(self, seqs: Sequence[int]) -> List[int]:
@@ -122,12 +124,17 @@ class PagedBatch:
     def __init__(self, cache: PagedKVCache, ids: np.ndarray):
         self.cache, self.ids = cache, ids
         self.batch_size, self.dtype = len(ids), cache.dtype
+        self._removed = cache._removed[ids]
+
+    def _check(self):
+        if (self.cache._removed[self.ids] != self._removed).any():
+            raise ValueError("some of the batch's sequences were removed since it was selected")
 
     def increment(self, n: int = 1):
         """Counts the ``n`` tokens per sequence that the last forward stored."""
         if n < 0:
             raise ValueError(f"stored tokens cannot be taken back, got {n}")
-        self.cache._ids(self.ids)  # none of them removed since
+        self._check()
         self.cache._reserve(self.ids, n)
         self.cache._advance(self.ids, n)
 
@@ -136,7 +143,7 @@ class PagedBatch:
         c, ids = self.cache, self.ids
         if n < 1 or not len(ids):
             raise ValueError(f"a forward needs sequences and tokens, got {len(ids)} of {n} tokens")
-        c._ids(ids)  # none of them removed since the selection
+        self._check()
         c._reserve(ids, n)
         B, ps = len(ids), c.page_size
         pos = c._len[ids][:, None] + np.arange(n)[None]
