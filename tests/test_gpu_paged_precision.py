@@ -78,3 +78,15 @@ def test_decode_keeps_probabilities_in_two_terms(dtype, hq, hk, hd):
         for b, n in enumerate(lens):
             k, v = (R.gather_keys(p, table[b], n) for p in (kp, vp))
             close(out[b:b + 1], *attend(q[b:b + 1], k, v, n - 1, window, sinks))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_limits_past_31_bits_see_everything(dtype):
+    g = gen(4)
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [50, 7], 2, 16, 32, dtype))
+    q = torch.randn(2, 4, 32, generator=g).to(dtype).to(DEV)
+    off = torch.arange(3, dtype=torch.int32, device=DEV)
+    want = ops.paged_attention(q, kp, vp, table, kl), ops.paged_prefill_attention(q, off, kp, vp, table, kl)
+    for kw in (dict(window=2 ** 31 - 1), dict(window=2 ** 40), dict(window=3, sinks=2 ** 31), dict(window=2 ** 31, sinks=2 ** 33)):
+        assert torch.equal(ops.paged_attention(q, kp, vp, table, kl, max_len=2 ** 40, **kw), want[0])
+        assert torch.equal(ops.paged_prefill_attention(q, off, kp, vp, table, kl, **kw), want[1])

@@ -196,3 +196,19 @@ def test_calls_run_on_the_tensors_device(monkeypatch):
     ops._call_on(0, "x", 1)
     ops._call_on(3, "y", 2)
     assert log == [("x", 1, 77), ("enter", 3), ("y", 2, 77), ("exit", 3)]
+
+
+def test_windows_sinks_and_bounds_past_31_bits_reach_the_kernel(monkeypatch):
+    """2^31 and more mean no limit: clamped alike for the call and its scratch."""
+    calls = []
+    monkeypatch.setattr(ops, "_device_of", lambda *t: 0)
+    monkeypatch.setattr(ops, "_call_on", lambda dev, name, *args: calls.append((name, args)))
+    kp = torch.zeros(4, 2, 8, 16)
+    table, lens = torch.zeros(1, 4, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
+    for kw in (dict(window=2 ** 40), dict(window=5, sinks=2 ** 31), dict(max_len=2 ** 40), dict(max_len=2 ** 32 + 1),
+               dict(window=2 ** 31 - 1, sinks=2 ** 35, max_len=2 ** 31)):
+        ops.paged_attention(torch.zeros(1, 2, 16), kp, kp, table, lens, **kw)
+        name, args = calls.pop()
+        assert name == "walsh_paged_attn_fwd" and args[6] == min(kw.get("max_len", 32), 32)  # what the table holds
+        f = dict(zip(("window", "sinks"), _lib.PAGED_KV.unpack(args[0])[14:16]))
+        assert all(f[k] == min(kw.get(k, 0), 2 ** 31 - 1) for k in f)

@@ -623,6 +623,7 @@ def _head_rows(x, heads, hd, dtype, what):
     return x, p, n, h, st, sh
 
 
+_INT_MAX = 0x7fffffff  # windows and sinks from here on see everything
 _INT32 = (torch.int32,)
 _INTS = (torch.int32, torch.int64)
 
@@ -676,7 +677,7 @@ def _paged_kv(k_pages, v_pages, page_table=None, kv_lens=None, window=0, sinks=0
             scale = hd ** -0.5
     return _lib.PAGED_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), dcode(dtype), n, h, ps, hd,
                               sp if n > 1 else 0, sh if h > 1 else 0, sr if ps > 1 else hd, tab, ts, cols, lens,
-                              min(window, 0x7fffffff), min(sinks, 0x7fffffff), scale or 0.0, e)
+                              min(window, _INT_MAX), min(sinks, _INT_MAX), scale or 0.0, e)
 
 
 def paged_append(q, k, v, k_pages, v_pages, slots, positions=None, rope=None, q_norm=None, k_norm=None, eps=1e-6,
@@ -759,6 +760,7 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, wind
     when a page id or length is out of range; keys of such a page are not
     seen."""
     dev = _device_of(k_pages, v_pages, q, page_table, kv_lens, out, err)
+    window, sinks = min(window, _INT_MAX), min(sinks, _INT_MAX)
     kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
     _, hk, ps, hd = k_pages.shape
     q, qp, B, hq, q_bs, q_hs = _head_rows(q, None, hd, k_pages.dtype, "q")
@@ -767,9 +769,8 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, wind
     out = _out_rows(out, q, (B, hq, hd))
     if B == 0:
         return out
-    if max_len is None:
-        max_len = page_table.shape[1] * ps
-    max_len = int(max_len)
+    held = page_table.shape[1] * ps
+    max_len = held if max_len is None else min(int(max_len), held)
     nbytes = _attn_scratch_bytes(dcode(q.dtype), hk, hd, window, sinks, B, hq, max_len)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes > 0 else None
     _call_on(dev, "walsh_paged_attn_fwd", kv, qp, q_bs, q_hs, B, hq, max_len, ptr(scratch), out.data_ptr())
