@@ -212,3 +212,16 @@ def test_windows_sinks_and_bounds_past_31_bits_reach_the_kernel(monkeypatch):
         assert name == "walsh_paged_attn_fwd" and args[6] == min(kw.get("max_len", 32), 32)  # what the table holds
         f = dict(zip(("window", "sinks"), _lib.PAGED_KV.unpack(args[0])[14:16]))
         assert all(f[k] == min(kw.get(k, 0), 2 ** 31 - 1) for k in f)
+
+
+@pytest.mark.parametrize("dtype,hq,hk,hd,B", [(0, 8, 8, 128, 8192), (0, 32, 1, 128, 2 ** 20), (2, 64, 64, 128, 2 ** 20 - 1),
+                                              (2, 1024, 1024, 16, 65535), (1, 40, 2, 64, 10 ** 6)])
+def test_the_largest_decode_grid_counts_in_31_bits(dtype, hq, hk, hd, B):
+    """The CTAs of a call (units times the ranges its scratch is for) for a bound of 2^31 - 1 keys."""
+    k = kv(dtype=dtype, kv_heads=hk, head_dim=hd, page_size=2 ** 20, table_cols=2047, page_stride=2 ** 20 * hd * hk,
+           head_stride=2 ** 20 * hd, row_stride=hd)
+    nbytes = _lib.lib().walsh_paged_attn_scratch_bytes(k, B, hq, 2 ** 31 - 1)
+    per_range = B * hq * (hd + 2) * 4
+    assert nbytes > 0 and nbytes % per_range == 0
+    group, tile = hq // hk, 4 if dtype == 0 else 8 if hq // hk <= 8 else 16
+    assert B * hk * -(-group // tile) * (nbytes // per_range) < 2 ** 31

@@ -611,6 +611,7 @@ static DecodePlan decode_plan(const walsh_paged_kv* kv, int B, int q_heads, int 
   int64_t split = units > 0 ? ctas / units : 1;
   if (split < bytes / kRangeBytes) split = bytes / kRangeBytes;
   split = min64(split, bytes / kRangeLeast);
+  if (units > 0) split = min64(split, ((1ll << 31) - 1) / units);  // the grid counts CTAs in 31 bits
   p.nsplit = p.warps == 1 || split < 1 ? 1 : (int)split;
   p.chunk = (int)((n + p.nsplit - 1) / p.nsplit);
   if (p.chunk < 1) p.chunk = 1;
