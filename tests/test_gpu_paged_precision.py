@@ -90,3 +90,23 @@ def test_limits_past_31_bits_see_everything(dtype):
     for kw in (dict(window=2 ** 31 - 1), dict(window=2 ** 40), dict(window=3, sinks=2 ** 31), dict(window=2 ** 31, sinks=2 ** 33)):
         assert torch.equal(ops.paged_attention(q, kp, vp, table, kl, max_len=2 ** 40, **kw), want[0])
         assert torch.equal(ops.paged_prefill_attention(q, off, kp, vp, table, kl, **kw), want[1])
+
+
+def test_positions_past_32_bits_are_reported_whatever_the_slots_type():
+    n, h, hd, page = 4, 2, 16, 4
+    x = torch.ones(n, h, hd, dtype=torch.float16, device=DEV)
+    t = torch.ones(3, hd // 2, device=DEV)
+    pos = torch.tensor([0, 2 ** 32 + 1, 2, -2 ** 32], device=DEV)
+    for slots in (torch.tensor([0, 1, 2, 3], dtype=i, device=DEV) for i in (torch.int32, torch.int64)):
+        kp = torch.zeros(1, h, page, hd, dtype=torch.float16, device=DEV)
+        vp = torch.zeros_like(kp)
+        err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        q = ops.paged_append(x, x, x, kp, vp, slots, positions=pos, rope=(t, t * 0), err=err)
+        assert int(err) == -9
+        for y in (q, kp[0].transpose(0, 1), vp[0].transpose(0, 1)):
+            assert (y[[0, 2]] == 1).all() and not y[[1, 3]].any()
+    # and slots past 32 bits beside int32 positions
+    err.zero_()
+    slots = torch.tensor([0, 2 ** 32 + 1, 2, 3], device=DEV)
+    ops.paged_append(None, x, 2 * x, kp, vp, slots, positions=torch.zeros(n, dtype=torch.int32, device=DEV), rope=(t, t * 0), err=err)
+    assert int(err) == -9 and (vp[0, :, [0, 2, 3]] == 2).all() and not vp[0, :, 1].any()

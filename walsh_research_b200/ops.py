@@ -715,8 +715,8 @@ def paged_append(q, k, v, k_pages, v_pages, slots, positions=None, rope=None, q_
     slots = _index_vector(slots, n, "slots", _INTS)
     if positions is not None:
         positions = _index_vector(positions, n, "positions", _INTS)
-        if positions.dtype is not slots.dtype:
-            positions = positions.to(slots.dtype)
+        if positions.dtype is not slots.dtype:  # widened, never narrowed: a value past 32 bits stays out of range
+            slots, positions = slots.long(), positions.long()
         size = cos.shape
         if (len(size) != 2 or size[1] * 2 != hd or sin.shape != size or cos.dtype is not torch.float32
                 or sin.dtype is not torch.float32):
