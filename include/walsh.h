@@ -755,6 +755,12 @@ walsh_status walsh_paged_attn_fwd(const walsh_paged_kv* kv, const void* q, int64
 walsh_status walsh_paged_prefill_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts, int64_t q_hs,
                                      int64_t q_rows, const int32_t* q_offsets, int B, int q_heads, int max_q, void* o,
                                      void* stream);
+/* The same with the probabilities of 16-bit types rounded to the type once for
+ * their product with v, as in walsh_attn_fwd's 16-bit kernels (above: kept
+ * as two terms, to 2^-18 and better).  float32 is the same either way. */
+walsh_status walsh_paged_prefill_rounded_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts, int64_t q_hs,
+                                             int64_t q_rows, const int32_t* q_offsets, int B, int q_heads, int max_q,
+                                             void* o, void* stream);
 
 /* One token per row of logits [rows, vocab] (rows ld elements apart; vocab <=
  * 2^18) from the uniform numbers u [rows] in [0, 1): weights exp(l / T); the

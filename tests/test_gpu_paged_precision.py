@@ -66,6 +66,26 @@ def test_prefill_keeps_probabilities_in_two_terms(dtype, hq, hk, hd, window, sin
         at += t
 
 
+@pytest.mark.parametrize("dtype", HALF + [torch.float32])
+@pytest.mark.parametrize("hq,hk,hd", [(32, 32, 16), (4, 2, 32), (8, 1, 64), (6, 2, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (64, 3)])
+def test_prefill_with_rounded_probabilities(dtype, hq, hk, hd, window, sinks):
+    """serving_reference.attend's bound counts one rounding of each probability; float32 has none."""
+    g = gen(hd + hq)
+    new, past = [200, 70], [0, 150]
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [a + b for a, b in zip(new, past)], hk, 16, hd, dtype))
+    q = (1.5 * torch.randn(sum(new), hq, hd, generator=g)).to(dtype).to(DEV)
+    off = torch.tensor([0] + new).cumsum(0).int().to(DEV)
+    out = ops.paged_prefill_attention(q, off, kp, vp, table, kl, window=window, sinks=sinks, rounded=True)
+    if dtype is torch.float32:
+        assert torch.equal(out, ops.paged_prefill_attention(q, off, kp, vp, table, kl, window=window, sinks=sinks))
+    at = 0
+    for b, t in enumerate(new):
+        k, v = (R.gather_keys(p, table[b], past[b] + t) for p in (kp, vp))
+        close(out[at:at + t], *R.attend(q[at:at + t], k, v, past[b], window, sinks))
+        at += t
+
+
 @pytest.mark.parametrize("dtype", HALF)
 @pytest.mark.parametrize("hq,hk,hd", [(8, 8, 16), (8, 1, 64), (9, 1, 16), (16, 1, 32), (24, 2, 64), (40, 2, 128)])
 def test_decode_keeps_probabilities_in_two_terms(dtype, hq, hk, hd):

@@ -90,6 +90,7 @@ SIGNATURES = {
     "walsh_paged_attn_fwd": [P, P, c_int64, c_int64, c_int, c_int, c_int, P, P, P],
     "walsh_paged_attn_scratch_bytes": [P, c_int, c_int, c_int],
     "walsh_paged_prefill_fwd": [P, P, c_int64, c_int64, c_int64, P, c_int, c_int, c_int, P, P],
+    "walsh_paged_prefill_rounded_fwd": [P, P, c_int64, c_int64, c_int64, P, c_int, c_int, c_int, P, P],
     "walsh_sample_tokens": [P, c_int, c_int64, c_int64, c_int, P, ctypes.c_double, c_int, ctypes.c_double,
                             ctypes.c_double, P, P, P, P, P, P, P],
 }

@@ -264,13 +264,14 @@ __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArg
 // stage ahead; steps of KT keys within a stage without barriers, and only those
 // that some row of the warp sees.  Per step and warp: S - m = Q K^T - m (m is the
 // MMAs' addend), P = 2^(c (S - m)) in float32, row sums of the float32 P, and O
-// += P V with P as two 16-bit terms, P rounded to the type and what that left
-// over, rounded again: 2^-18 (bf16) or 2^-22 (fp16, down to its smallest step) of
-// each probability, below the output's own rounding.  P rounded once would save
-// half of these MMAs and the splitting (150 against 179 us in the case below, 199
-// against 256 with 32 channels), but moves two outputs of five by a step.  m, O
-// and the row sums move only when a row's maximum has grown by more than 8 powers
-// of two (P <= 2^8).
+// += P V.  TWO: P enters as two 16-bit terms, rounded to the type and what that left
+// over, rounded again: good to 2^-18 (bf16) or 2^-22 (fp16, down to its smallest
+// step) of each probability, below the output's own rounding.  Otherwise P is
+// rounded once, as in the dense attention kernels, for callers that ask for it: half
+// of these MMAs and no splitting (150 against 179 us in the case below, 199 against
+// 256 with 32 channels), but two outputs of five move by a step.  m, O and the row
+// sums move only when a row's maximum has grown by more than 8 powers of two (P <=
+// 2^8).
 // With 16 channels the exponentials are the floor (16 per clock and SM), with 32
 // they and the MMAs take the same time; instructions bound it (8 x 2048 tokens,
 // 32 heads of 16, window 512: 179 us; the floor 55).
@@ -312,7 +313,7 @@ __device__ __forceinline__ void mma_rowc<__nv_bfloat16>(float* d, const uint32_t
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c_lo), "f"(c_hi));
 }
 
-template <typename T, int HD, int W, int MT, int KT, int KS, int MINB>
+template <typename T, int HD, int W, int MT, int KT, int KS, int MINB, bool TWO>
 __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const PrefillArgs<T> a) {
   constexpr int QT = W * MT * 16, NT = W * 32, CH = HD / 8, STAGE = KS * HD;
   extern __shared__ __align__(16) unsigned char smb[];
@@ -528,8 +529,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
             thr_min = fminf(thr_min, thr[mt][h]);
           }
       }
-      // P as two 16-bit terms, O += P V with both
-      uint32_t pf[MT][KT / 16][4], pl[MT][KT / 16][4];
+      uint32_t pf[MT][KT / 16][4], pl[MT][TWO ? KT / 16 : 1][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint64_t rs0 = 0, rs1 = 0;
@@ -540,8 +540,13 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
           rs0 = f2_fma(p0, one2, rs0);
           rs1 = f2_fma(p1, one2, rs1);
           const int kk = i >> 1, j = (i & 1) * 2;
-          split_p<T>(p0, &pf[mt][kk][j], &pl[mt][kk][j]);
-          split_p<T>(p1, &pf[mt][kk][j + 1], &pl[mt][kk][j + 1]);
+          if constexpr (TWO) {
+            split_p<T>(p0, &pf[mt][kk][j], &pl[mt][kk][j]);
+            split_p<T>(p1, &pf[mt][kk][j + 1], &pl[mt][kk][j + 1]);
+          } else {
+            pf[mt][kk][j] = pack_p<T>(f2_lo(p0), f2_hi(p0));
+            pf[mt][kk][j + 1] = pack_p<T>(f2_lo(p1), f2_hi(p1));
+          }
         }
         l[mt][0] += f2_lo(rs0) + f2_hi(rs0);
         l[mt][1] += f2_lo(rs1) + f2_hi(rs1);
@@ -556,8 +561,10 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
           for (int mt = 0; mt < MT; ++mt) {
             mma16<T>(acc[mt][2 * dp], pf[mt][kk], vf[0], vf[1]);
             mma16<T>(acc[mt][2 * dp + 1], pf[mt][kk], vf[2], vf[3]);
-            mma16<T>(acc[mt][2 * dp], pl[mt][kk], vf[0], vf[1]);
-            mma16<T>(acc[mt][2 * dp + 1], pl[mt][kk], vf[2], vf[3]);
+            if constexpr (TWO) {
+              mma16<T>(acc[mt][2 * dp], pl[mt][kk], vf[0], vf[1]);
+              mma16<T>(acc[mt][2 * dp + 1], pl[mt][kk], vf[2], vf[3]);
+            }
           }
         }
     };
@@ -616,9 +623,10 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
 }
 
 template <typename T, int HD, int W, int MT, int KT, int KS, int MINB>
-static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
+static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, bool two, cudaStream_t s) {
   constexpr int smem = 4 * KS * HD * 2;
-  auto* kern = paged_prefill_mma_kernel<T, HD, W, MT, KT, KS, MINB>;
+  auto* kern = two ? paged_prefill_mma_kernel<T, HD, W, MT, KT, KS, MINB, true>
+                   : paged_prefill_mma_kernel<T, HD, W, MT, KT, KS, MINB, false>;
   if (smem > 40 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
     return launch_status();
   const int64_t tiles = ((int64_t)max_q * a.group.d + W * MT * 16 - 1) / (W * MT * 16);
@@ -627,7 +635,7 @@ static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, cudaSt
 }
 
 // Warps, 16-row tiles per warp, keys per step and per stage, CTAs per SM.
-// Measured, replayed from a graph: 16 channels (8 x 2048 tokens, 32 heads, window
+// Measured with two terms, replayed from a graph: 16 channels (8 x 2048 tokens, 32 heads, window
 // 512): (4, 1, 64, 128, 5) 179 us, (4, 1, 64, 128, 4) 178, (8, 1, 32, 256, 3) 184,
 // (4, 2, 32, 256, 4) 165, but 5.8 against 4.8 us for a few short prompts; 32
 // channels (3 later parts up to 3500, 64 heads, window 1024): (4, 2, 32, 256, 3)
@@ -636,17 +644,17 @@ static int launch_prefill_tile(const PrefillArgs<T>& a, int B, int max_q, cudaSt
 // 211; 128 (8 x 800, 16 on 2): (4, 1, 64, 64, 2) 130, (4, 1, 32, 64, 2) 131, (8, 1,
 // 64, 64, 1) 143.
 template <typename T, int HD>
-static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
-  if constexpr (HD == 16) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 5>(a, B, max_q, s);
-  else if constexpr (HD == 32) return launch_prefill_tile<T, HD, 4, 2, 32, 256, 3>(a, B, max_q, s);
-  else if constexpr (HD == 64) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 3>(a, B, max_q, s);
-  else return launch_prefill_tile<T, HD, 4, 1, 64, 64, 2>(a, B, max_q, s);
+static int launch_prefill_mma(const PrefillArgs<T>& a, int B, int max_q, bool two, cudaStream_t s) {
+  if constexpr (HD == 16) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 5>(a, B, max_q, two, s);
+  else if constexpr (HD == 32) return launch_prefill_tile<T, HD, 4, 2, 32, 256, 3>(a, B, max_q, two, s);
+  else if constexpr (HD == 64) return launch_prefill_tile<T, HD, 4, 1, 64, 128, 3>(a, B, max_q, two, s);
+  else return launch_prefill_tile<T, HD, 4, 1, 64, 64, 2>(a, B, max_q, two, s);
 }
 
 template <typename T, int HD>
-static int launch_prefill(const PrefillArgs<T>& a, int B, int max_q, cudaStream_t s) {
+static int launch_prefill(const PrefillArgs<T>& a, int B, int max_q, bool two, cudaStream_t s) {
   if constexpr (sizeof(T) == 2) {
-    return launch_prefill_mma<T, HD>(a, B, max_q, s);
+    return launch_prefill_mma<T, HD>(a, B, max_q, two, s);
   } else {
     constexpr int QT = 64, KT = HD == 128 ? 32 : 64, LD = HD + 4;
     constexpr int smem = ((QT + 2 * KT) * LD + QT * (KT + 4)) * 4;
@@ -664,9 +672,8 @@ static int launch_prefill(const PrefillArgs<T>& a, int B, int max_q, cudaStream_
 
 using namespace walsh;
 
-extern "C" walsh_status walsh_paged_prefill_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts, int64_t q_hs,
-                                                int64_t q_rows, const int32_t* q_offsets, int B, int q_heads,
-                                                int max_q, void* o, void* stream) {
+static int prefill_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts, int64_t q_hs, int64_t q_rows,
+                       const int32_t* q_offsets, int B, int q_heads, int max_q, bool two, void* o, void* stream) {
   if (int e = injected("paged_prefill_fwd")) return e;
   if (int e = check_pages(kv, true)) return e;
   WALSH_CHECK_ARG(q && q_offsets && o);
@@ -686,10 +693,22 @@ extern "C" walsh_status walsh_paged_prefill_fwd(const walsh_paged_kv* kv, const 
     a.scale_log2 = kv->scale * 1.4426950408889634f;
     cudaStream_t s = (cudaStream_t)stream;
     switch (kv->head_dim) {
-      case 16: return launch_prefill<ET, 16>(a, B, max_q, s);
-      case 32: return launch_prefill<ET, 32>(a, B, max_q, s);
-      case 64: return launch_prefill<ET, 64>(a, B, max_q, s);
-      default: return launch_prefill<ET, 128>(a, B, max_q, s);
+      case 16: return launch_prefill<ET, 16>(a, B, max_q, two, s);
+      case 32: return launch_prefill<ET, 32>(a, B, max_q, two, s);
+      case 64: return launch_prefill<ET, 64>(a, B, max_q, two, s);
+      default: return launch_prefill<ET, 128>(a, B, max_q, two, s);
     }
   }());
+}
+
+extern "C" walsh_status walsh_paged_prefill_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts, int64_t q_hs,
+                                                int64_t q_rows, const int32_t* q_offsets, int B, int q_heads,
+                                                int max_q, void* o, void* stream) {
+  return prefill_fwd(kv, q, q_ts, q_hs, q_rows, q_offsets, B, q_heads, max_q, true, o, stream);
+}
+
+extern "C" walsh_status walsh_paged_prefill_rounded_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts,
+                                                        int64_t q_hs, int64_t q_rows, const int32_t* q_offsets, int B,
+                                                        int q_heads, int max_q, void* o, void* stream) {
+  return prefill_fwd(kv, q, q_ts, q_hs, q_rows, q_offsets, B, q_heads, max_q, false, o, stream);
 }

@@ -179,5 +179,6 @@ class PagedLayer:
         kw = dict(window=c.window, sinks=c.sinks, err=c.err)
         if s.n == 1:
             return ops.paged_attention(q, self.k_pages, self.v_pages, s.page_table, s.kv_lens, max_len=s.max_len, **kw)
+        # prompts as over the dense cache, whose kernels round the probabilities once too
         return ops.paged_prefill_attention(q, s.q_offsets, self.k_pages, self.v_pages, s.page_table, s.kv_lens,
-                                           max_q=s.n, **kw)
+                                           max_q=s.n, rounded=True, **kw)

@@ -778,13 +778,15 @@ def paged_attention(q, k_pages, v_pages, page_table, kv_lens, max_len=None, wind
 
 
 def paged_prefill_attention(q, q_offsets, k_pages, v_pages, page_table, kv_lens, max_q=None, window=0, sinks=0,
-                            scale=None, out=None, err=None):
+                            scale=None, out=None, err=None, rounded=False):
     """Causal attention of several new tokens per sequence over its pages: rows
     q_offsets[b] .. q_offsets[b+1]-1 (int32 [B+1]) of q [N, Hq, hd] are the
     last tokens of sequence b, already appended (query t of T at position
     kv_len - T + t).  Pages, lengths, window, sinks, scale and err as in
     paged_attention; ``max_q`` bounds the spans on the host (default N).  Rows
-    of ``out`` outside every span are left as they are."""
+    of ``out`` outside every span are left as they are.  16-bit types keep the
+    probabilities to 2^-18 and better; ``rounded`` rounds them once to the
+    type, as ops.attention does, in three quarters of the time."""
     dev = _device_of(k_pages, v_pages, q, q_offsets, page_table, kv_lens, out, err)
     kv = _paged_kv(k_pages, v_pages, page_table, kv_lens, window, sinks, scale, err)
     hd = k_pages.shape[3]
@@ -794,8 +796,8 @@ def paged_prefill_attention(q, q_offsets, k_pages, v_pages, page_table, kv_lens,
     out = _out_rows(out, q, (n, hq, hd))
     if n == 0 or B == 0:
         return out
-    _call_on(dev, "walsh_paged_prefill_fwd", kv, qp, q_ts, q_hs, n, q_offsets.data_ptr(), B, hq,
-             n if max_q is None else min(int(max_q), n), out.data_ptr())
+    _call_on(dev, "walsh_paged_prefill_rounded_fwd" if rounded else "walsh_paged_prefill_fwd", kv, qp, q_ts, q_hs, n,
+             q_offsets.data_ptr(), B, hq, n if max_q is None else min(int(max_q), n), out.data_ptr())
     return out
 
 
