@@ -130,3 +130,15 @@ def test_positions_past_32_bits_are_reported_whatever_the_slots_type():
     slots = torch.tensor([0, 2 ** 32 + 1, 2, 3], device=DEV)
     ops.paged_append(None, x, 2 * x, kp, vp, slots, positions=torch.zeros(n, dtype=torch.int32, device=DEV), rope=(t, t * 0), err=err)
     assert int(err) == -9 and (vp[0, :, [0, 2, 3]] == 2).all() and not vp[0, :, 1].any()
+
+
+def test_prefill_bound_of_zero_still_computes_the_spans():
+    """max_q only sizes the grid; a bound that is too small is not an empty call."""
+    g = gen(6)
+    for dtype in (torch.float16, torch.float32):
+        kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [90, 7], 2, 16, 32, dtype))
+        q = torch.randn(97, 4, 32, generator=g).to(dtype).to(DEV)
+        off = torch.tensor([0, 90, 97], dtype=torch.int32, device=DEV)
+        out = torch.full_like(q, 7.0)
+        want = ops.paged_prefill_attention(q, off, kp, vp, table, kl)
+        assert torch.equal(ops.paged_prefill_attention(q, off, kp, vp, table, kl, max_q=0, out=out), want)

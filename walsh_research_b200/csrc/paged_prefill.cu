@@ -683,7 +683,8 @@ static int prefill_fwd(const walsh_paged_kv* kv, const void* q, int64_t q_ts, in
   const int64_t vec = kv->dtype == WALSH_F32 ? 4 : 8;
   WALSH_CHECK_SHAPE(q_ts >= 0 && q_hs >= 0);
   if (((((uintptr_t)q) | ((uintptr_t)o)) & 15u) != 0 || q_ts % vec || q_hs % vec) return WALSH_ERR_ALIGN;
-  if (B == 0 || max_q == 0 || q_rows == 0) return WALSH_OK;
+  if (B == 0 || q_rows == 0) return WALSH_OK;
+  if (max_q == 0) max_q = 1;  // (longer spans are still computed)
   return WALSH_DISPATCH_DTYPE(kv->dtype, ET, [&]() -> int {
     PrefillArgs<ET> a;
     a.pg = make_pages<ET>(kv);
