@@ -142,3 +142,23 @@ def test_prefill_bound_of_zero_still_computes_the_spans():
         out = torch.full_like(q, 7.0)
         want = ops.paged_prefill_attention(q, off, kp, vp, table, kl)
         assert torch.equal(ops.paged_prefill_attention(q, off, kp, vp, table, kl, max_q=0, out=out), want)
+
+
+@pytest.mark.parametrize("dtype", HALF + [torch.float32])
+@pytest.mark.parametrize("hq,hk,hd", [(4, 2, 16), (8, 1, 64), (2, 2, 128)])
+def test_attention_in_place_with_hidden_values_that_are_not_finite(dtype, hq, hk, hd):
+    """out may be q: rows computed again (hidden NaN and infinities) read their queries as they were."""
+    g = gen(7)
+    n = 90
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [n], hk, 16, hd, dtype))
+    for j, x in ((40, float("nan")), (77, float("inf")), (89, float("nan"))):
+        vp[int(table[0, j // 16]), :, j % 16] = x
+    q = torch.randn(n, hq, hd, generator=g).to(dtype).to(DEV)
+    off = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    want = ops.paged_prefill_attention(q, off, kp, vp, table, kl, window=20, sinks=2)
+    mine = q.clone()
+    assert ops.paged_prefill_attention(mine, off, kp, vp, table, kl, window=20, sinks=2, out=mine) is mine
+    assert torch.equal(mine.nan_to_num(9.0), want.nan_to_num(9.0)) and torch.isfinite(want[:40].float()).all()
+    one = q[:1].clone()
+    want = ops.paged_attention(one, kp, vp, table, kl, window=12)
+    assert torch.equal(ops.paged_attention(one, kp, vp, table, kl, window=12, out=one).nan_to_num(9.0), want.nan_to_num(9.0))

@@ -44,8 +44,9 @@ __device__ __forceinline__ int query_span(const PrefillArgs<T>& a, int b, int64_
 
 // One row again by one warp, over the keys it sees and no others.  A tile
 // multiplies hidden keys by a probability of 0, which is no use when the value
-// is infinite or NaN (a later token's, say): rows that come out as NaN are
-// computed once more by this, so that only what a row sees reaches it.
+// is infinite or NaN (a later token's, say): rows that come out as NaN are not
+// stored but computed once more by this, so that only what a row sees reaches it
+// (o may be q: a row of it is read before any lane stores its own part).
 template <typename T, int HD>
 __device__ __noinline__ void prefill_row_again(const PrefillArgs<T>& a, int b, int hk, const T* qp, int pos, T* op) {
   constexpr int DL = (HD + 31) / 32;  // channels per lane
@@ -83,6 +84,7 @@ __device__ __noinline__ void prefill_row_again(const PrefillArgs<T>& a, int b, i
         if (i * 32 + lane < HD) acc[i] = fmaf(pj, to_f(vb[oj + i * 32 + lane]), acc[i]);
     }
   }
+  __syncwarp();
 #pragma unroll
   for (int i = 0; i < DL; ++i)
     if (i * 32 + lane < HD) op[i * 32 + lane] = round_f<T>(l == 0.f ? 0.f : acc[i] / l);
@@ -236,17 +238,18 @@ __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArg
       for (int o = 1; o < 16; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
       const int r = ty * 4 + i;
       bool nan = false;
-      if (r < nr) {
+#pragma unroll
+      for (int d = 0; d < HD / 16; ++d) {
+        acc[i][d] = L == 0.f ? 0.f : acc[i][d] / L;
+        nan |= r < nr && acc[i][d] != acc[i][d];
+      }
+      const unsigned again = __ballot_sync(0xffffffffu, nan);
+      if (r < nr && !(again & (0xffffu << (16 * (ty & 1))))) {
         const uint32_t t = fdiv((uint32_t)(r0 + r), a.group), g = (uint32_t)(r0 + r) - t * G;
         T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + g) * HD;
 #pragma unroll
-        for (int d = 0; d < HD / 16; ++d) {
-          const float x = L == 0.f ? 0.f : acc[i][d] / L;
-          nan |= x != x;
-          op[tx + 16 * d] = round_f<T>(x);
-        }
+        for (int d = 0; d < HD / 16; ++d) op[tx + 16 * d] = round_f<T>(acc[i][d]);
       }
-      const unsigned again = __ballot_sync(0xffffffffu, nan);
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         if (again & (0xffffu << (16 * h))) {
@@ -597,20 +600,23 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_prefill_mma_kernel(const P
 #pragma unroll
         for (int o = 1; o <= 2; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
         const int r = wr0 + mt * 16 + g + 8 * h;
+        const float inv = L == 0.f ? 0.f : 1.f / L;
         bool nan = false;
-        if (r < nr) {
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+          const float u = acc[mt][i][2 * h] *= inv, w = acc[mt][i][2 * h + 1] *= inv;
+          nan |= r < nr && (u != u || w != w);
+        }
+        unsigned again = __ballot_sync(0xffffffffu, nan);
+        if (r < nr && !(again & (15u << (lane & 28)))) {
           const uint32_t x = (uint32_t)(r0 + r), t = fdiv(x, a.group), gi = x - t * G;
           T* op = a.o + ((first + t) * Hq + (int64_t)hk * G + gi) * HD;
-          const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
           for (int i = 0; i < HD / 8; ++i) {
-            const float u = acc[mt][i][2 * h] * inv, w = acc[mt][i][2 * h + 1] * inv;
-            nan |= u != u || w != w;
-            T pair[2] = {round_f<T>(u), round_f<T>(w)};
+            T pair[2] = {round_f<T>(acc[mt][i][2 * h]), round_f<T>(acc[mt][i][2 * h + 1])};
             *reinterpret_cast<uint32_t*>(op + i * 8 + 2 * t4) = *reinterpret_cast<uint32_t*>(pair);
           }
         }
-        unsigned again = __ballot_sync(0xffffffffu, nan);
         while (again) {
           const int q = (__ffs(again) - 1) >> 2;  // the lane quad of a row
           again &= ~(15u << (4 * q));
