@@ -162,3 +162,32 @@ def test_attention_in_place_with_hidden_values_that_are_not_finite(dtype, hq, hk
     one = q[:1].clone()
     want = ops.paged_attention(one, kp, vp, table, kl, window=12)
     assert torch.equal(ops.paged_attention(one, kp, vp, table, kl, window=12, out=one).nan_to_num(9.0), want.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("dtype", HALF + [torch.float32])
+@pytest.mark.parametrize("hq,hk,hd", [(1, 1, 16), (8, 1, 64), (16, 1, 32), (20, 1, 128), (8, 2, 128)])
+@pytest.mark.parametrize("n", [40, 3000])
+def test_decode_infinite_values_of_tiny_probability(dtype, hq, hk, hd, n):
+    """A value that is infinite reaches its channel although its probability,
+    e^-25, is nothing in float16; other channels stay as they are."""
+    g = gen(n + hd)
+    kp, vp, table, kl = (t.to(DEV) for t in R.make_pool(g, [n, 30], hk, 16, hd, dtype))
+    kp.zero_()
+    j = n // 2 + 3
+    page, row = int(table[0, j // 16]), j % 16
+    kp[page, :, row, 0] = -25
+    vp[page, :, row, 0], vp[page, :, row, 3] = float("inf"), float("-inf")
+    q = torch.zeros(2, hq, hd, dtype=dtype, device=DEV)
+    q[:, :, 0] = 1
+    out = ops.paged_attention(q, kp, vp, table, kl, scale=1.0)
+    assert (out[0, :, 0] == float("inf")).all() and (out[0, :, 3] == float("-inf")).all()
+    v = R.gather_keys(vp, table[0], n).double()
+    v[j] = 0                                               # e^-25 of it
+    want = (v.sum(0) / (n - 1)).repeat_interleave(hq // hk, 0)
+    a = (v.abs().sum(0) / (n - 1)).repeat_interleave(hq // hk, 0)
+    # equal probabilities: exact in any type; float32 sums of n values in at least
+    # 16 parts, the division, and one rounding of the result; e^-25 of a value below 6
+    rest = [c for c in range(hd) if c not in (0, 3)]
+    bound = torch.finfo(dtype).eps / 2 * want.abs() + 2 * (n / 16 + 64) * 2.0 ** -24 * a + 1e-10
+    assert ((out[0].double() - want).abs() <= bound)[:, rest].all()
+    assert torch.isfinite(out[1].float()).all()

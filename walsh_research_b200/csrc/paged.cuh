@@ -3,9 +3,11 @@
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <math_constants.h>
 #include <stdint.h>
 
 #include "common.cuh"
+#include "mma.cuh"
 
 namespace walsh {
 
@@ -86,6 +88,49 @@ __device__ __forceinline__ Visible visible_keys(int pos, int window, int sinks) 
   v.nsink = min(sinks, v.lo);
   v.n = v.nsink + (pos + 1 - v.lo);
   return v;
+}
+
+// One query row (qp, of the group of kv head hk) over the n keys from number beg
+// on, by one warp in float32: running maximum m (of the scores times log2 e), sum l
+// and the lane's channels i * 32 + lane of o, undivided.
+template <typename T, int HD>
+__device__ __forceinline__ void attend_row(const Pages<T>& p, int b, int hk, const T* qp, const Visible& vis, int beg,
+                                           int n, float scale_log2, float* m_out, float* l_out, float* acc) {
+  constexpr int DL = (HD + 31) / 32;  // channels per lane
+  const int lane = threadIdx.x & 31;
+  const int* trow = p.table + (int64_t)b * p.table_stride;
+  const T* kb = p.k + (int64_t)hk * p.head_stride;
+  const T* vb = p.v + (int64_t)hk * p.head_stride;
+  float m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+  for (int i = 0; i < DL; ++i) acc[i] = 0.f;
+  for (int x0 = 0; x0 < n; x0 += 32) {
+    int64_t off = -1;
+    float s = -CUDART_INF_F;
+    if (x0 + lane < n) off = key_offset(p, trow, vis.key(beg + x0 + lane));
+    if (off >= 0) {
+      float dot = 0.f;
+      for (int d = 0; d < HD; ++d) dot = fmaf(to_f(qp[d]), to_f(kb[off + d]), dot);
+      s = dot * scale_log2;
+    }
+    const float mn = fmaxf(m, warp_max(s)), sub = mn == -CUDART_INF_F ? 0.f : mn;
+    const float corr = ex2_f32(m - sub), w = off >= 0 ? ex2_f32(s - sub) : 0.f;
+    m = mn;
+    l = l * corr + warp_sum(w);
+#pragma unroll
+    for (int i = 0; i < DL; ++i) acc[i] *= corr;
+    unsigned todo = __ballot_sync(0xffffffffu, off >= 0);
+    while (todo) {
+      const int j = __ffs(todo) - 1;
+      todo &= todo - 1;
+      const float wj = __shfl_sync(0xffffffffu, w, j);
+      const int64_t oj = __shfl_sync(0xffffffffu, off, j);
+#pragma unroll
+      for (int i = 0; i < DL; ++i)
+        if (i * 32 + lane < HD) acc[i] = fmaf(wj, to_f(vb[oj + i * 32 + lane]), acc[i]);
+    }
+  }
+  *m_out = m, *l_out = l;
 }
 
 // Host: fills Pages<T> from the C description.

@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
 // (bf16) to 22 bits: with up to 8 heads the rows 8 - 15 carry the second term at
 // no cost, with 9 to 16 heads it takes MMAs of its own (64 x 4000 keys,
 // 64 heads on 4 of 64 channels 54 us both ways, 48 on 4 of 32 36 -> 38.5, 32 on 2
-// of 128 60 -> 66.5).
+// of 128 60 -> 66.5).  Rows that come out as NaN are computed again.
 // ---------------------------------------------------------------------------
 template <int HD>
 __device__ __forceinline__ int dec_swz(int r, int c) {  // 16-byte piece c of row r: its place in the row
@@ -239,9 +239,27 @@ template <typename T> __device__ __forceinline__ uint32_t dec_pack(float lo, flo
 template <> __device__ __forceinline__ uint32_t dec_pack<__half>(float lo, float hi) { return pack_f16(lo, hi); }
 template <> __device__ __forceinline__ uint32_t dec_pack<__nv_bfloat16>(float lo, float hi) { return pack_bf16(lo, hi); }
 
+// One row of a warp's slice again in float32, over the n keys from number beg on:
+// a probability that is nothing in 16 bits makes NaN of an infinite value, which
+// float32 keeps infinite.  (m, l, o) go where the warps are joined.  (The kernel's
+// arguments are a __grid_constant__: passed on by reference they would be copied to
+// local memory, 256 x 1024 keys 56.5 us against 50.7.)
+template <typename T, int HD>
+__device__ __noinline__ void decode_row_again(const DecodeArgs<T>& a, const Visible vis, int b, int hk, int h, int beg,
+                                              int n, float* jo, float* jm) {
+  constexpr int DL = (HD + 31) / 32;
+  const int lane = threadIdx.x & 31;
+  float m, l, acc[DL];
+  attend_row<T, HD>(a.pg, b, hk, a.q + (int64_t)b * a.q_bs + (int64_t)h * a.q_hs, vis, beg, n, a.scale_log2, &m, &l, acc);
+#pragma unroll
+  for (int i = 0; i < DL; ++i)
+    if (i * 32 + lane < HD) jo[i * 32 + lane] = acc[i];
+  if (lane == 0) jm[0] = m, jm[1] = l;
+}
+
 // RH: halves of the 16 MMA rows in use (1: up to 8 heads, 2: up to 16)
 template <typename T, int HD, int RH, int W, int KT, int NS, bool CL>
-__global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeArgs<T> a) {
+__global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const __grid_constant__ DecodeArgs<T> a) {
   constexpr int CH = HD / 8, STAGE = 2 * KT * HD, RI = 32 / CH;  // RI: rows per copy instruction
   constexpr int OL = HD + 4;                                     // padded row of the join buffer
   extern __shared__ __align__(16) unsigned char smb[];
@@ -278,7 +296,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
   };
   // bit r: row r of the stage holds a key
   uint32_t okq[NS][RL];
-  auto load = [&](int st, int buf) {
+  auto load = [&](int buf) {
     T* dst = ring + buf * STAGE;
 #pragma unroll
     for (int i = 0; i < KT / RI; ++i) {
@@ -288,7 +306,6 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
       cp_async16(dst + at, kb + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
       cp_async16(dst + KT * HD + at, vb + (o < 0 ? 0 : o), o < 0 ? 0 : 16);
     }
-    (void)st;
   };
 #pragma unroll
   for (int i = 0; i < NS; ++i)
@@ -298,7 +315,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
     lookup(0);
 #pragma unroll
     for (int s = 0; s < NS - 1; ++s) {
-      if (s < nst) load(s, s);
+      if (s < nst) load(s);
 #pragma unroll
       for (int j = 0; j < RL; ++j) okq[s][j] = __ballot_sync(0xffffffffu, s < nst && off[j] >= 0);
       cp_async_commit();
@@ -399,7 +416,7 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
       // the buffer that the stage before this one left takes stage st + NS - 1
       constexpr int NB = NS - 1;
       const int nb = (u + NB) % NS;
-      if (st + NB < nst) load(st + NB, nb);
+      if (st + NB < nst) load(nb);
 #pragma unroll
       for (int j = 0; j < RL; ++j) okq[nb][j] = __ballot_sync(0xffffffffu, st + NB < nst && off[j] >= 0);
       cp_async_commit();
@@ -430,7 +447,12 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
 #pragma unroll
   for (int h = 0; h < RH; ++h) {
     const int r = g + 8 * h;
-    if (r < ng) {
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < HD / 8; ++i)
+      nan |= r < ng && (acc[i][2 * h] != acc[i][2 * h] || acc[i][2 * h + 1] != acc[i][2 * h + 1]);
+    unsigned again = __ballot_sync(0xffffffffu, nan);
+    if (r < ng && !(again & (15u << (lane & 28)))) {
       float* row = jo + (warp * 8 * RH + r) * OL;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i)
@@ -439,6 +461,11 @@ __global__ void __launch_bounds__(W * 32) paged_decode_mma_kernel(const DecodeAr
         jm[(warp * 8 * RH + r) * 2] = m[h] * sc;
         jm[(warp * 8 * RH + r) * 2 + 1] = l[h];
       }
+    }
+    while (again) {
+      const int q = (__ffs(again) - 1) >> 2, at = warp * 8 * RH + q + 8 * h;  // the lane quad of a row
+      again &= ~(15u << (4 * q));
+      decode_row_again<T, HD>(a, vis, b, hk, h0 + q + 8 * h, wbeg, n, jo + at * OL, jm + at * 2);
     }
   }
   if constexpr (W > 1) __syncthreads();

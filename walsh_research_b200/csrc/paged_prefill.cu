@@ -49,41 +49,11 @@ __device__ __forceinline__ int query_span(const PrefillArgs<T>& a, int b, int64_
 // (o may be q: a row of it is read before any lane stores its own part).
 template <typename T, int HD>
 __device__ __noinline__ void prefill_row_again(const PrefillArgs<T>& a, int b, int hk, const T* qp, int pos, T* op) {
-  constexpr int DL = (HD + 31) / 32;  // channels per lane
+  constexpr int DL = (HD + 31) / 32;
   const int lane = threadIdx.x & 31;
-  const int* trow = a.pg.table + (int64_t)b * a.pg.table_stride;
-  const T* kb = a.pg.k + (int64_t)hk * a.pg.head_stride;
-  const T* vb = a.pg.v + (int64_t)hk * a.pg.head_stride;
   const Visible vis = visible_keys(pos, a.pg.window, a.pg.sinks);
-  float m = -CUDART_INF_F, l = 0.f, acc[DL];
-#pragma unroll
-  for (int i = 0; i < DL; ++i) acc[i] = 0.f;
-  for (int x0 = 0; x0 < vis.n; x0 += 32) {
-    int64_t off = -1;
-    float s = -CUDART_INF_F;
-    if (x0 + lane < vis.n) off = key_offset(a.pg, trow, vis.key(x0 + lane));
-    if (off >= 0) {
-      float dot = 0.f;
-      for (int d = 0; d < HD; ++d) dot = fmaf(to_f(qp[d]), to_f(kb[off + d]), dot);
-      s = dot * a.scale_log2;
-    }
-    const float mn = fmaxf(m, warp_max(s)), sub = mn == -CUDART_INF_F ? 0.f : mn;
-    const float corr = ex2_f32(m - sub), p = off >= 0 ? ex2_f32(s - sub) : 0.f;
-    m = mn;
-    l = l * corr + warp_sum(p);
-#pragma unroll
-    for (int i = 0; i < DL; ++i) acc[i] *= corr;
-    unsigned todo = __ballot_sync(0xffffffffu, off >= 0);
-    while (todo) {
-      const int j = __ffs(todo) - 1;
-      todo &= todo - 1;
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-      const int64_t oj = __shfl_sync(0xffffffffu, off, j);
-#pragma unroll
-      for (int i = 0; i < DL; ++i)
-        if (i * 32 + lane < HD) acc[i] = fmaf(pj, to_f(vb[oj + i * 32 + lane]), acc[i]);
-    }
-  }
+  float m, l, acc[DL];
+  attend_row<T, HD>(a.pg, b, hk, qp, vis, 0, vis.n, a.scale_log2, &m, &l, acc);
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < DL; ++i)
