@@ -133,3 +133,19 @@ def test_a_batch_of_a_removed_sequence_is_refused_although_its_row_is_in_use_aga
     new.begin(2)
     new.increment(2)
     assert c.lengths(b) == [2]
+
+
+def test_a_forward_that_is_refused_reserves_nothing():
+    """Positions past the rotation table, a batch of another size or type, start positions."""
+    from walsh_research_b200.model import mHCWalsh
+    c = make()
+    (a,) = c.add()
+    c.select([a]).begin(6)
+    c.select([a]).increment(6)
+    batch = c.select([a])
+    for args in ((1, 7, 0, torch.float16, 12), (2, 7, 0, torch.float16, 24), (1, 7, 0, torch.float32, 24),
+                 (1, 7, 3, torch.float16, 24), (1, 19, 0, torch.float16, 30)):
+        with pytest.raises(ValueError):
+            mHCWalsh._begin_paged(batch, *args)
+        assert c.free_pages == 8 and c.lengths([a]) == [6]
+    assert mHCWalsh._begin_paged(batch, 1, 7, 0, torch.float16, 13).max_len == 13 and c.free_pages == 6

@@ -488,10 +488,10 @@ class mHCWalsh(nn.Module):
                              f"{B} in {idt}")
         if start_pos != 0:
             raise ValueError("start_pos does not apply to a paged cache: every sequence continues at its own length")
-        step = batch.begin(T)
-        if step.max_len > n_pos:
-            raise ValueError(f"position {step.max_len - 1} is beyond the {n_pos} of the rotation table")
-        return step
+        last = batch.longest + T - 1
+        if last >= n_pos:
+            raise ValueError(f"position {last} is beyond the {n_pos} of the rotation table")
+        return batch.begin(T)
 
     # Batched decode can run the batch in `decode_streams` parts, each on its
     # own CUDA stream: sequences share nothing inside the layer stack, so one

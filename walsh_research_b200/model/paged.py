@@ -126,6 +126,10 @@ class PagedBatch:
         self.batch_size, self.dtype = len(ids), cache.dtype
         self._removed = cache._removed[ids]
 
+    @property
+    def longest(self) -> int:
+        return int(self.cache._len[self.ids].max(initial=0))
+
     def _check(self):
         if (self.cache._removed[self.ids] != self._removed).any():
             raise ValueError("some of the batch's sequences were removed since it was selected")
