@@ -489,7 +489,7 @@ class mHCWalsh(nn.Module):
         if start_pos != 0:
             raise ValueError("start_pos does not apply to a paged cache: every sequence continues at its own length")
         last = batch.longest + T - 1
-        if last >= n_pos:
+        if n_pos <= last < batch.cache.max_seq_len:  # (longer than the cache takes: begin's own error)
             raise ValueError(f"position {last} is beyond the {n_pos} of the rotation table")
         return batch.begin(T)
 
