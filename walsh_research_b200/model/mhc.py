@@ -628,7 +628,8 @@ class mHCWalsh(nn.Module):
         step when given) or when ``max_seq_len`` (default block_size, at most
         the rotation table's 2 block_size) tokens are cached; of a longer prompt
         the last ``max_seq_len`` ids are read.  ``window`` and ``sinks`` as in
-        PagedKVCache."""
+        PagedKVCache.  Waits for the last step, whose kernels may have met an
+        index out of range (IndexError)."""
         limit = self.config.block_size if max_seq_len is None else int(max_seq_len)
         if not 0 < limit <= self.freqs_cis.shape[0]:
             raise ValueError(f"max_seq_len must be in 1 .. {self.freqs_cis.shape[0]}, got {limit}")
@@ -674,6 +675,7 @@ class mHCWalsh(nn.Module):
             nxt = draw(out[:, -1])
             for i, t in zip(live, nxt[:, 0].unbind()):
                 tokens[i].append(t)
+        cache.check()
         return [torch.cat((p, torch.stack(t).to(p.dtype))) for p, t in zip(given, tokens)]
 
     @torch.no_grad()
