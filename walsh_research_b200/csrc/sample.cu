@@ -1304,12 +1304,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
 
 // Parts up to this size are staged: two CTAs then share an SM.
 constexpr int kStageBytes = 99 * 1024;
+static_assert(kStageBytes >= kList * 16, "a list fits where a part does");
 
 template <typename T, int CS, bool STAGE>
 static int launch_sample_as(const SampleArgs<T>& a, int part, cudaStream_t s) {
   const int smem = max(STAGE ? part : 0, kList * 16);  // a list takes the part's place, with its weights
   auto* kern = sample_kernel<T, CS, STAGE>;
-  if (STAGE && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+  // the most of any call: the limit holds for the whole process, and another thread's call may come between this and the launch
+  if (STAGE && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kStageBytes) != cudaSuccess)
     return launch_status();
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)a.rows * CS);
