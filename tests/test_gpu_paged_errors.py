@@ -25,3 +25,11 @@ def test_generate_batch_raises_what_a_kernel_reported(monkeypatch):
         m.generate_batch(prompts, 3, top_k=1)
     monkeypatch.undo()
     assert torch.equal(m.generate_batch(prompts, 3, top_k=1)[0][:3], prompts[0])
+
+
+def test_a_cache_stays_on_the_device_it_was_made_on():
+    """"cuda" is the device that is current at construction, not at each call."""
+    c = paged.PagedKVCache(1, 4, 4, 2, 16, "cuda", max_seqs=1, max_seq_len=8)
+    assert c.device == c.k_pages[0].device and c.device.index is not None
+    step = c.select(c.add()).begin(3)
+    assert step.slots.device == step.page_table.device == c.k_pages[0].device

@@ -35,12 +35,12 @@ class PagedKVCache:
             raise ValueError("a paged cache needs pages, a page size, sequences and a length, and no negative window")
         self.n_layers, self.n_pages, self.page_size = n_layers, n_pages, page_size
         self.n_head, self.head_dim, self.dtype = n_head, head_dim, dtype
-        self.device = torch.device(device)
         self.max_seq_len, self.window, self.sinks = max_seq_len, window, sinks
         shape = (n_pages, n_head, page_size, head_dim)
         self.k_pages: List[torch.Tensor] = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(n_layers)]
         self.v_pages: List[torch.Tensor] = [torch.zeros(shape, device=device, dtype=dtype) for _ in range(n_layers)]
         self.err = torch.zeros(1, dtype=torch.int32, device=device)
+        self.device = self.err.device  # with its index: "cuda" may be another one by the next call
         self._free = list(range(n_pages - 1, -1, -1))
         self._rows = list(range(max_seqs - 1, -1, -1))
         self._table = np.full((max_seqs, -(-max_seq_len // page_size)), -1, dtype=np.int32)
