@@ -14,8 +14,8 @@
 // of their CTAs; more leave (m, l, o) in the workspace for paged_join_kernel.
 // Both combine them in order of the ranges, so results do not depend on timing.
 // Measured (of the HBM copy rate): 256 sequences of up to 1024 keys, 32 heads of
-// 16 channels, 49.6 us (0.84); 12 of up to 32768, 8 shared heads of 64, 82 us
-// (0.90); 48 under a window of 1000, 64 heads of 32, 59.8 us (0.93).
+// 16 channels, 50.8 us (0.82); 12 of up to 32768, 8 shared heads of 64, 81 us
+// (0.91); 48 under a window of 1000, 64 heads of 32, 61.4 us (0.90).
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -226,8 +226,8 @@ __global__ void __launch_bounds__(W * 32) paged_decode_vec_kernel(const DecodeAr
 // P enters as two 16-bit terms, rounded and what that left over, so it keeps 16
 // (bf16) to 22 bits: with up to 8 heads the rows 8 - 15 carry the second term at
 // no cost, with 9 to 16 heads it takes MMAs of its own (64 x 4000 keys,
-// 64 heads on 4 of 64 channels 54 us both ways, 48 on 4 of 32 36 -> 38.5, 32 on 2
-// of 128 60 -> 66.5).  Rows that come out as NaN are computed again.
+// 64 heads on 4 of 64 channels 54 -> 56 us, 64 on 4 of 16 17 -> 19.5, 32 on 2 of 128
+// 60 -> 64.5).  Rows that come out as NaN are computed again.
 // ---------------------------------------------------------------------------
 template <int HD>
 __device__ __forceinline__ int dec_swz(int r, int c) {  // 16-byte piece c of row r: its place in the row
@@ -580,8 +580,8 @@ static int launch_decode_mma(const DecodeArgs<T>& a, int64_t ctas, cudaStream_t 
   // 8 KB of K and V per stage (4 KB for 16 channels)
   constexpr int KT = HD <= 32 ? 64 : HD == 64 ? 32 : 16;
   // two stages in flight and the warps' number cover the latency; the smaller
-  // ring leaves room for more warps (256 x 1024 keys, 16 channels: 2 stages
-  // 49.4 us, 3 50.7, 4 58.4; 12 x 32768, 64 channels: 82.3, 89.4, 94.8)
+  // ring leaves room for more warps (256 x up to 1024 keys, 16 channels: 2 stages
+  // 50.7 us, 3 51.8, 4 61.7; 12 x up to 32768, 64 channels: 81.2, 84.1, 112)
   constexpr int NS = 2;
   constexpr int ring = W * NS * 2 * KT * HD * 2, join = (W * 8 * RH * (HD + 4 + 2) + (CL ? 8 * RH * (HD + 2) : 0)) * 4;
   return launch_ctas(paged_decode_mma_kernel<T, HD, RH, W, KT, NS, CL>, a, ctas, W * 32, ring > join ? ring : join,
@@ -616,9 +616,12 @@ struct DecodePlan {
 };
 constexpr int64_t kRangeBytes = 256 << 10;  // longer ranges are cut for the balance between sequences
 constexpr int64_t kRangeLeast = 32 << 10;   // shorter ones cost more to join than they save
-// from so many units up to so many bytes each, a warp per unit: 256 x 1024 keys
-// (8192 units of 64 KB) 49.6 us against 58 with four, 100 x 200 keys 8.2 against
-// 14.3; but 64 x 4000 (2048 of 256 KB) 71 against 48, 30 x 500 (960) 9.0 against 7.7
+// from so many units up to so many bytes each, a warp per unit.  32 heads of 16,
+// lengths up to the one named: 256 x 1024 keys (8192 units of 64 KB) 50.6 us against
+// 58.2 with four, 100 x 200 8.8 against 13.9, 100 x 600 17.6 against 20.5; about
+// even at 100 x 1200 (77 KB) 28.8 and 29.1, 100 x 1500 (96 KB) 33.6 and 32.8, 64 x
+// 1024 (2048 units) 21.0 and 19.3, 62 x 1024 19.9 and 18.7; all of one length they
+// pass earlier, 100 x 1200 50.5 and 44.2, 100 x 2000 79 and 65
 constexpr int kSingleUnits = 2000;
 constexpr int64_t kSingleBytes = 100000;
 static DecodePlan decode_plan(const walsh_paged_kv* kv, int B, int q_heads, int max_len) {
@@ -631,10 +634,13 @@ static DecodePlan decode_plan(const walsh_paged_kv* kv, int B, int q_heads, int 
   const int64_t bytes = n * 2 * kv->head_dim * (kv->dtype == WALSH_F32 ? 4 : 2);  // of a unit
   // one warp per unit when there are enough units for the GPU, or nothing to share
   p.warps = (units >= kSingleUnits && bytes <= kSingleBytes) || bytes < (8 << 10) ? 1 : 4;
-  // CTAs of four warps that fit on the GPU together: no range waits for another
-  // (2 x 20000 keys of 64 channels, 3 per SM 20.3 us, 4 24.2; 16 x 8000 of 32, 3
-  // 14.2, 5 11.8; 4 x 4000 of 16, 3 10.3, 4 9.1, 5 (too many for clusters) 11.1)
-  const int ctas = 148 * (kv->head_dim == 16 ? 4 : kv->head_dim == 32 ? 5 : 3);
+  // CTAs of four warps that run together, so that no range waits for another: their
+  // rings of 64 KB leave room for 3 on an SM (2 x 20000 keys, 32 on 8 heads of 64
+  // channels, 3 per SM 21.1 us, 4 25.1, 5 25.0; 32 on 4 of 32, 3 11.4, 4 15.5, 5
+  // 16.0; but 37 x 4000 of these 27.4 against 23.1 with 5, whose ranges are too many
+  // for clusters); with 16 channels and 32 KB 4 do best (4 x 4000, 32 heads, 3 11.5,
+  // 4 10.2, 5 12.7)
+  const int ctas = 148 * (kv->head_dim == 16 ? 4 : 3);
   int64_t split = units > 0 ? ctas / units : 1;
   if (split < bytes / kRangeBytes) split = bytes / kRangeBytes;
   split = min64(split, bytes / kRangeLeast);
@@ -642,9 +648,11 @@ static DecodePlan decode_plan(const walsh_paged_kv* kv, int B, int q_heads, int 
   p.nsplit = p.warps == 1 || split < 1 ? 1 : (int)split;
   p.chunk = (int)((n + p.nsplit - 1) / p.nsplit);
   if (p.chunk < 1) p.chunk = 1;
-  // the clusters' one launch saves the joining kernel and its scratch (1 x 4099
-  // keys 7.8 -> 6.6 us) while all of them run at once; beyond that CTAs that wait
-  // for their cluster keep others out (12 x 32768 keys: 95 us against 84)
+  // the clusters' one launch saves the joining kernel and its scratch (1 x 4099 keys
+  // of 32 heads of 16 8.0 -> 7.1 us, 4 x 4000 11.6 -> 10.2; but 8 x 8000, 32 on 8 of
+  // 64, 31.4 -> 34.2, in clusters of 6) while all of them run at once; beyond that
+  // CTAs that wait for their cluster keep others out (48 x 4000, 16 on 2 of 128: 44.9
+  // us against 43.0)
   p.cluster = p.nsplit > 1 && p.nsplit <= 8 && units * p.nsplit <= 148 * 4;
   return p;
 }
