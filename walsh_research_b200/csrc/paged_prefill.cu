@@ -64,6 +64,7 @@ __device__ __noinline__ void prefill_row_again(const PrefillArgs<T>& a, int b, i
 // rows (scores, softmax and accumulator), so only K and V tiles need barriers.
 // Shared-memory loads bound it: a thread's KT / 16 x 4 scores and its four rows of P V
 // read operands as float4 (KT = 64; 32 for 128 channels, whose tiles fill the memory).
+// 4 x 1000 tokens: 64 heads of 32 753 us, 16 on 2 heads of 128 673.
 template <typename T, int HD, int KT>
 __global__ void __launch_bounds__(256) paged_prefill_vec_kernel(const PrefillArgs<T> a) {
   constexpr int QT = 64, KJ = KT / 16, LD = HD + 4, LP = KT + 4, VEC = 16 / (int)sizeof(T), CH = HD / VEC;

@@ -19,8 +19,8 @@
 // Bytes are the floor (256 rows of 50257 float32 logits: 7.9 us), instructions
 // the bound: about 140 thousand warp instructions per row with top-p (one pass
 // for the largest logit, one for the total and a histogram, one for the masses
-// above the border) run at 60 % of the issue slots, 73 us; 1 row with top-k 50
-// takes 12.5 us, the barriers and dependent steps of a row.
+// above the border) run at 60 % of the issue slots, 72.5 us; 1 row with top-k 50
+// takes 12.3 us, the barriers and dependent steps of a row.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 

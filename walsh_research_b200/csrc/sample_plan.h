@@ -11,9 +11,11 @@ constexpr int kSampleThreads = 512, kSampleWarps = kSampleThreads / 32;
 
 // CTAs per row: one when the rows alone occupy every SM (the barriers and scalar
 // steps of a row are paid per CTA), else more while a thread still has eight
-// tokens.  Rows of 50257 tokens: 64 in float32 with top-p 26.5 us on 4 CTAs each
-// (53 on 8); 256 in float32 72.8 us on one, read again from L2, 70.7 on two,
-// held; with top-k 50 31.9 and 43.2 us; 256 in bf16 56.4 us on one, held.
+// tokens.  Rows of 50257 tokens: 64 in float32 with top-p 27.4 us on 4 CTAs each (47
+// on one, 27.2 on two, 53 on 8), with top-k 50 21.2 (21.1, 16.2, 31.6); 256 in
+// float32 with top-p 73.9 us on one, read again from L2, 70.3 on two, held; with
+// top-k 50 31.7 and 43.0, plain 46 and 50; 256 in bf16 with top-p 56.9 on one, held,
+// 70.8 on two.
 inline int sample_cluster(int64_t rows, int vocab) {
   int cs = 1;
   while (cs < 8 && rows * cs < 148 && vocab / cs > kSampleThreads * 8) cs *= 2;
